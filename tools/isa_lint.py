@@ -26,7 +26,8 @@ import tempfile
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "faiss_amd", "csrc")
 HIPCC = "/opt/rocm/bin/hipcc"
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC"]
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fPIC", "-Xclang", "-target-feature",
+         "-Xclang", "-packed-fp32-ops"]
 
 PROBE = r"""
 #include <hip/hip_runtime.h>
