@@ -180,6 +180,16 @@ def load_library():
         "faiss_amd_GpuIndexIVF_search_preassigned_with_params": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, vp]),
         "faiss_amd_GpuIndexIVF_stored_vectors": (i32, [vp, P(i64)]),
         "faiss_amd_GpuIndexIVF_arena_stats": (i32, [vp, P(i64), P(i64), P(i64)]),
+        # faiss_amd/decoding.py
+        "faiss_amd_plan_blocks": (i32, [vp, vp, vp]),
+        "faiss_amd_PagedCache_add": (i32, [vp, vp, vp, vp]),
+        "faiss_amd_PagedCache_reconstruct": (i32, [vp, vp, i32, vp, i32, vp, vp, vp]),
+        "faiss_amd_PagedCache_attend": (i32, [vp, vp, vp, vp]),
+        "faiss_amd_PagedCache_attend_workspace": (i32, [vp, vp, vp, P(sz)]),
+        "faiss_amd_beam_select": (i32, [vp, vp, vp]),
+        "faiss_amd_beam_select_workspace": (i32, [vp, vp, P(sz)]),
+        "faiss_amd_reorder_beams": (i32, [vp, i32, vp, vp, i32, i32, i32, vp]),
+        "faiss_amd_fork_blocks": (i32, [vp, i32, vp, vp, vp]),
     }
     for name, (res, args) in protos.items():
         fn = getattr(lib, name)  # AttributeError => the library does not export the symbol

@@ -8,6 +8,7 @@
 #include <string>
 #include "index.h"
 #include "kernels.h"
+#include "decoding.h"
 
 using namespace faiss_amd;
 
@@ -1076,6 +1077,61 @@ int faiss_amd_GpuIndexIVF_list_major_rule(const FaissAmdIndex* index, int64_t n,
     FA_TRY
     FA_THROW_IF_NOT_MSG(p_output, "null output");
     *p_output = as<GpuIndexIVF>(const_cast<FaissAmdIndex*>(index), "GpuIndexIVF")->list_major_rule(n, nprobe, k, false) ? 1 : 0;
+    FA_CATCH
+}
+
+// ---- operators of a decoding program (decoding.h)
+// (sizes and types are checked before the handle, memory behind it)
+static const GpuResources* G(const FaissAmdGpuResources* r) { return r ? r->res.get() : nullptr; }
+int faiss_amd_plan_blocks(FaissAmdGpuResources* res, const FaissAmdPlanBlocksParams* args, void* stream) {
+    FA_TRY
+    plan_blocks(G(res), args, (hipStream_t)stream);
+    FA_CATCH
+}
+int faiss_amd_PagedCache_add(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdCacheAddParams* args, void* stream) {
+    FA_TRY
+    cache_add(G(res), cache, args, (hipStream_t)stream);
+    FA_CATCH
+}
+int faiss_amd_PagedCache_reconstruct(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, int n, const int* blocks, int type,
+                                     void* keys, void* values, void* stream) {
+    FA_TRY
+    cache_reconstruct(G(res), cache, n, blocks, type, keys, values, (hipStream_t)stream);
+    FA_CATCH
+}
+int faiss_amd_PagedCache_attend(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdAttendParams* args, void* stream) {
+    FA_TRY
+    cache_attend(G(res), cache, args, (hipStream_t)stream, nullptr);
+    FA_CATCH
+}
+int faiss_amd_PagedCache_attend_workspace(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdAttendParams* args,
+                                          size_t* p_bytes) {
+    FA_TRY
+    FA_THROW_IF_NOT_MSG(p_bytes, "null output");
+    cache_attend(G(res), cache, args, nullptr, p_bytes);
+    FA_CATCH
+}
+int faiss_amd_beam_select(FaissAmdGpuResources* res, const FaissAmdBeamSelectParams* args, void* stream) {
+    FA_TRY
+    beam_select(G(res), args, (hipStream_t)stream, nullptr);
+    FA_CATCH
+}
+int faiss_amd_beam_select_workspace(FaissAmdGpuResources* res, const FaissAmdBeamSelectParams* args, size_t* p_bytes) {
+    FA_TRY
+    FA_THROW_IF_NOT_MSG(p_bytes, "null output");
+    beam_select(G(res), args, nullptr, p_bytes);
+    FA_CATCH
+}
+int faiss_amd_reorder_beams(FaissAmdGpuResources* res, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams,
+                            int keep, void* stream) {
+    FA_TRY
+    reorder_beams(G(res), n, states, parents, batch, beams, keep, (hipStream_t)stream);
+    FA_CATCH
+}
+int faiss_amd_fork_blocks(FaissAmdGpuResources* res, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* args,
+                          void* stream) {
+    FA_TRY
+    fork_blocks(G(res), n, caches, args, (hipStream_t)stream);
     FA_CATCH
 }
 

@@ -1,0 +1,836 @@
+// faiss_amd/csrc/decoding_kernels.hip -- the operators around the attention over a paged cache (decoding.h): block tables and slot
+// maps, adding and reading back tokens, beam selection, reordering by parent.
+#include "decoding.h"
+#include <algorithm>
+
+namespace faiss_amd {
+namespace {
+
+typedef unsigned long long u64;
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ int lane64() {
+    return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+}
+
+// ================================================================================================ block tables and slot maps
+// Requests are served in order.  Request b needs take_b = blocks(new) - blocks(old) more blocks (or returns that many); it is
+// granted if the blocks and the slots that the requests up to b ask for together are there.  Both sums only grow with b, so
+// the granted requests that add tokens are a prefix of those that ask, and where a request's blocks and slots begin is an
+// exclusive prefix sum: one pass.  Free blocks wait in a ring: taken from its front, returned behind its end -- the two ranges
+// cannot meet (all blocks together fit the ring), so nothing has to be ordered between requests.
+constexpr int kPlanThreads = 1024;
+
+struct PlanScratch { // per request
+    int *oldLen, *newLen, *takeStart, *giveStart, *head; // head: {front, count}
+};
+__host__ __device__ inline PlanScratch plan_scratch(int* p, int batch) {
+    return {p, p + batch, p + 2 * batch, p + 3 * batch, p + 4 * batch};
+}
+
+// inclusive sums over the workgroup of two non-negative 64-bit values; every thread calls it
+__device__ __forceinline__ void wg_scan2(u64& x, u64& y, u64 (*part)[2]) {
+    const int lane = lane64(), wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const u64 a = __shfl_up(x, o, 64), b = __shfl_up(y, o, 64);
+        if (lane >= o) {
+            x += a;
+            y += b;
+        }
+    }
+    __syncthreads();
+    if (lane == 63) {
+        part[wave][0] = x;
+        part[wave][1] = y;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        x += part[w][0];
+        y += part[w][1];
+    }
+}
+
+__device__ __forceinline__ int ring_at(int head, u64 i, int n) { // (head + i) mod n, i < 2 n
+    u64 p = (u64)head + i;
+    while (p >= (u64)n) p -= n;
+    return (int)p;
+}
+
+// table entries that request b gains and ring entries that it returns; thread `tid` of `nt`
+__device__ __forceinline__ void plan_fill_blocks(const PlanArgs& a, const PlanScratch& s, int b, int tid, int nt) {
+    if (!a.granted[b]) return;
+    const int bs = a.blockSize;
+    const int have = (s.oldLen[b] + bs - 1) / bs, want = (s.newLen[b] + bs - 1) / bs;
+    const int head = s.head[0], count = s.head[1];
+    int* row = a.table + (int64_t)b * a.tableStride;
+    int* own = a.owned ? a.owned + (int64_t)b * a.ownedStride : nullptr;
+    for (int i = have + tid; i < want; i += nt) {
+        const int p = a.ring[ring_at(head, (u64)s.takeStart[b] + (i - have), a.numBlocks)];
+        row[i] = p;
+        if (own) own[i] = p;
+    }
+    for (int i = want + tid; i < have; i += nt)
+        a.ring[ring_at(head, (u64)count + s.giveStart[b] + (i - want), a.numBlocks)] = own ? own[i] : row[i];
+}
+
+// slot of the t-th new token of the call
+__device__ __forceinline__ int plan_slot(const PlanArgs& a, const PlanScratch& s, int t) {
+    if (t >= a.queryOffsets[a.batch]) return -1;
+    int lo = 0, hi = a.batch; // last request that starts at or before t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a.queryOffsets[mid] <= t)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    const int bs = a.blockSize;
+    const int pos = s.oldLen[lo] + (t - a.queryOffsets[lo]), col = pos / bs, have = (s.oldLen[lo] + bs - 1) / bs;
+    const int p = col >= have ? a.ring[ring_at(s.head[0], (u64)s.takeStart[lo] + (col - have), a.numBlocks)]
+                              : a.table[(int64_t)lo * a.tableStride + col];
+    return (unsigned)p < (unsigned)a.numBlocks ? p * bs + (pos - col * bs) : -1;
+}
+
+// ALL: table and slots too, for calls of few tokens -- one workgroup and one launch
+template <bool ALL>
+__global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(PlanArgs a) {
+    __shared__ u64 part[kPlanThreads / 64][2];
+    __shared__ u64 tot[2];
+    const PlanScratch s = plan_scratch(a.scratch, a.batch);
+    const int bs = a.blockSize;
+    const long long cap = (long long)a.cols * bs;
+    long long h0 = a.state[0] % a.numBlocks;
+    if (h0 < 0) h0 += a.numBlocks;
+    const long long count = min(max((long long)a.state[1], 0ll), (long long)a.numBlocks);
+    u64 takeBase = 0, tokBase = 0, giveBase = 0, taken = 0, placed = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += kPlanThreads) {
+        const int b = b0 + threadIdx.x;
+        int oldLen = 0, newLen = 0, need = 0, tok = 0;
+        bool ok = false;
+        if (b < a.batch) {
+            oldLen = a.lengths[b];
+            newLen = a.newLengths[b];
+            ok = oldLen >= 0 && newLen >= 0 && oldLen <= cap && newLen <= cap;
+            if (ok) {
+                need = (int)(((long long)newLen + bs - 1) / bs) - (int)(((long long)oldLen + bs - 1) / bs);
+                tok = max(newLen - oldLen, 0);
+            }
+        }
+        u64 ct = need > 0 ? need : 0, cn = tok;
+        wg_scan2(ct, cn, part);
+        ct += takeBase;
+        cn += tokBase;
+        const bool granted = ok && (tok == 0 || (ct <= (u64)count && cn <= (u64)a.maxTokens));
+        // totals of the granted requests: sums up to the last one that adds
+        u64 give = granted && need < 0 ? -need : 0, dummy = 0;
+        const u64 ownGive = give;
+        __syncthreads();
+        if (threadIdx.x == 0) tot[0] = tot[1] = 0;
+        wg_scan2(give, dummy, part); // (its barriers order the reset)
+        if (granted && tok > 0) {
+            atomicMax(&tot[0], ct);
+            atomicMax(&tot[1], cn);
+        }
+        __syncthreads();
+        taken = max(taken, tot[0]);
+        placed = max(placed, tot[1]);
+        if (b < a.batch) {
+            s.oldLen[b] = oldLen;
+            s.newLen[b] = newLen;
+            s.takeStart[b] = (int)min(ct - (need > 0 ? need : 0), (u64)INT32_MAX);
+            s.giveStart[b] = (int)min(giveBase + give - ownGive, (u64)INT32_MAX);
+            a.granted[b] = granted;
+            a.lengthsOut[b] = granted ? newLen : oldLen;
+            // (a refused request starts where the granted ones end: it has no tokens)
+            a.queryOffsets[b] = (int)min(cn - tok, placed);
+        }
+        // running totals: the last thread's sums
+        __syncthreads();
+        if (threadIdx.x == kPlanThreads - 1) {
+            part[0][0] = ct;
+            part[0][1] = cn;
+            part[1][0] = giveBase + give;
+        }
+        __syncthreads();
+        takeBase = part[0][0];
+        tokBase = part[0][1];
+        giveBase = part[1][0];
+    }
+    if (threadIdx.x == 0) {
+        s.head[0] = (int)h0;
+        s.head[1] = (int)count;
+        a.queryOffsets[a.batch] = (int)placed;
+        a.stateOut[0] = ring_at((int)h0, taken, a.numBlocks);
+        a.stateOut[1] = min(count - (long long)taken + (long long)giveBase, (long long)a.numBlocks);
+    }
+    if (!ALL) return;
+    __syncthreads();
+    for (int b = threadIdx.x >> 6; b < a.batch; b += kPlanThreads / 64) plan_fill_blocks(a, s, b, threadIdx.x & 63, 64);
+    for (int t = threadIdx.x; t < a.maxTokens; t += kPlanThreads) a.slots[t] = plan_slot(a, s, t);
+}
+
+constexpr int kPlanSlots = 1024; // per workgroup
+__global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a) {
+    const PlanScratch s = plan_scratch(a.scratch, a.batch);
+    if ((int)blockIdx.x < a.batch) {
+        plan_fill_blocks(a, s, blockIdx.x, threadIdx.x, 256);
+        return;
+    }
+    const int64_t t0 = (int64_t)(blockIdx.x - a.batch) * kPlanSlots;
+    for (int64_t t = t0 + threadIdx.x; t < min(t0 + kPlanSlots, (int64_t)a.maxTokens); t += 256) a.slots[t] = plan_slot(a, s, (int)t);
+}
+
+// ================================================================================================ adding and reading tokens
+// scale of a (block, head) = the smallest power of two with which its largest element stays in the codes' range.  Powers of two:
+// a block whose scale has to grow is re-expressed without a division, exactly in e4m3 (but for the last codes above zero), and an
+// element is rounded once when it is added -- with scales of amax / range every growth would round all older codes anew.  The
+// price is in int8, half a bit of the step on average (at most one); e4m3 has the same relative step at every scale.
+constexpr int kMaxBlockSize = 256;
+
+template <int CODE>
+__device__ __forceinline__ float pow2_scale(unsigned amax_bits) { // bits of a finite |x|
+    if (amax_bits == 0) return 0.f;
+    const int top = CODE == CACHE_E4M3 ? 8 : 6;                                // 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6
+    const unsigned frac = CODE == CACHE_E4M3 ? 0x600000u : 0x7e0000u;
+    int e = (int)(amax_bits >> 23) - 127 - top + ((amax_bits & 0x7fffffu) > frac ? 1 : 0);
+    e = max(e, -126);
+    return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
+}
+template <int CODE>
+__device__ __forceinline__ unsigned encode1(float x) {
+    if (CODE == CACHE_E4M3) return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xffu;
+    return (unsigned)(int)__builtin_rintf(x) & 0xffu;
+}
+template <int CODE>
+__device__ __forceinline__ float decode1(unsigned byte) {
+    if (CODE == CACHE_E4M3) return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0);
+    return (float)(int)(signed char)byte;
+}
+// the four codes of a word multiplied by ratio <= 1 and rounded
+template <int CODE>
+__device__ __forceinline__ unsigned rescale4(unsigned w, float ratio) {
+    unsigned r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r |= encode1<CODE>(decode1<CODE>((w >> (8 * i)) & 0xffu) * ratio) << (8 * i);
+    return r;
+}
+__device__ __forceinline__ float elem(const void* p, int64_t i, int type) {
+    const unsigned short u = ((const unsigned short*)p)[i];
+    return type == DT_F16 ? (float)__builtin_bit_cast(_Float16, u) : __builtin_bit_cast(float, (unsigned)u << 16);
+}
+
+// A workgroup per token; the first token of each block stays and serves all the call's tokens of that block (found by a scan over
+// the slots, so a block's tokens may stand anywhere in the call; of several tokens for one slot the last wins).  A wavefront
+// takes one head's keys or values at a time: largest element, scale, codes.
+template <int CODE>
+__global__ __launch_bounds__(256) void cache_add_kernel(AddArgs a) {
+    const CacheView& c = a.cache;
+    const int bs = c.blockSize, D = c.headDim, H = c.numHeads;
+    const int me = blockIdx.x;
+    const int64_t nslots = (int64_t)c.numBlocks * bs;
+    const int slot = a.slots[me];
+    if (slot < 0 || slot >= nslots) return;
+    const int block = slot / bs;
+    if (me > 0) {
+        const int before = a.slots[me - 1];
+        if (before >= 0 && before / bs == block) return;
+    }
+    __shared__ int token[kMaxBlockSize];
+    __shared__ int earlier;
+    for (int i = threadIdx.x; i < bs; i += 256) token[i] = -1;
+    if (threadIdx.x == 0) earlier = 0;
+    __syncthreads();
+    const int first = block * bs;
+    for (int j = threadIdx.x; j < a.tokens; j += 256) {
+        const unsigned o = (unsigned)(a.slots[j] - first);
+        if (o < (unsigned)bs) {
+            atomicMax(&token[o], j);
+            if (j < me) earlier = 1;
+        }
+    }
+    __syncthreads();
+    if (earlier) return;
+    const bool fresh = token[0] >= 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int unit = wave; unit < 2 * H; unit += 4) {
+        const bool isV = unit >= H;
+        const int h = isV ? unit - H : unit;
+        const void* x = isV ? a.value : a.key;
+        const int64_t ts = isV ? a.valueTokenStride : a.keyTokenStride, base = (int64_t)h * (isV ? a.valueHeadStride : a.keyHeadStride);
+        unsigned big = 0;
+        for (int o = 0; o < bs; ++o) {
+            const int t = token[o];
+            if (t < 0) continue;
+            for (int d = lane; d < D; d += 64)
+                big = max(big, __builtin_bit_cast(unsigned, elem(x, base + t * ts + d, a.type)) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) big = max(big, (unsigned)__shfl_xor((int)big, o, 64));
+        float* sp = (isV ? c.vs : c.ks) + (int64_t)block * H + h;
+        const float old = *sp;
+        const float before = fresh ? 0.f : old;
+        float after = __builtin_nanf("");
+        // anything that is no number makes the block's scale, and with it all its values, no number until the block is begun anew
+        if (big < 0x7f800000u && before >= 0.f && before < INFINITY) after = fmaxf(before, pow2_scale<CODE>(big));
+        const bool number = after == after;
+        const float inv = number && after > 0.f ? 1.f / after : 0.f;
+        const float ratio = after > 0.f ? before / after : 0.f;
+        const bool rescale = fresh || (number && ratio != 1.f);
+        uint8_t* codes = (isV ? c.v : c.k) + ((int64_t)block * H + h) * (int64_t)bs * D;
+        if (!isV) {
+            for (int o = 0; o < bs; ++o) {
+                const int t = token[o];
+                if (t < 0 && !rescale) continue;
+                for (int d = 4 * lane; d < D; d += 256) {
+                    unsigned* p = (unsigned*)(codes + (int64_t)o * D + d);
+                    unsigned w = 0;
+                    if (t >= 0) {
+                        if (number)
+                            for (int i = 0; i < 4; ++i) w |= encode1<CODE>(elem(x, base + t * ts + d + i, a.type) * inv) << (8 * i);
+                    } else {
+                        w = ratio == 0.f ? 0u : rescale4<CODE>(*p, ratio);
+                    }
+                    *p = w;
+                }
+            }
+        } else {
+            for (int g = 0; g < bs; g += 16) {
+                unsigned have = 0;
+                for (int i = 0; i < 16; ++i) have |= token[g + i] >= 0 ? 1u << i : 0u;
+                if (!have && !rescale) continue;
+                for (int d = lane; d < D; d += 64) {
+                    u32x4* p = (u32x4*)(codes + (int64_t)d * bs + g);
+                    u32x4 w = {0u, 0u, 0u, 0u};
+                    if (have != 0xffffu && !(rescale && ratio == 0.f)) w = *p;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (rescale && ratio != 0.f) w[i] = rescale4<CODE>(w[i], ratio);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int t = token[g + 4 * i + e];
+                            if (t < 0) continue;
+                            const unsigned b = number ? encode1<CODE>(elem(x, base + t * ts + d, a.type) * inv) : 0u;
+                            w[i] = (w[i] & ~(0xffu << (8 * e))) | (b << (8 * e));
+                        }
+                    }
+                    *p = w;
+                }
+            }
+        }
+        if (lane == 0) *sp = after;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ T narrow(float x);
+template <>
+__device__ __forceinline__ float narrow<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ _Float16 narrow<_Float16>(float x) { return (_Float16)x; }
+template <>
+__device__ __forceinline__ __bf16 narrow<__bf16>(float x) { return (__bf16)x; }
+
+// a workgroup per (block, head)
+template <int CODE, typename T>
+__global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs a) {
+    const CacheView& c = a.cache;
+    const int bs = c.blockSize, D = c.headDim, H = c.numHeads;
+    const int i = blockIdx.x / H, h = blockIdx.x - i * H;
+    const int block = a.blocks[i];
+    T* ko = (T*)a.key + (int64_t)blockIdx.x * bs * D;
+    T* vo = (T*)a.value + (int64_t)blockIdx.x * bs * D;
+    if ((unsigned)block >= (unsigned)c.numBlocks) { // no such block: no such values
+        for (int x = threadIdx.x; x < bs * D; x += 256) ko[x] = vo[x] = narrow<T>(__builtin_nanf(""));
+        return;
+    }
+    const int64_t at = (int64_t)block * H + h;
+    const float ks = c.ks[at], vs = c.vs[at];
+    const uint8_t* kc = c.k + at * bs * D;
+    const uint8_t* vc = c.v + at * bs * D;
+    for (int x = 4 * threadIdx.x; x < bs * D; x += 1024) {
+        const unsigned w = *(const unsigned*)(kc + x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) ko[x + e] = narrow<T>(decode1<CODE>((w >> (8 * e)) & 0xffu) * ks);
+    }
+    for (int x = threadIdx.x; x < bs * D; x += 256) {
+        const int t = x / D, d = x - t * D;
+        vo[x] = narrow<T>(decode1<CODE>(vc[(int64_t)d * bs + t]) * vs);
+    }
+}
+
+// ================================================================================================ beam selection
+// value(w, v) = score_w + x_wv - log sum_v exp x_wv.  Inside a beam candidates rank as their logits do, so one pass over the logits
+// keeps the `keep` best (logit, lowest v) of every piece of a row beside its maximum and sum of exponentials; a second launch
+// joins the pieces of a row, then the rows of a batch item.  The exponentials' sum is accumulated in 64 bits and candidates of
+// different beams are compared as 64-bit values: they come in the order of the exact values unless those agree to ~1e-8.
+constexpr int kBeamVpt = 16;                                   // logits per lane and step
+constexpr int kBeamCap = kMaxBeams + 64 * kBeamVpt;            // keys a wavefront may hold at once
+constexpr int kBeamKeys = 2048;                                // keys of a row that the second launch joins
+
+struct BeamSched {
+    int parts;
+    u64* keys;    // [rows][parts][keep]
+    double* sums; // [rows][parts]
+    float* maxs;  // [rows][parts]
+};
+
+// (ordkey, index) of a logit: smaller is better; ~0 for what is no candidate
+__device__ __forceinline__ u64 beam_key(float x, unsigned v) {
+    return x > -INFINITY ? ((u64)~float_flip(x) << 32) | v : ~0ull;
+}
+__device__ __forceinline__ float beam_logit(u64 key) { return float_unflip(~(unsigned)(key >> 32)); }
+
+// The `keep`-th smallest of the n unique keys in LDS (n > keep): bits from the top, one ballot per key and bit.
+__device__ __forceinline__ u64 wave_kth(const u64* list, int n, int keep) {
+    const int lane = lane64();
+    u64 t = 0;
+    if (n <= 64) {
+        const u64 k = lane < n ? list[lane] : ~0ull;
+        for (int b = 63; b >= 0; --b) {
+            const u64 c = t | ((1ull << b) - 1);
+            if (__popcll(__ballot(lane < n && k <= c)) < keep) t |= 1ull << b;
+        }
+        return t;
+    }
+    for (int b = 63; b >= 0; --b) {
+        const u64 c = t | ((1ull << b) - 1);
+        int cnt = 0;
+        for (int i = lane; i < n; i += 64) cnt += list[i] <= c;
+        cnt = __builtin_amdgcn_readlane((int)wave_incl_scan((unsigned)cnt), 63);
+        if (cnt < keep) t |= 1ull << b;
+    }
+    return t;
+}
+// keeps the keys <= kth of the n in LDS, in place
+__device__ __forceinline__ int wave_cut(u64* list, int n, u64 kth) {
+    const int lane = lane64();
+    int out = 0;
+    for (int i0 = 0; i0 < n; i0 += 64) {
+        const u64 k = i0 + lane < n ? list[i0 + lane] : ~0ull;
+        const bool in = i0 + lane < n && k <= kth;
+        const u64 m = __ballot(in);
+        __builtin_amdgcn_wave_barrier();
+        if (in) list[out + __popcll(m & ((1ull << lane) - 1))] = k;
+        out += __popcll(m);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    return out;
+}
+
+template <typename T>
+__device__ __forceinline__ float logit(T x) { return (float)x; }
+
+template <typename T>
+__global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s) {
+    constexpr int PER = 16 / sizeof(T); // logits of a 16-byte load
+    constexpr int LD = kBeamVpt / PER;
+    __shared__ __align__(16) u64 lists[4][kBeamCap];
+    __shared__ double ss[4];
+    __shared__ float sm[4];
+    __shared__ int sn[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t row = blockIdx.x / s.parts;
+    const int part = (int)(blockIdx.x - row * s.parts);
+    const int bi = (int)(row / a.beams), w = (int)(row - (int64_t)bi * a.beams);
+    const int keep = a.keep;
+    u64* out = s.keys + (row * s.parts + part) * keep;
+    if (a.finished && a.finished[row]) { // its one candidate is made by the second launch
+        if (threadIdx.x < keep) out[threadIdx.x] = ~0ull;
+        return;
+    }
+    const T* x = (const T*)a.logits + (int64_t)bi * a.batchStride + (int64_t)w * a.beamStride;
+    // granules of 16 bytes from the row's first logit, shared out to the parts and wavefronts in runs of 64 x LD.  By index and not
+    // by address: rows of the same logits then have the same sum to the last bit wherever they lie, and equal beams stay tied
+    // (the loads need no alignment)
+    const int64_t granules = (a.vocab + PER - 1) / PER;
+    const int64_t steps = (granules + 64 * LD - 1) / (64 * LD);
+    u64* list = lists[wave];
+    int n = 0;
+    u64 thr = ~0ull; // only keys below it can be among the best
+    float m = -INFINITY;
+    double sum = 0.0;
+    for (int64_t st = (int64_t)part * 4 + wave; st < steps; st += (int64_t)s.parts * 4) {
+        float v[kBeamVpt];
+        unsigned best = ~0u;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < LD; ++i) {
+            const int64_t e0 = ((st * LD + i) * 64 + lane) * PER;
+            if (e0 + PER <= a.vocab) {
+                T t[PER];
+                __builtin_memcpy(t, x + e0, 16);
+#pragma unroll
+                for (int e = 0; e < PER; ++e) v[i * PER + e] = logit(t[e]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < PER; ++e) {
+                    const int64_t at = e0 + e;
+                    v[i * PER + e] = at < a.vocab ? logit(x[at]) : -INFINITY;
+                }
+            }
+        }
+        bool odd = false; // a NaN
+#pragma unroll
+        for (int i = 0; i < kBeamVpt; ++i) {
+            mx = fmaxf(mx, v[i]);
+            odd |= v[i] != v[i];
+            const unsigned k = v[i] > -INFINITY ? ~float_flip(v[i]) : ~0u;
+            best = min(best, k);
+        }
+        // running maximum and sum of the lane
+        const float mn = fmaxf(m, mx);
+        if (mn > -INFINITY) {
+            float p = 0.f;
+#pragma unroll
+            for (int i = 0; i < kBeamVpt; ++i) p += __builtin_amdgcn_exp2f((v[i] - mn) * 1.4426950408889634f);
+            sum = sum * (double)__builtin_amdgcn_exp2f((m - mn) * 1.4426950408889634f) + (double)p;
+        }
+        if (odd) sum = __builtin_nan("");
+        m = mn;
+        // candidates.  The keep-th best of the lanes' best logits bounds what can be among the keep best of this step.
+        unsigned lim = (unsigned)(thr >> 32);
+        if (thr == ~0ull) {
+            unsigned t = 0;
+            for (int b = 31; b >= 0; --b) {
+                const unsigned c = t | ((1u << b) - 1);
+                if (__popcll(__ballot(best <= c)) < keep) t |= 1u << b;
+            }
+            lim = t;
+        }
+        if (!__ballot(best <= lim && best != ~0u)) continue;
+#pragma unroll
+        for (int i = 0; i < kBeamVpt; ++i) {
+            const unsigned k = v[i] > -INFINITY ? ~float_flip(v[i]) : ~0u;
+            const int64_t at = ((st * LD + i / PER) * 64 + lane) * PER + i % PER;
+            const u64 key = ((u64)k << 32) | (unsigned)at;
+            const bool in = k != ~0u && k <= lim && key < thr;
+            const u64 mask = __ballot(in);
+            if (!mask) continue;
+            if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
+            n += __popcll(mask);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        if (n > keep) {
+            thr = wave_kth(list, n, keep);
+            n = wave_cut(list, n, thr);
+        }
+    }
+    // the wavefront's maximum and sum, then the workgroup's
+    float M = m;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    double S = (m == -INFINITY && sum == sum) ? 0.0 : sum * (double)__builtin_amdgcn_exp2f((m - M) * 1.4426950408889634f);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) S += __shfl_xor(S, o, 64);
+    if (lane == 0) {
+        sm[wave] = M;
+        ss[wave] = S;
+        sn[wave] = n;
+    }
+    __syncthreads();
+    if (wave) return;
+    // wavefront 0 appends the others' lists to its own (4 keep <= 256 keys)
+    for (int o = 1; o < 4; ++o) {
+        const int no = sn[o];
+        for (int i = lane; i < no; i += 64) list[n + i] = lists[o][i];
+        n += no;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+    if (n > keep) n = wave_cut(list, n, wave_kth(list, n, keep));
+    for (int i = lane; i < keep; i += 64) out[i] = i < n ? list[i] : ~0ull;
+    if (lane == 0) {
+        float MM = -INFINITY;
+        for (int o = 0; o < 4; ++o) MM = fmaxf(MM, sm[o]);
+        double SS = 0.0;
+        for (int o = 0; o < 4; ++o)
+            if (sm[o] > -INFINITY || ss[o] != ss[o]) SS += ss[o] * exp((double)sm[o] - (double)MM);
+        s.maxs[row * s.parts + part] = MM;
+        s.sums[row * s.parts + part] = SS;
+    }
+}
+
+__device__ __forceinline__ u64 double_flip(double x) { // larger is smaller
+    const u64 u = __builtin_bit_cast(u64, x == 0.0 ? 0.0 : x);
+    return ~((u >> 63) ? ~u : (u | (1ull << 63)));
+}
+
+// a workgroup of 16 wavefronts per batch item
+constexpr int kBeamJoin = 1024;
+__global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSched s) {
+    __shared__ u64 val[kMaxBeams * kMaxBeams]; // double_flip of a candidate's value
+    __shared__ unsigned tok[kMaxBeams * kMaxBeams];
+    __shared__ u64 lists[kBeamJoin / 64][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, keep = a.keep, b = blockIdx.x;
+    for (int w = wave; w < a.beams; w += kBeamJoin / 64) {
+        const int64_t row = (int64_t)b * a.beams + w;
+        const double score = (double)a.scores[row];
+        u64* vw = val + w * keep;
+        unsigned* tw = tok + w * keep;
+        if (a.finished && a.finished[row]) {
+            for (int i = lane; i < keep; i += 64) {
+                vw[i] = i == 0 && score > -INFINITY ? double_flip(score) : ~0ull;
+                tw[i] = (unsigned)a.padToken;
+            }
+            continue;
+        }
+        // log of the sum of the row's exponentials
+        float M = -INFINITY;
+        for (int p = lane; p < s.parts; p += 64) M = fmaxf(M, s.maxs[row * s.parts + p]);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        double S = 0.0;
+        for (int p = lane; p < s.parts; p += 64) {
+            const float pm = s.maxs[row * s.parts + p];
+            const double ps = s.sums[row * s.parts + p];
+            if (pm > -INFINITY || ps != ps) S += ps * exp((double)pm - (double)M);
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) S += __shfl_xor(S, o, 64);
+        const double lse = (double)M + log(S);
+        // the row's best: keys below the keep-th best of the lanes' best, cut in LDS; in rounds where they do not fit
+        const u64* keys = s.keys + row * s.parts * keep;
+        const int total = s.parts * keep;
+        u64* list = lists[wave];
+        int n = 0;
+        u64 thr = ~0ull;
+        for (int i0 = 0; i0 < total; i0 += 128) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int i = i0 + 64 * j + lane;
+                const u64 k = i < total ? keys[i] : ~0ull;
+                const bool in = k < thr;
+                const u64 mask = __ballot(in);
+                if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = k;
+                n += __popcll(mask);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            if (n > keep) {
+                thr = wave_kth(list, n, keep);
+                n = wave_cut(list, n, thr);
+            }
+        }
+        for (int i = lane; i < keep; i += 64) {
+            u64 v = ~0ull;
+            unsigned t = 0;
+            if (i < n) {
+                const double value = score + ((double)beam_logit(list[i]) - lse);
+                if (value > -INFINITY) v = double_flip(value); // (NaN: no candidate)
+                t = (unsigned)list[i];
+            }
+            vw[i] = v;
+            tw[i] = t;
+        }
+    }
+    __syncthreads();
+    // rank of each candidate among those of the batch item: by value, then beam, then token
+    const int total = a.beams * keep;
+    int valid = 0;
+    for (int i0 = 0; i0 < total; i0 += kBeamJoin) {
+        const int i = i0 + threadIdx.x;
+        const bool is = i < total && val[min(i, total - 1)] != ~0ull;
+        valid += __syncthreads_count(is);
+        if (!is) continue;
+        const u64 v = val[i];
+        const unsigned t = tok[i];
+        const int w = i / keep;
+        int rank = 0;
+        for (int j = 0; j < total; ++j) {
+            const u64 o = val[j];
+            const int ow = j / keep;
+            rank += o < v || (o == v && (ow < w || (ow == w && tok[j] < t)));
+            if (rank >= keep) break;
+        }
+        if (rank < keep) {
+            const int64_t at = (int64_t)b * keep + rank;
+            const u64 u = ~v;
+            a.outScores[at] = (float)__builtin_bit_cast(double, (u >> 63) ? (u & ~(1ull << 63)) : ~u);
+            a.parents[at] = w;
+            a.tokens[at] = (int)t;
+        }
+    }
+    for (int i = valid + threadIdx.x; i < keep; i += kBeamJoin) { // fewer candidates than asked for
+        const int64_t at = (int64_t)b * keep + i;
+        a.outScores[at] = -INFINITY;
+        a.parents[at] = -1;
+        a.tokens[at] = -1;
+    }
+}
+
+// ================================================================================================ reordering by parent
+struct ReorderTable {
+    ReorderState st[kMaxReorderStates];
+    int first[kMaxReorderStates + 1]; // workgroups of a row before state i
+};
+constexpr int kReorderBytes = 16384; // of a row per workgroup
+
+__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderTable tab, int n, const int* parents, int beams, int keep) {
+    const int chunk = blockIdx.y;
+    int lo = 0;
+    while (lo + 1 < n && tab.first[lo + 1] <= chunk) ++lo;
+    const ReorderState& s = tab.st[lo];
+    const int64_t row = blockIdx.x;
+    const int b = (int)(row / keep);
+    const int parent = parents[row];
+    const int64_t at = (int64_t)(chunk - tab.first[lo]) * kReorderBytes, len = min((int64_t)kReorderBytes, s.rowBytes - at);
+    uint8_t* out = (uint8_t*)s.out + row * s.rowBytes + at;
+    const bool none = parent < 0 || parent >= beams; // such a row becomes zero
+    const uint8_t* in = (const uint8_t*)s.in + (int64_t)b * s.inBatchBytes + (int64_t)(none ? 0 : parent) * s.inBeamBytes + at;
+    for (int64_t i = threadIdx.x; i < len; i += 256) out[i] = none ? 0 : in[i];
+}
+
+struct ForkTable {
+    CacheView c[kMaxForkCaches];
+};
+// blockIdx.x: row; blockIdx.y: 0 the table, 1 + i cache i
+__global__ __launch_bounds__(256) void fork_blocks_kernel(ForkArgs a, ForkTable tab, int blockSize, int numBlocks, int withTable) {
+    const int row = blockIdx.x, b = row / a.beams;
+    int parent = a.parents[row];
+    parent = parent < 0 || parent >= a.beams ? row : b * a.beams + parent;
+    const int cap = a.cols * blockSize;
+    const int len = min(max(a.lengths[parent], 0), cap), mine = min(max(a.lengths[row], 0), cap);
+    const int tail = len % blockSize ? len / blockSize : -1; // column of the parent's partly filled block
+    const int src = tail >= 0 ? a.table[(int64_t)parent * a.tableStride + tail] : -1;
+    const int dst = a.spare[row];
+    const bool ok = tail >= 0 && (unsigned)src < (unsigned)numBlocks && (unsigned)dst < (unsigned)numBlocks;
+    if (withTable && blockIdx.y == 0) {
+        for (int j = threadIdx.x; j < a.cols; j += 256)
+            a.tableOut[(int64_t)row * a.cols + j] = j == tail ? (ok ? dst : -1) : a.table[(int64_t)parent * a.tableStride + j];
+        if (threadIdx.x == 0) {
+            a.lengthsOut[row] = a.lengths[parent];
+            a.spareOut[row] = tail < 0 ? dst : mine % blockSize ? a.table[(int64_t)row * a.tableStride + mine / blockSize] : -1;
+        }
+        return;
+    }
+    if (!ok) return;
+    const CacheView& c = tab.c[blockIdx.y - withTable];
+    const int64_t bytes = (int64_t)c.numHeads * blockSize * c.headDim;
+    const u32x4 *k = (const u32x4*)(c.k + src * bytes), *v = (const u32x4*)(c.v + src * bytes);
+    u32x4 *ko = (u32x4*)(c.k + dst * bytes), *vo = (u32x4*)(c.v + dst * bytes);
+    for (int64_t i = threadIdx.x; i < bytes / 16; i += 256) {
+        ko[i] = k[i];
+        vo[i] = v[i];
+    }
+    for (int h = threadIdx.x; h < c.numHeads; h += 256) {
+        c.ks[(int64_t)dst * c.numHeads + h] = c.ks[(int64_t)src * c.numHeads + h];
+        c.vs[(int64_t)dst * c.numHeads + h] = c.vs[(int64_t)src * c.numHeads + h];
+    }
+}
+
+void beam_sched(const BeamArgs& a, int num_cus, BeamSched& s, size_t& bytes) {
+    const int64_t rows = (int64_t)a.batch * a.beams;
+    // about eight workgroups per CU, each wavefront a step of its own, and no more keys of a row than its join takes at once
+    int64_t parts = (8 * (int64_t)num_cus + rows - 1) / std::max<int64_t>(rows, 1);
+    parts = std::min<int64_t>(parts, (a.vocab + 4 * 64 * kBeamVpt - 1) / (4 * 64 * kBeamVpt));
+    parts = std::min<int64_t>(parts, kBeamKeys / a.keep);
+    s.parts = (int)std::max<int64_t>(parts, 1);
+    const size_t kb = round_up((size_t)rows * s.parts * a.keep * 8, 256), sb = round_up((size_t)rows * s.parts * 8, 256);
+    char* p = (char*)a.workspace;
+    s.keys = (u64*)p;
+    s.sums = (double*)(p + kb);
+    s.maxs = (float*)(p + kb + sb);
+    bytes = kb + sb + round_up((size_t)rows * s.parts * 4, 256);
+}
+
+} // namespace
+
+size_t plan_scratch_ints(int batch) { return (size_t)batch * 4 + 2; }
+
+void launch_plan_blocks(const PlanArgs& a, hipStream_t stream) {
+    if (a.maxTokens <= 4 * kPlanThreads && a.batch <= kPlanThreads) {
+        plan_scan_kernel<true><<<1, kPlanThreads, 0, stream>>>(a);
+    } else {
+        plan_scan_kernel<false><<<1, kPlanThreads, 0, stream>>>(a);
+        HIP_CHECK(hipGetLastError());
+        plan_fill_kernel<<<(unsigned)(a.batch + div_up(a.maxTokens, kPlanSlots)), 256, 0, stream>>>(a);
+    }
+    HIP_CHECK(hipGetLastError());
+}
+
+void launch_cache_add(const AddArgs& a, hipStream_t stream) {
+    if (a.tokens == 0) return;
+    if (a.cache.code == CACHE_E4M3)
+        cache_add_kernel<CACHE_E4M3><<<a.tokens, 256, 0, stream>>>(a);
+    else
+        cache_add_kernel<CACHE_INT8><<<a.tokens, 256, 0, stream>>>(a);
+    HIP_CHECK(hipGetLastError());
+}
+
+template <int CODE>
+static void launch_reconstruct(const ReconstructArgs& a, hipStream_t stream) {
+    const unsigned grid = (unsigned)((int64_t)a.n * a.cache.numHeads);
+    if (a.type == DT_F32)
+        cache_reconstruct_kernel<CODE, float><<<grid, 256, 0, stream>>>(a);
+    else if (a.type == DT_F16)
+        cache_reconstruct_kernel<CODE, _Float16><<<grid, 256, 0, stream>>>(a);
+    else
+        cache_reconstruct_kernel<CODE, __bf16><<<grid, 256, 0, stream>>>(a);
+}
+void launch_cache_reconstruct(const ReconstructArgs& a, hipStream_t stream) {
+    if (a.n == 0) return;
+    FA_THROW_IF_NOT_MSG((int64_t)a.n * a.cache.numHeads < ((int64_t)1 << 31), "reconstruct: too many blocks for one call");
+    if (a.cache.code == CACHE_E4M3)
+        launch_reconstruct<CACHE_E4M3>(a, stream);
+    else
+        launch_reconstruct<CACHE_INT8>(a, stream);
+    HIP_CHECK(hipGetLastError());
+}
+
+size_t beam_select_workspace(const BeamArgs& a, int num_cus) {
+    BeamSched s;
+    size_t bytes;
+    beam_sched(a, num_cus, s, bytes);
+    return bytes;
+}
+void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream) {
+    if (a.batch == 0) return;
+    BeamSched s;
+    size_t bytes;
+    beam_sched(a, num_cus, s, bytes);
+    const int64_t grid = (int64_t)a.batch * a.beams * s.parts;
+    FA_THROW_IF_NOT_MSG(grid < ((int64_t)1 << 31), "beam_select: too many rows for one call");
+    if (a.type == DT_F32)
+        beam_scan_kernel<float><<<(unsigned)grid, 256, 0, stream>>>(a, s);
+    else if (a.type == DT_F16)
+        beam_scan_kernel<_Float16><<<(unsigned)grid, 256, 0, stream>>>(a, s);
+    else
+        beam_scan_kernel<__bf16><<<(unsigned)grid, 256, 0, stream>>>(a, s);
+    HIP_CHECK(hipGetLastError());
+    beam_join_kernel<<<a.batch, kBeamJoin, 0, stream>>>(a, s);
+    HIP_CHECK(hipGetLastError());
+}
+
+void launch_beam_reorder(const ReorderState* states, int n, const int* parents, int batch, int beams, int keep, hipStream_t stream) {
+    const int64_t rows = (int64_t)batch * keep;
+    if (rows == 0) return;
+    ReorderTable tab;
+    int k = 0;
+    int64_t first = 0;
+    for (int i = 0; i < n; ++i) {
+        if (states[i].rowBytes == 0) continue;
+        tab.st[k] = states[i];
+        tab.first[k++] = (int)first;
+        first += (states[i].rowBytes + kReorderBytes - 1) / kReorderBytes;
+        FA_THROW_IF_NOT_MSG(first <= 65535, "reorder: rows too long for one call");
+    }
+    if (k == 0) return;
+    tab.first[k] = (int)first;
+    beam_reorder_kernel<<<dim3((unsigned)rows, (unsigned)first), 256, 0, stream>>>(tab, k, parents, beams, keep);
+    HIP_CHECK(hipGetLastError());
+}
+
+void launch_fork_blocks(const ForkArgs& a, const CacheView* caches, int n, hipStream_t stream) {
+    const int rows = a.batch * a.beams;
+    if (rows == 0) return;
+    const int bs = caches[0].blockSize, nb = caches[0].numBlocks;
+    for (int i = 0; i == 0 || i < n; i += kMaxForkCaches) {
+        ForkTable tab;
+        const int m = std::min(kMaxForkCaches, n - i);
+        for (int j = 0; j < m; ++j) tab.c[j] = caches[i + j];
+        fork_blocks_kernel<<<dim3((unsigned)rows, (unsigned)(m + (i == 0))), 256, 0, stream>>>(a, tab, bs, nb, i == 0);
+        HIP_CHECK(hipGetLastError());
+    }
+}
+
+} // namespace faiss_amd

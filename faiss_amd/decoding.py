@@ -1,0 +1,381 @@
+"""faiss_amd/decoding.py -- operators of a program that decodes with a model next to its searches, over torch tensors.
+
+    cache = PagedCache(res, num_blocks, block_size, num_heads, head_dim, code="e4m3")   # one per layer
+    plan = plan_blocks(res, table, lengths, new_lengths, ring, state, block_size, max_tokens)
+    cache.add(k, v, plan.slots)
+    out = cache.attend(q, table, plan.lengths, query_offsets=plan.query_offsets)
+    scores, parents, tokens = beam_select(res, logits, scores, num_beams)
+    states = reorder_beams(res, states, parents)
+    table, lengths, spare = fork_blocks(res, caches, table, lengths, spare, parents)
+
+The work of a call is ordered on torch's current stream of the resources' device and nothing is synchronised, so calls can be
+captured into a graph; results and scratch come from torch's allocator.  What the calls compute, and what they do with lengths,
+slots, block ids and parents that are out of range, is stated in include/faiss_amd_c.h.  Tensors must be on the resources'
+device; arguments of the wrong shape, type or device raise ValueError / TypeError before anything is launched.
+"""
+import collections
+import ctypes
+import math
+
+import torch
+
+from . import _check, load_library
+
+_HALF = {torch.float16: 2, torch.bfloat16: 3}
+_FLOAT = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}
+_CODES = {"int8": 0, "e4m3": 1}
+_CODE_OF = {torch.int8: 0, torch.float8_e4m3fn: 1}
+_P, _I, _I64, _F, _SZ = ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t
+
+
+class _CacheStruct(ctypes.Structure):
+    _fields_ = [("keys", _P), ("values", _P), ("keyScales", _P), ("valueScales", _P), ("code", _I), ("numBlocks", _I),
+                ("blockSize", _I), ("numHeads", _I), ("headDim", _I)]
+
+
+class _PlanStruct(ctypes.Structure):
+    _fields_ = [("blockTable", _P), ("ownedTable", _P), ("tableStride", _I64), ("ownedStride", _I64), ("lengths", _P),
+                ("newLengths", _P), ("freeRing", _P), ("freeState", _P), ("lengthsOut", _P), ("freeStateOut", _P),
+                ("queryOffsets", _P), ("slots", _P), ("granted", _P), ("workspace", _P), ("batch", _I), ("numColumns", _I),
+                ("numBlocks", _I), ("blockSize", _I), ("maxTokens", _I)]
+
+
+class _AddStruct(ctypes.Structure):
+    _fields_ = [("keys", _P), ("values", _P), ("keyTokenStride", _I64), ("keyHeadStride", _I64), ("valueTokenStride", _I64),
+                ("valueHeadStride", _I64), ("slots", _P), ("tokens", _I), ("type", _I)]
+
+
+class _AttendStruct(ctypes.Structure):
+    _fields_ = [("queries", _P), ("out", _P), ("lse", _P), ("queryTokenStride", _I64), ("queryHeadStride", _I64),
+                ("outTokenStride", _I64), ("outHeadStride", _I64), ("blockTable", _P), ("tableStride", _I64), ("lengths", _P),
+                ("queryOffsets", _P), ("batch", _I), ("tokens", _I), ("heads", _I), ("numColumns", _I), ("maxQueries", _I),
+                ("type", _I), ("causal", _I), ("scale", _F), ("workspace", _P), ("workspaceBytes", _SZ)]
+
+
+class _BeamStruct(ctypes.Structure):
+    _fields_ = [("logits", _P), ("batchStride", _I64), ("beamStride", _I64), ("scores", _P), ("finished", _P), ("outScores", _P),
+                ("outParents", _P), ("outTokens", _P), ("vocab", _I64), ("batch", _I), ("beams", _I), ("keep", _I),
+                ("padToken", _I), ("type", _I), ("workspace", _P), ("workspaceBytes", _SZ)]
+
+
+class _StateStruct(ctypes.Structure):
+    _fields_ = [("in_", _P), ("out", _P), ("batchBytes", _I64), ("beamBytes", _I64), ("rowBytes", _I64)]
+
+
+class _ForkStruct(ctypes.Structure):
+    _fields_ = [("blockTable", _P), ("tableStride", _I64), ("lengths", _P), ("spare", _P), ("parents", _P), ("tableOut", _P),
+                ("lengthsOut", _P), ("spareOut", _P), ("batch", _I), ("beams", _I), ("numColumns", _I)]
+
+
+_byref = ctypes.byref
+
+
+def _tensor(res, t, name, dtype=None, dim=None, dense=True):
+    """`t` is a tensor of res's device with the dtype(s), number of dimensions and (dense) the contiguous layout asked for"""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch tensor" % name)
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError("%s must be %s, not %s" % (name, dtype, t.dtype))
+    if dim is not None and t.dim() != dim:
+        raise ValueError("%s must have %d dimensions, not %d" % (name, dim, t.dim()))
+    if not t.is_cuda or t.device.index != res.device:
+        raise ValueError("%s must be on the resources' device cuda:%d, not %s" % (name, res.device, t.device))
+    if dense and not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)
+    return t
+
+
+def _rows(res, t, name, dtype=torch.int32):
+    """a table whose rows are dense and do not overlap"""
+    _tensor(res, t, name, dtype, 2, dense=False)
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError("the rows of %s must be dense" % name)
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError("the rows of %s must not overlap" % name)
+    return t
+
+
+def _row_stride(t):
+    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+
+
+def _same_length(t, n, name):
+    if t.shape[0] != n:
+        raise ValueError("%s must have %d entries, not %d" % (name, n, t.shape[0]))
+    return t
+
+
+def _dense_last(t, name):
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError("the last dimension of %s must be dense" % name)
+
+
+def _stream(res):
+    return torch.cuda.current_stream(res.device).cuda_stream
+
+
+def _device(res):
+    return torch.device("cuda", res.device)
+
+
+BlockPlan = collections.namedtuple("BlockPlan", "lengths free_state query_offsets slots granted")
+
+
+def plan_blocks(res, block_table, lengths, new_lengths, free_ring, free_state, block_size, max_tokens, owned_table=None,
+                lengths_out=None, free_state_out=None):
+    """Block tables and slot maps on the device from request lengths (faiss_amd_plan_blocks).
+
+    block_table [batch, columns] and free_ring [num_blocks] (int32) are updated in place; lengths, new_lengths [batch] int32;
+    free_state [2] int64 = {front, count}; lengths_out / free_state_out may be the tensors given (None: new ones).  ->
+    BlockPlan(lengths [batch], free_state, query_offsets [batch + 1], slots [max_tokens], granted [batch])."""
+    _rows(res, block_table, "block_table")
+    n, cols = block_table.shape
+    for t, name in ((lengths, "lengths"), (new_lengths, "new_lengths")):
+        _same_length(_tensor(res, t, name, torch.int32, 1), n, name)
+    _tensor(res, free_ring, "free_ring", torch.int32, 1)
+    _same_length(_tensor(res, free_state, "free_state", torch.int64, 1), 2, "free_state")
+    if owned_table is not None:
+        _rows(res, owned_table, "owned_table")
+        if owned_table.shape != block_table.shape:
+            raise ValueError("owned_table must have the shape of block_table")
+    dev = _device(res)
+    if lengths_out is None:
+        lengths_out = torch.empty(n, dtype=torch.int32, device=dev)
+    else:
+        _same_length(_tensor(res, lengths_out, "lengths_out", torch.int32, 1), n, "lengths_out")
+    if free_state_out is None:
+        free_state_out = torch.empty(2, dtype=torch.int64, device=dev)
+    else:
+        _same_length(_tensor(res, free_state_out, "free_state_out", torch.int64, 1), 2, "free_state_out")
+    max_tokens = int(max_tokens)
+    # offsets, grants and scratch in one allocation
+    ints = torch.empty(6 * n + 3, dtype=torch.int32, device=dev)
+    offsets, granted, scratch = ints[:n + 1], ints[n + 1:2 * n + 1], ints[2 * n + 1:]
+    slots = torch.empty(max(max_tokens, 0), dtype=torch.int32, device=dev)
+    a = _PlanStruct(block_table.data_ptr() or None, owned_table.data_ptr() if owned_table is not None else None,
+                    _row_stride(block_table), _row_stride(owned_table) if owned_table is not None else 0, lengths.data_ptr() or None,
+                    new_lengths.data_ptr() or None, free_ring.data_ptr() or None, free_state.data_ptr(), lengths_out.data_ptr() or None,
+                    free_state_out.data_ptr(), offsets.data_ptr(), slots.data_ptr() or None, granted.data_ptr(), scratch.data_ptr(),
+                    n, cols, free_ring.shape[0], int(block_size), max_tokens)
+    _check(res._lib.faiss_amd_plan_blocks(res._h, _byref(a), _stream(res)))
+    return BlockPlan(lengths_out, free_state_out, offsets, slots, granted)
+
+
+class PagedCache:
+    """Keys and values of one layer in blocks of 8-bit codes, one scale per block and head.
+
+    Tensors: k_codes [num_blocks, num_heads, block_size, head_dim], v_codes [num_blocks, num_heads, head_dim, block_size]
+    (torch.int8 or torch.float8_e4m3fn), k_scales, v_scales [num_blocks, num_heads] float32; a value is code * scale."""
+
+    def __init__(self, res, num_blocks, block_size, num_heads, head_dim, code="e4m3"):
+        if code not in _CODES:
+            raise ValueError("code must be 'int8' or 'e4m3'")
+        dt = torch.int8 if code == "int8" else torch.float8_e4m3fn
+        dev = _device(res)
+        k = torch.zeros((num_blocks, num_heads, block_size, head_dim), dtype=torch.int8, device=dev).view(dt)
+        v = torch.zeros((num_blocks, num_heads, head_dim, block_size), dtype=torch.int8, device=dev).view(dt)
+        self._set(res, k, v, torch.zeros((num_blocks, num_heads), device=dev), torch.zeros((num_blocks, num_heads), device=dev))
+
+    @classmethod
+    def wrap(cls, res, k_codes, v_codes, k_scales, v_scales):
+        """a cache over tensors that the caller holds"""
+        self = cls.__new__(cls)
+        self._set(res, k_codes, v_codes, k_scales, v_scales)
+        return self
+
+    def _set(self, res, k, v, ks, vs):
+        if k.dtype not in _CODE_OF or v.dtype != k.dtype:
+            raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn, keys and values alike")
+        _tensor(res, k, "k_codes", None, 4)
+        _tensor(res, v, "v_codes", None, 4)
+        n, h, b, d = k.shape
+        if tuple(v.shape) != (n, h, d, b):
+            raise ValueError("v_codes must have the shape %s, not %s" % ((n, h, d, b), tuple(v.shape)))
+        for t, name in ((ks, "k_scales"), (vs, "v_scales")):
+            if tuple(_tensor(res, t, name, torch.float32, 2).shape) != (n, h):
+                raise ValueError("%s must have the shape %s" % (name, (n, h)))
+        if b not in (16, 32, 64, 128, 256):
+            raise ValueError("block size must be 16, 32, 64, 128 or 256")
+        if d not in (64, 96, 128, 192, 256):
+            raise ValueError("head dimension must be 64, 96, 128, 192 or 256")
+        if n < 1 or h < 1 or n * b >= 1 << 31:
+            raise ValueError("number of blocks or heads out of range")
+        self.res, self.k_codes, self.v_codes, self.k_scales, self.v_scales = res, k, v, ks, vs
+        self.num_blocks, self.num_heads, self.block_size, self.head_dim = n, h, b, d
+        self.code = "int8" if k.dtype == torch.int8 else "e4m3"
+        self._s = _CacheStruct(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), _CODE_OF[k.dtype], n, b, h, d)
+        self._ref = _byref(self._s)
+        self._lib = load_library()
+
+    def add(self, k, v, slots):
+        """store the tokens k, v [tokens, num_heads, head_dim] (float16 / bfloat16) at slots [tokens] (int32; -1: skipped)"""
+        res = self.res
+        for t, name in ((k, "k"), (v, "v")):
+            _tensor(res, t, name, None, 3, dense=False)
+            if t.shape[1] != self.num_heads or t.shape[2] != self.head_dim:
+                raise ValueError("%s must be [tokens, %d, %d]" % (name, self.num_heads, self.head_dim))
+            _dense_last(t, name)
+        if k.dtype not in _HALF or v.dtype != k.dtype:
+            raise TypeError("k and v must be float16 or bfloat16, both the same")
+        n = k.shape[0]
+        _same_length(v, n, "v")
+        _same_length(_tensor(res, slots, "slots", torch.int32, 1), n, "slots")
+        a = _AddStruct(k.data_ptr() or None, v.data_ptr() or None, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                       slots.data_ptr() or None, n, _HALF[k.dtype])
+        _check(self._lib.faiss_amd_PagedCache_add(res._h, self._ref, _byref(a), _stream(res)))
+
+    def reconstruct(self, blocks, dtype=torch.float32):
+        """the values of blocks [n] (int32) -> k, v [n, num_heads, block_size, head_dim]; NaN for an id out of range"""
+        res = self.res
+        _tensor(res, blocks, "blocks", torch.int32, 1)
+        if dtype not in _FLOAT:
+            raise TypeError("dtype must be float32, float16 or bfloat16")
+        shape = (blocks.shape[0], self.num_heads, self.block_size, self.head_dim)
+        k, v = torch.empty(shape, dtype=dtype, device=blocks.device), torch.empty(shape, dtype=dtype, device=blocks.device)
+        _check(self._lib.faiss_amd_PagedCache_reconstruct(res._h, self._ref, shape[0], blocks.data_ptr() or None, _FLOAT[dtype],
+                                                          k.data_ptr() or None, v.data_ptr() or None, _stream(res)))
+        return k, v
+
+    def attend(self, q, block_table, lengths, query_offsets=None, scale=None, causal=True, max_queries=None, out=None,
+               return_lse=False):
+        """Attention of q [tokens, heads, head_dim] (float16 / bfloat16) over the cache -> out (, lse [tokens, heads]).
+
+        block_table [batch, columns], lengths [batch] (int32): each request's blocks and tokens, its new ones included; request
+        b's queries are the rows query_offsets[b] ... query_offsets[b + 1] - 1 (int32 [batch + 1]; None: row b) and stand at
+        its end.  scale: 1 / sqrt(head_dim) by default.  max_queries: an upper bound of a request's queries, which saves
+        work that only longer ones need.  Rows of no request are left as they are in `out` (zero if it is None)."""
+        res = self.res
+        _tensor(res, q, "q", None, 3, dense=False)
+        if q.dtype not in _HALF:
+            raise TypeError("q must be float16 or bfloat16")
+        t, h, d = q.shape
+        if d != self.head_dim or h < 1 or h % self.num_heads:
+            raise ValueError("q must be [tokens, a multiple of %d, %d]" % (self.num_heads, self.head_dim))
+        _dense_last(q, "q")
+        _rows(res, block_table, "block_table")
+        n = block_table.shape[0]
+        _same_length(_tensor(res, lengths, "lengths", torch.int32, 1), n, "lengths")
+        if query_offsets is None:
+            if t != n:
+                raise ValueError("without query_offsets q must have one row per request")
+            most = 1
+        else:
+            _same_length(_tensor(res, query_offsets, "query_offsets", torch.int32, 1), n + 1, "query_offsets")
+            most = t if max_queries is None else int(max_queries)
+        if out is None:
+            out = torch.empty((t, h, d), dtype=q.dtype, device=q.device) if query_offsets is None else torch.zeros(
+                (t, h, d), dtype=q.dtype, device=q.device)
+        else:
+            _tensor(res, out, "out", q.dtype, 3, dense=False)
+            if out.shape != q.shape:
+                raise ValueError("out must have the shape of q")
+            _dense_last(out, "out")
+        lse = None
+        if return_lse:
+            lse = torch.full((t, h), -math.inf, device=q.device)
+        a = _AttendStruct(q.data_ptr() or None, out.data_ptr() or None, lse.data_ptr() if return_lse else None, q.stride(0), q.stride(1),
+                          out.stride(0), out.stride(1), block_table.data_ptr() or None, _row_stride(block_table), lengths.data_ptr() or None,
+                          query_offsets.data_ptr() if query_offsets is not None else None, n, t, h, block_table.shape[1],
+                          max(most, 0), _HALF[q.dtype], 1 if causal else 0, 1.0 / math.sqrt(d) if scale is None else float(scale),
+                          None, 0)
+        lib, ref = self._lib, _byref(a)
+        size = _SZ(0)
+        _check(lib.faiss_amd_PagedCache_attend_workspace(res._h, self._ref, ref, _byref(size)))
+        if size.value:
+            ws = torch.empty(size.value, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspaceBytes = ws.data_ptr(), size.value
+        _check(lib.faiss_amd_PagedCache_attend(res._h, self._ref, ref, _stream(res)))
+        return (out, lse) if return_lse else out
+
+
+def beam_select(res, logits, scores, num_beams, finished=None, pad_token=0):
+    """The num_beams best of each batch item's candidates beam x token -> (scores float32, parents int32, tokens int32), each
+    [batch, num_beams], best first, ties to the lowest beam, then the lowest token (faiss_amd_beam_select).
+
+    logits [batch, beams, vocab] (float32 / float16 / bfloat16), scores [batch, beams] float32; finished [batch, beams] (bool):
+    such a beam's only candidate is pad_token with its score unchanged.  Fewer candidates: score -inf, parent and token -1."""
+    _tensor(res, logits, "logits", None, 3, dense=False)
+    if logits.dtype not in _FLOAT:
+        raise TypeError("logits must be float32, float16 or bfloat16")
+    n, w, v = logits.shape
+    _dense_last(logits, "logits")
+    if tuple(_tensor(res, scores, "scores", torch.float32, 2).shape) != (n, w):
+        raise ValueError("scores must have the shape %s" % ((n, w),))
+    if finished is not None:
+        if finished.dtype not in (torch.bool, torch.uint8):
+            raise TypeError("finished must be bool or uint8")
+        if tuple(_tensor(res, finished, "finished", None, 2).shape) != (n, w):
+            raise ValueError("finished must have the shape %s" % ((n, w),))
+    k = int(num_beams)
+    dev = logits.device
+    if k < 1:
+        raise ValueError("num_beams must be in [1, 64]")
+    out = torch.empty((n, k), device=dev)
+    which = torch.empty((2, n, k), dtype=torch.int32, device=dev)
+    parents, tokens = which[0], which[1]
+    a = _BeamStruct(logits.data_ptr() or None, logits.stride(0), logits.stride(1), scores.data_ptr() or None,
+                    finished.data_ptr() if finished is not None else None, out.data_ptr() or None, parents.data_ptr() or None,
+                    tokens.data_ptr() or None, v, n, w, k, int(pad_token), _FLOAT[logits.dtype], None, 0)
+    lib, ref = res._lib, _byref(a)
+    size = _SZ(0)
+    _check(lib.faiss_amd_beam_select_workspace(res._h, ref, _byref(size)))
+    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspaceBytes = ws.data_ptr() or None, size.value
+    _check(lib.faiss_amd_beam_select(res._h, ref, _stream(res)))
+    return out, parents, tokens
+
+
+def reorder_beams(res, states, parents):
+    """states: tensors [batch, beams, ...] of any type -> new tensors [batch, num, ...] with out[b, j] = state[b, parents[b, j]]
+    (parents [batch, num] int32; a row whose parent is out of range becomes zero).  A state's rows must be dense."""
+    _tensor(res, parents, "parents", torch.int32, 2)
+    n, k = parents.shape
+    arr = (_StateStruct * len(states))()
+    outs, w = [], None
+    for i, t in enumerate(states):
+        _tensor(res, t, "states[%d]" % i, dense=False)
+        if t.dim() < 2 or t.shape[0] != n:
+            raise ValueError("states[%d] must be [%d, beams, ...]" % (i, n))
+        if w is None:
+            w = t.shape[1]
+        if t.shape[1] != w or w < 1:
+            raise ValueError("the states must have the same number of beams")
+        if not t[:1, :1].is_contiguous():
+            raise ValueError("the rows of states[%d] must be dense" % i)
+        out = torch.empty((n, k) + tuple(t.shape[2:]), dtype=t.dtype, device=t.device)
+        outs.append(out)
+        size = t.element_size()
+        arr[i] = _StateStruct(t.data_ptr() or None, out.data_ptr() or None, t.stride(0) * size, t.stride(1) * size,
+                              math.prod(t.shape[2:]) * size)
+    if outs:
+        _check(res._lib.faiss_amd_reorder_beams(res._h, len(outs), arr, parents.data_ptr() or None, n, w, k, _stream(res)))
+    return outs
+
+
+def fork_blocks(res, caches, block_table, lengths, spare, parents):
+    """Reorders beams over paged caches (all the layers that block_table leads to): row b * beams + j takes over the blocks of row
+    b * beams + parents[b, j]; full blocks are shared, a partly filled last one is copied into the row's spare block.  ->
+    new (block_table, lengths, spare).  block_table [batch * beams, columns], lengths, spare [batch * beams], parents [batch,
+    beams], all int32 (faiss_amd_fork_blocks)."""
+    _rows(res, block_table, "block_table")
+    _tensor(res, parents, "parents", torch.int32, 2)
+    n, w = parents.shape
+    rows, cols = block_table.shape
+    if rows != n * w:
+        raise ValueError("block_table must have batch * beams = %d rows" % (n * w))
+    for t, name in ((lengths, "lengths"), (spare, "spare")):
+        _same_length(_tensor(res, t, name, torch.int32, 1), rows, name)
+    if not caches:
+        raise ValueError("at least one cache")
+    for c in caches:
+        if c.res.device != res.device:
+            raise ValueError("the caches must be on the resources' device")
+    dev = block_table.device
+    table, lens, sp = (torch.empty((rows, cols), dtype=torch.int32, device=dev), torch.empty(rows, dtype=torch.int32, device=dev),
+                       torch.empty(rows, dtype=torch.int32, device=dev))
+    arr = (_CacheStruct * len(caches))(*[c._s for c in caches])
+    a = _ForkStruct(block_table.data_ptr() or None, _row_stride(block_table), lengths.data_ptr() or None, spare.data_ptr() or None,
+                    parents.data_ptr() or None, table.data_ptr() or None, lens.data_ptr() or None, sp.data_ptr() or None, n, w, cols)
+    if rows:
+        _check(res._lib.faiss_amd_fork_blocks(res._h, len(caches), arr, _byref(a), _stream(res)))
+    return table, lens, sp

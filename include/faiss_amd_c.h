@@ -474,6 +474,137 @@ int faiss_amd_GpuIndexIVF_last_scan_arith(const FaissAmdIndex* index, int* p_ari
 /* *p_output = 1 when mode 0 sends a batch of n queries with this nprobe and k through the list-major scan */
 int faiss_amd_GpuIndexIVF_list_major_rule(const FaissAmdIndex* index, int64_t n, int nprobe, int64_t k, int* p_output);
 
+/* ---- operators for a program that decodes with a model next to its searches: an 8-bit paged cache of keys and values, the block
+ *      tables that lead to it, attention over it, beam selection and reordering.  No counterpart in the reference; they stand
+ *      beside the operators of the same kinds above (8-bit codes of the scalar quantizer, k-selection, bfKnn over raw pointers).
+ *      Every pointer is device memory of res's device.  `stream` is the hipStream_t the call's work is ordered on (NULL: the
+ *      device's null stream); nothing is synchronised or allocated, scratch is the caller's, so every call can be captured into
+ *      a graph.  The calling thread's current device is left as it was.  Arrays of numbers the host cannot see (lengths,
+ *      offsets, block ids, slots, parents) are checked on the device as stated at each call.
+ *
+ *      The cache of one layer: keys   [numBlocks][numHeads][blockSize][headDim], one byte each, 16-byte aligned
+ *                              values [numBlocks][numHeads][headDim][blockSize], one byte each, 16-byte aligned
+ *                              keyScales, valueScales [numBlocks][numHeads]; a value is code * scale.
+ *      code: 0 = int8, 1 = e4m3; blockSize: 16, 32, 64, 128, 256; headDim: 64, 96, 128, 192, 256; numBlocks * blockSize < 2^31.
+ *      Types of other operands: 1 = F32, 2 = F16, 3 = BF16 (DistanceDataType). */
+typedef struct FaissAmdPagedCache {
+    void *keys, *values;
+    float *keyScales, *valueScales;
+    int code, numBlocks, blockSize, numHeads, headDim;
+} FaissAmdPagedCache;
+
+/* Block tables and slot maps from request lengths.  blockTable [batch][tableStride] (numColumns used) lists each request's
+ * blocks; lengths / newLengths [batch] are its tokens now and afterwards; freeRing [numBlocks] with freeState {front, count}
+ * holds the free blocks.  In request order, blocks are taken from the ring's front (returned behind its end when a request
+ * shrinks; blocks returned by a call are not handed out by the same call), and each new token gets a slot block * blockSize +
+ * offset.  A request is granted (granted[b] = 1) if the blocks and slots asked for up to and with it are there; a request that
+ * is not -- also one whose lengths are negative or beyond numColumns * blockSize -- keeps its length and gets no slots.
+ * queryOffsets [batch + 1]: where each request's new tokens begin; slots [maxTokens]: -1 behind the last one and where the
+ * table names no block.  ownedTable (nullable, same shape): new blocks are noted there too and returned blocks are read from
+ * there -- for tables that faiss_amd_fork_blocks has made share blocks.  lengthsOut / freeStateOut may be lengths / freeState.
+ * workspace: 4 * batch + 2 ints. */
+typedef struct FaissAmdPlanBlocksParams {
+    int* blockTable;
+    int* ownedTable;
+    int64_t tableStride, ownedStride;
+    const int *lengths, *newLengths;
+    int* freeRing;
+    const int64_t* freeState;
+    int* lengthsOut;
+    int64_t* freeStateOut;
+    int *queryOffsets, *slots, *granted, *workspace;
+    int batch, numColumns, numBlocks, blockSize, maxTokens;
+} FaissAmdPlanBlocksParams;
+int faiss_amd_plan_blocks(FaissAmdGpuResources* res, const FaissAmdPlanBlocksParams* args, void* stream);
+
+/* Adds tokens to the cache: keys / values [tokens][numHeads][headDim] (F16 or BF16, strides in elements, the last dimension
+ * dense), slots [tokens] (a slot outside the cache, like -1, is skipped; of several tokens for one slot the last counts).  A
+ * (block, head)'s scale is the smallest power of two with which its elements stay within 448 (e4m3) or 127 (int8) and never
+ * shrinks; when it grows, the block's other codes are re-expressed.  A token at offset 0 begins its block anew: the old scale
+ * is forgotten and every offset that the call does not write becomes zero.  An element that is no finite number makes its
+ * block's scale for that head NaN until the block is begun anew. */
+typedef struct FaissAmdCacheAddParams {
+    const void *keys, *values;
+    int64_t keyTokenStride, keyHeadStride, valueTokenStride, valueHeadStride;
+    const int* slots;
+    int tokens, type;
+} FaissAmdCacheAddParams;
+int faiss_amd_PagedCache_add(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdCacheAddParams* args, void* stream);
+
+/* Reads blocks back: keys, values [n][numHeads][blockSize][headDim] of the given type; NaN for a block id out of range. */
+int faiss_amd_PagedCache_reconstruct(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, int n, const int* blocks, int type,
+                                     void* keys, void* values, void* stream);
+
+/* Attention: out[r][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q[r][h] . k_j), query head h over key-value head
+ * h / (heads / numHeads).  Request b's queries are the rows queryOffsets[b] ... queryOffsets[b + 1] - 1 (NULL: row b; offsets
+ * must not decrease and are clamped to `tokens`); they are its last ones: query i of n sees the tokens j <= length - n + i if
+ * causal, all `length` tokens otherwise.  A row that sees nothing is zero (lse -inf); rows of no request are left as they
+ * are.  A row that sees a block id out of range (or tokens behind the table's last column) is NaN.  lse (nullable)
+ * [tokens][heads]: log sum_j p_j.  q / out: F16 or BF16, strides in elements, the last dimension dense.  maxQueries: an upper
+ * bound of a request's queries; a smaller one costs time, not results.  workspace (may be NULL when its size is 0): at least
+ * faiss_amd_PagedCache_attend_workspace bytes, 256-byte aligned. */
+typedef struct FaissAmdAttendParams {
+    const void* queries;
+    void* out;
+    float* lse;
+    int64_t queryTokenStride, queryHeadStride, outTokenStride, outHeadStride;
+    const int* blockTable;
+    int64_t tableStride;
+    const int *lengths, *queryOffsets;
+    int batch, tokens, heads, numColumns, maxQueries, type, causal;
+    float scale;
+    void* workspace;
+    size_t workspaceBytes;
+} FaissAmdAttendParams;
+int faiss_amd_PagedCache_attend(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdAttendParams* args, void* stream);
+int faiss_amd_PagedCache_attend_workspace(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdAttendParams* args,
+                                          size_t* p_bytes);
+
+/* Beam search's selection: of the candidates (w, v) of a batch item, value = scores[b][w] + logits[b][w][v] - log sum_u exp
+ * logits[b][w][u], the `keep` largest in order, ties to the lowest w, then the lowest v.  logits F32 / F16 / BF16 with strides in
+ * elements, the last dimension dense; finished (nullable, bytes [batch][beams]): such a beam's only candidate is (w, padToken)
+ * with the value scores[b][w].  Candidates of probability zero or without a number (a row with NaN or +inf) are none; where
+ * fewer than `keep` remain, score -inf, parent -1, token -1.  beams, keep <= 64.  Outputs [batch][keep]. */
+typedef struct FaissAmdBeamSelectParams {
+    const void* logits;
+    int64_t batchStride, beamStride;
+    const float* scores;
+    const uint8_t* finished;
+    float* outScores;
+    int *outParents, *outTokens;
+    int64_t vocab;
+    int batch, beams, keep, padToken, type;
+    void* workspace;
+    size_t workspaceBytes;
+} FaissAmdBeamSelectParams;
+int faiss_amd_beam_select(FaissAmdGpuResources* res, const FaissAmdBeamSelectParams* args, void* stream);
+int faiss_amd_beam_select_workspace(FaissAmdGpuResources* res, const FaissAmdBeamSelectParams* args, size_t* p_bytes);
+
+/* Reorders states of any type by parent: out[b][j] = in[b][parents[b][j]], rows of rowBytes bytes; a row whose parent is out of
+ * range becomes zero.  `states`: host array.  out is dense [batch][keep][rowBytes] and must not overlap any in. */
+typedef struct FaissAmdBeamState {
+    const void* in;
+    void* out;
+    int64_t batchBytes, beamBytes, rowBytes; /* strides of `in` */
+} FaissAmdBeamState;
+int faiss_amd_reorder_beams(FaissAmdGpuResources* res, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams,
+                            int keep, void* stream);
+
+/* Reorders beams over paged caches (`caches`: host array of n, all layers that the table leads to): row b * beams + j takes over
+ * the blocks of row b * beams + parents[b][j] (its own if that is out of range).  Full blocks are shared; a partly filled last
+ * block is copied into spare[row], which takes its place in the row's table, and the row's own last block becomes its spare
+ * one.  spare [batch * beams]: one block per row that no table names; the beams of a batch item have the same length.
+ * Outputs [batch * beams][numColumns], [batch * beams], [batch * beams] overlap no input.  A spare block out of range where
+ * one is needed: the row's table gets -1 there. */
+typedef struct FaissAmdForkBlocksParams {
+    const int* blockTable;
+    int64_t tableStride;
+    const int *lengths, *spare, *parents;
+    int *tableOut, *lengthsOut, *spareOut;
+    int batch, beams, numColumns;
+} FaissAmdForkBlocksParams;
+int faiss_amd_fork_blocks(FaissAmdGpuResources* res, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
