@@ -46,7 +46,7 @@ CacheView view(const FaissAmdPagedCache* c) {
                         "block size must be 16, 32, 64, 128 or 256");
     FA_THROW_IF_NOT_MSG(c->headDim == 64 || c->headDim == 96 || c->headDim == 128 || c->headDim == 192 || c->headDim == 256,
                         "head dimension must be 64, 96, 128, 192 or 256");
-    FA_THROW_IF_NOT_MSG(c->numHeads >= 1 && c->numHeads <= 65535, "number of heads out of range");
+    FA_THROW_IF_NOT_MSG(c->numHeads >= 1 && c->numHeads <= 32767, "number of heads out of range");
     FA_THROW_IF_NOT_MSG(c->numBlocks >= 1 && (int64_t)c->numBlocks * c->blockSize < ((int64_t)1 << 31), "number of blocks out of range");
     CacheView v;
     v.k = (uint8_t*)c->keys;

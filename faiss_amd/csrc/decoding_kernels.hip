@@ -9,6 +9,7 @@ namespace {
 typedef unsigned long long u64;
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ int lane64() {
     return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
@@ -199,127 +200,211 @@ __device__ __forceinline__ float pow2_scale(unsigned amax_bits) { // bits of a f
     return __builtin_bit_cast(float, (unsigned)(e + 127) << 23);
 }
 template <int CODE>
-__device__ __forceinline__ unsigned encode1(float x) {
-    if (CODE == CACHE_E4M3) return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xffu;
-    return (unsigned)(int)__builtin_rintf(x) & 0xffu;
+__device__ __forceinline__ unsigned encode4(float x0, float x1, float x2, float x3) {
+    if constexpr (CODE == CACHE_E4M3) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false);
+        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(x2, x3, w, true);
+    } else {
+        // x + 1.5 * 2^23 is rounded to an integer (half to even) that stands in the low bits, in two's complement
+        const float r = 12582912.f;
+        const unsigned a = __builtin_bit_cast(unsigned, x0 + r), b = __builtin_bit_cast(unsigned, x1 + r);
+        const unsigned c = __builtin_bit_cast(unsigned, x2 + r), d = __builtin_bit_cast(unsigned, x3 + r);
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0400u), __builtin_amdgcn_perm(b, a, 0x0c0c0400u), 0x05040100u);
+    }
 }
 template <int CODE>
-__device__ __forceinline__ float decode1(unsigned byte) {
-    if (CODE == CACHE_E4M3) return __builtin_amdgcn_cvt_f32_fp8((int)byte, 0);
-    return (float)(int)(signed char)byte;
+__device__ __forceinline__ void decode4(unsigned w, float x[4]) {
+    if constexpr (CODE == CACHE_E4M3) {
+        x[0] = __builtin_amdgcn_cvt_f32_fp8((int)w, 0);
+        x[1] = __builtin_amdgcn_cvt_f32_fp8((int)w, 1);
+        x[2] = __builtin_amdgcn_cvt_f32_fp8((int)w, 2);
+        x[3] = __builtin_amdgcn_cvt_f32_fp8((int)w, 3);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = (float)(int)(signed char)(w >> (8 * i));
+    }
 }
-// the four codes of a word multiplied by ratio <= 1 and rounded
+// the four codes of a word multiplied by ratio < 1 and rounded
 template <int CODE>
 __device__ __forceinline__ unsigned rescale4(unsigned w, float ratio) {
-    unsigned r = 0;
+    float x[4];
+    decode4<CODE>(w, x);
+    return encode4<CODE>(x[0] * ratio, x[1] * ratio, x[2] * ratio, x[3] * ratio);
+}
+// four words of four bytes, transposed: byte j of word i becomes byte i of word j
+__device__ __forceinline__ void transpose4(unsigned w[4]) {
+    const unsigned a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u);
+    const unsigned c = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+    w[0] = __builtin_amdgcn_perm(c, a, 0x05040100u);
+    w[1] = __builtin_amdgcn_perm(c, a, 0x07060302u);
+    w[2] = __builtin_amdgcn_perm(d, b, 0x05040100u);
+    w[3] = __builtin_amdgcn_perm(d, b, 0x07060302u);
+}
+// eight adjacent elements of 16 bits; VEC: they are 16-byte aligned
+template <bool VEC>
+__device__ __forceinline__ u32x4 elems8(const void* p, int64_t at) {
+    if (VEC) return *(const u32x4*)((const unsigned short*)p + at);
+    unsigned short u[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) r |= encode1<CODE>(decode1<CODE>((w >> (8 * i)) & 0xffu) * ratio) << (8 * i);
+    for (int i = 0; i < 8; ++i) u[i] = ((const unsigned short*)p)[at + i];
+    u32x4 r;
+    __builtin_memcpy(&r, u, 16);
     return r;
 }
-__device__ __forceinline__ float elem(const void* p, int64_t i, int type) {
-    const unsigned short u = ((const unsigned short*)p)[i];
-    return type == DT_F16 ? (float)__builtin_bit_cast(_Float16, u) : __builtin_bit_cast(float, (unsigned)u << 16);
+template <int CODE>
+__device__ __forceinline__ u32x2 encode8(u32x4 raw, int type, float inv) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned lo = raw[i] & 0xffffu, hi = raw[i] >> 16;
+        x[2 * i] = (type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)lo) : __builtin_bit_cast(float, lo << 16)) * inv;
+        x[2 * i + 1] = (type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)hi) : __builtin_bit_cast(float, hi << 16)) * inv;
+    }
+    return u32x2{encode4<CODE>(x[0], x[1], x[2], x[3]), encode4<CODE>(x[4], x[5], x[6], x[7])};
 }
 
-// A workgroup per token; the first token of each block stays and serves all the call's tokens of that block (found by a scan over
-// the slots, so a block's tokens may stand anywhere in the call; of several tokens for one slot the last wins).  A wavefront
-// takes one head's keys or values at a time: largest element, scale, codes.
-template <int CODE>
-__global__ __launch_bounds__(256) void cache_add_kernel(AddArgs a) {
+// blockIdx.y: SG units, a unit being the keys or the values of a head, each with NT threads.  blockIdx.x: `chunk` tokens of the call.  Where a token's block differs from its
+// predecessor's the workgroup scans the call's slots for all tokens of that block: if none comes earlier it serves them (a block's
+// tokens may stand anywhere in the call; of several tokens for one slot the last wins), else another workgroup does.
+// Keys are written as 8 dimensions of a token, values as 4 tokens of 8 dimensions: 4 x 4 bytes are transposed in registers, so
+// that both layouts get words (16389 tokens of 8 x 128, int8, blocks of 64: see the table of times).
+template <int CODE, bool VEC, int NT, int SG>
+__global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk) {
     const CacheView& c = a.cache;
-    const int bs = c.blockSize, D = c.headDim, H = c.numHeads;
-    const int me = blockIdx.x;
+    const int bs = c.blockSize, D = c.headDim, H = c.numHeads, oct = D / 8;
     const int64_t nslots = (int64_t)c.numBlocks * bs;
-    const int slot = a.slots[me];
-    if (slot < 0 || slot >= nslots) return;
-    const int block = slot / bs;
-    if (me > 0) {
-        const int before = a.slots[me - 1];
-        if (before >= 0 && before / bs == block) return;
-    }
-    __shared__ int token[kMaxBlockSize];
+    const int lane = threadIdx.x & 63, sub = threadIdx.x / NT, tid = threadIdx.x - sub * NT;
+    __shared__ __align__(16) int token[kMaxBlockSize];
     __shared__ int earlier;
-    for (int i = threadIdx.x; i < bs; i += 256) token[i] = -1;
-    if (threadIdx.x == 0) earlier = 0;
-    __syncthreads();
-    const int first = block * bs;
-    for (int j = threadIdx.x; j < a.tokens; j += 256) {
-        const unsigned o = (unsigned)(a.slots[j] - first);
-        if (o < (unsigned)bs) {
-            atomicMax(&token[o], j);
-            if (j < me) earlier = 1;
+    __shared__ unsigned part[SG][NT / 64];
+    const int t0 = blockIdx.x * chunk, t1 = min(t0 + chunk, a.tokens);
+    // a lane per token of the chunk (every wavefront the same): does a run of one block's tokens begin here?
+    const int shift = 31 - __builtin_clz(bs);
+    const int mine = t0 + lane < t1 ? a.slots[t0 + lane] : -1, prev = t0 + lane < t1 && t0 + lane > 0 ? a.slots[t0 + lane - 1] : -1;
+    u64 begins = __ballot(mine >= 0 && mine < nslots && (prev < 0 || (prev >> shift) != (mine >> shift)));
+    for (; begins; begins &= begins - 1) {
+        const int me = t0 + __ffsll((long long)begins) - 1;
+        const int block = __builtin_amdgcn_readlane(mine, me - t0) >> shift;
+        __syncthreads();
+        for (int i = threadIdx.x; i < bs; i += NT * SG) token[i] = -1;
+        if (threadIdx.x == 0) earlier = 0;
+        __syncthreads();
+        const int first = block * bs;
+        for (int j0 = threadIdx.x; j0 < a.tokens; j0 += 8 * NT * SG) { // eight loads in flight: the scan is latency, not bytes
+            int s[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[e] = j0 + NT * SG * e < a.tokens ? a.slots[j0 + NT * SG * e] : -1;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int j = j0 + NT * SG * e;
+                const unsigned o = (unsigned)(s[e] - first); // (-1 - first >= bs as an unsigned number)
+                if (o < (unsigned)bs) {
+                    atomicMax(&token[o], j);
+                    if (j < me) earlier = 1;
+                }
+            }
         }
-    }
-    __syncthreads();
-    if (earlier) return;
-    const bool fresh = token[0] >= 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int unit = wave; unit < 2 * H; unit += 4) {
+        __syncthreads();
+        if (earlier) continue;
+        const bool fresh = token[0] >= 0;
+        const int unit = blockIdx.y * SG + sub;
+        const bool live = unit < 2 * H;
         const bool isV = unit >= H;
-        const int h = isV ? unit - H : unit;
+        const int h = !live ? 0 : isV ? unit - H : unit;
         const void* x = isV ? a.value : a.key;
         const int64_t ts = isV ? a.valueTokenStride : a.keyTokenStride, base = (int64_t)h * (isV ? a.valueHeadStride : a.keyHeadStride);
-        unsigned big = 0;
-        for (int o = 0; o < bs; ++o) {
-            const int t = token[o];
-            if (t < 0) continue;
-            for (int d = lane; d < D; d += 64)
-                big = max(big, __builtin_bit_cast(unsigned, elem(x, base + t * ts + d, a.type)) & 0x7fffffffu);
+        // a thread's piece: 4 tokens x 8 dimensions; neighbours hold the next dimensions (keys), the next tokens (values)
+        const int quads = bs / 4, pieces = quads * oct; // (pieces <= 2048: i / oct by a reciprocal is exact)
+        const unsigned recip = 65536 / oct + 1;
+        auto piece = [&](int i, int& q, int& o) {
+            q = isV ? i & (quads - 1) : (int)((i * recip) >> 16);
+            o = isV ? i >> (shift - 2) : i - q * oct;
+        };
+        auto load = [&](int q, int o, u32x4 (&raw)[4]) {
+            const int4 t = *(const int4*)&token[4 * q];
+            const int tt[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[e] = elems8<VEC>(x, base + max(tt[e], t0) * ts + 8 * o);
+            if (min(min(tt[0], tt[1]), min(tt[2], tt[3])) < 0) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) raw[e] = tt[e] >= 0 ? raw[e] : u32x4{0u, 0u, 0u, 0u};
+            }
+        };
+        // largest element: sixteen bits without the sign order like the numbers
+        u32x4 raw[4];
+        u16x2 most = {0, 0};
+        for (int i = tid; i < (live ? pieces : 0); i += NT) {
+            int q, o;
+            piece(i, q, o);
+            load(q, o, raw);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, raw[e][w] & 0x7fff7fffu));
         }
+        unsigned big = max(most[0], most[1]);
 #pragma unroll
         for (int o = 32; o; o >>= 1) big = max(big, (unsigned)__shfl_xor((int)big, o, 64));
+        if (lane == 0) part[sub][tid >> 6] = big;
         float* sp = (isV ? c.vs : c.ks) + (int64_t)block * H + h;
         const float old = *sp;
+        __syncthreads(); // (and every thread has read the old scale)
+        for (int w = 0; w < NT / 64; ++w) big = max(big, part[sub][w]);
+        const float amax = a.type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)big) : __builtin_bit_cast(float, big << 16);
         const float before = fresh ? 0.f : old;
         float after = __builtin_nanf("");
         // anything that is no number makes the block's scale, and with it all its values, no number until the block is begun anew
-        if (big < 0x7f800000u && before >= 0.f && before < INFINITY) after = fmaxf(before, pow2_scale<CODE>(big));
+        if (amax < INFINITY && before >= 0.f && before < INFINITY) after = fmaxf(before, pow2_scale<CODE>(__builtin_bit_cast(unsigned, amax)));
         const bool number = after == after;
         const float inv = number && after > 0.f ? 1.f / after : 0.f;
         const float ratio = after > 0.f ? before / after : 0.f;
-        const bool rescale = fresh || (number && ratio != 1.f);
+        const bool rescale = fresh || (number && ratio != 1.f), clear = rescale && ratio == 0.f;
         uint8_t* codes = (isV ? c.v : c.k) + ((int64_t)block * H + h) * (int64_t)bs * D;
-        if (!isV) {
-            for (int o = 0; o < bs; ++o) {
-                const int t = token[o];
-                if (t < 0 && !rescale) continue;
-                for (int d = 4 * lane; d < D; d += 256) {
-                    unsigned* p = (unsigned*)(codes + (int64_t)o * D + d);
-                    unsigned w = 0;
-                    if (t >= 0) {
-                        if (number)
-                            for (int i = 0; i < 4; ++i) w |= encode1<CODE>(elem(x, base + t * ts + d + i, a.type) * inv) << (8 * i);
-                    } else {
-                        w = ratio == 0.f ? 0u : rescale4<CODE>(*p, ratio);
-                    }
-                    *p = w;
-                }
-            }
-        } else {
-            for (int g = 0; g < bs; g += 16) {
-                unsigned have = 0;
-                for (int i = 0; i < 16; ++i) have |= token[g + i] >= 0 ? 1u << i : 0u;
-                if (!have && !rescale) continue;
-                for (int d = lane; d < D; d += 64) {
-                    u32x4* p = (u32x4*)(codes + (int64_t)d * bs + g);
-                    u32x4 w = {0u, 0u, 0u, 0u};
-                    if (have != 0xffffu && !(rescale && ratio == 0.f)) w = *p;
+        for (int i = tid; i < (live ? pieces : 0); i += NT) {
+            int q, o;
+            piece(i, q, o);
+            const int4 t = *(const int4*)&token[4 * q];
+            const int tt[4] = {t.x, t.y, t.z, t.w};
+            unsigned mask = 0; // tokens that are written
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (rescale && ratio != 0.f) w[i] = rescale4<CODE>(w[i], ratio);
+            for (int e = 0; e < 4; ++e) mask |= tt[e] >= 0 ? 0xffu << (8 * e) : 0u;
+            if (!mask && !rescale) continue;
+            if (pieces > NT) load(q, o, raw); // (else it is still there)
+            u32x2 w[4];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int t = token[g + 4 * i + e];
-                            if (t < 0) continue;
-                            const unsigned b = number ? encode1<CODE>(elem(x, base + t * ts + d, a.type) * inv) : 0u;
-                            w[i] = (w[i] & ~(0xffu << (8 * e))) | (b << (8 * e));
+            for (int e = 0; e < 4; ++e) w[e] = number ? encode8<CODE>(raw[e], a.type, inv) : u32x2{0u, 0u};
+            if (!isV) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    u32x2* p = (u32x2*)(codes + (int64_t)(4 * q + e) * D + 8 * o);
+                    if (tt[e] < 0) {
+                        if (!rescale) continue;
+                        if (!clear) {
+                            const u32x2 was = *p;
+                            w[e] = u32x2{rescale4<CODE>(was[0], ratio), rescale4<CODE>(was[1], ratio)};
                         }
                     }
-                    *p = w;
+                    *p = w[e];
+                }
+            } else {
+                unsigned lo[4] = {w[0][0], w[1][0], w[2][0], w[3][0]}, hi[4] = {w[0][1], w[1][1], w[2][1], w[3][1]};
+                transpose4(lo);
+                transpose4(hi);
+                unsigned* p = (unsigned*)(codes + (int64_t)(8 * o) * bs + 4 * q);
+                unsigned was[8];
+                if (mask != ~0u && !clear) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) was[e] = p[e * (bs / 4)];
+                }
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    unsigned now = e < 4 ? lo[e & 3] : hi[e & 3];
+                    if (mask != ~0u && !clear) now = (now & mask) | ((rescale ? rescale4<CODE>(was[e], ratio) : was[e]) & ~mask);
+                    p[e * (bs / 4)] = now;
                 }
             }
         }
-        if (lane == 0) *sp = after;
+        if (live && tid == 0) *sp = after;
     }
 }
 
@@ -332,31 +417,50 @@ __device__ __forceinline__ _Float16 narrow<_Float16>(float x) { return (_Float16
 template <>
 __device__ __forceinline__ __bf16 narrow<__bf16>(float x) { return (__bf16)x; }
 
-// a workgroup per (block, head)
+template <int CODE, typename T>
+__device__ __forceinline__ void store8(T* p, unsigned lo, unsigned hi, float scale) {
+    float x[8];
+    decode4<CODE>(lo, x);
+    decode4<CODE>(hi, x + 4);
+    T r[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = narrow<T>(x[e] * scale);
+    __builtin_memcpy(__builtin_assume_aligned(p, 16), r, 8 * sizeof(T));
+}
+
+// a workgroup per (block, head), the keys or the values of it (blockIdx.y); the values' bytes are transposed as cache_add_kernel does
 template <int CODE, typename T>
 __global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs a) {
     const CacheView& c = a.cache;
-    const int bs = c.blockSize, D = c.headDim, H = c.numHeads;
+    const int bs = c.blockSize, D = c.headDim, H = c.numHeads, oct = D / 8;
     const int i = blockIdx.x / H, h = blockIdx.x - i * H;
     const int block = a.blocks[i];
-    T* ko = (T*)a.key + (int64_t)blockIdx.x * bs * D;
-    T* vo = (T*)a.value + (int64_t)blockIdx.x * bs * D;
-    if ((unsigned)block >= (unsigned)c.numBlocks) { // no such block: no such values
-        for (int x = threadIdx.x; x < bs * D; x += 256) ko[x] = vo[x] = narrow<T>(__builtin_nanf(""));
-        return;
-    }
-    const int64_t at = (int64_t)block * H + h;
-    const float ks = c.ks[at], vs = c.vs[at];
-    const uint8_t* kc = c.k + at * bs * D;
-    const uint8_t* vc = c.v + at * bs * D;
-    for (int x = 4 * threadIdx.x; x < bs * D; x += 1024) {
-        const unsigned w = *(const unsigned*)(kc + x);
+    const bool isV = blockIdx.y == 1;
+    T* out = (T*)(isV ? a.value : a.key) + (int64_t)blockIdx.x * bs * D;
+    const bool none = (unsigned)block >= (unsigned)c.numBlocks; // no such block: no such values
+    const int64_t at = none ? 0 : (int64_t)block * H + h;
+    const float scale = none ? __builtin_nanf("") : isV ? c.vs[at] : c.ks[at];
+    const uint8_t* codes = (isV ? c.v : c.k) + at * bs * D;
+    if (!isV) {
+        for (int x = threadIdx.x; x < bs * oct; x += 256) {
+            const u32x2 w = *(const u32x2*)(codes + 8 * x);
+            store8<CODE>(out + 8 * x, w[0], w[1], scale);
+        }
+    } else {
+        const int quads = bs / 4;
+        for (int x = threadIdx.x; x < quads * oct; x += 256) {
+            const int q = x / oct, o = x - q * oct;
+            unsigned lo[4], hi[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) ko[x + e] = narrow<T>(decode1<CODE>((w >> (8 * e)) & 0xffu) * ks);
-    }
-    for (int x = threadIdx.x; x < bs * D; x += 256) {
-        const int t = x / D, d = x - t * D;
-        vo[x] = narrow<T>(decode1<CODE>(vc[(int64_t)d * bs + t]) * vs);
+            for (int e = 0; e < 4; ++e) {
+                lo[e] = *(const unsigned*)(codes + (int64_t)(8 * o + e) * bs + 4 * q);
+                hi[e] = *(const unsigned*)(codes + (int64_t)(8 * o + 4 + e) * bs + 4 * q);
+            }
+            transpose4(lo);
+            transpose4(hi);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store8<CODE>(out + (int64_t)(4 * q + e) * D + 8 * o, lo[e], hi[e], scale);
+        }
     }
 }
 
@@ -748,18 +852,36 @@ void launch_plan_blocks(const PlanArgs& a, hipStream_t stream) {
     HIP_CHECK(hipGetLastError());
 }
 
+template <int CODE>
+static void launch_add(const AddArgs& a, bool vec, hipStream_t stream) {
+    // a workgroup per token while there are few (each is a block of its own in a decoding step), 16 tokens of a prompt's runs
+    const int chunk = a.tokens <= 1024 ? 1 : 32;
+    const unsigned gx = (unsigned)div_up(a.tokens, chunk), units = 2 * a.cache.numHeads;
+    // one wavefront per unit where a block is small work; the scan over many slots is shared by four units
+    const bool small = chunk == 1 && a.cache.blockSize * a.cache.headDim <= 8192;
+    if (!vec)
+        cache_add_kernel<CODE, false, 256, 1><<<dim3(gx, units), 256, 0, stream>>>(a, chunk);
+    else if (small)
+        cache_add_kernel<CODE, true, 64, 1><<<dim3(gx, units), 64, 0, stream>>>(a, chunk);
+    else if (chunk == 1)
+        cache_add_kernel<CODE, true, 256, 1><<<dim3(gx, units), 256, 0, stream>>>(a, chunk);
+    else
+        cache_add_kernel<CODE, true, 256, 4><<<dim3(gx, (unsigned)div_up(units, 4)), 1024, 0, stream>>>(a, chunk);
+}
 void launch_cache_add(const AddArgs& a, hipStream_t stream) {
     if (a.tokens == 0) return;
+    const bool vec = ((uintptr_t)a.key | (uintptr_t)a.value) % 16 == 0 &&
+            (a.keyTokenStride | a.keyHeadStride | a.valueTokenStride | a.valueHeadStride) % 8 == 0;
     if (a.cache.code == CACHE_E4M3)
-        cache_add_kernel<CACHE_E4M3><<<a.tokens, 256, 0, stream>>>(a);
+        launch_add<CACHE_E4M3>(a, vec, stream);
     else
-        cache_add_kernel<CACHE_INT8><<<a.tokens, 256, 0, stream>>>(a);
+        launch_add<CACHE_INT8>(a, vec, stream);
     HIP_CHECK(hipGetLastError());
 }
 
 template <int CODE>
 static void launch_reconstruct(const ReconstructArgs& a, hipStream_t stream) {
-    const unsigned grid = (unsigned)((int64_t)a.n * a.cache.numHeads);
+    const dim3 grid((unsigned)((int64_t)a.n * a.cache.numHeads), 2);
     if (a.type == DT_F32)
         cache_reconstruct_kernel<CODE, float><<<grid, 256, 0, stream>>>(a);
     else if (a.type == DT_F16)
