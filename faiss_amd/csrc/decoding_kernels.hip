@@ -470,7 +470,8 @@ __global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs 
 // joins the pieces of a row, then the rows of a batch item.  The exponentials' sum is accumulated in 64 bits and candidates of
 // different beams are compared as 64-bit values: they come in the order of the exact values unless those agree to ~1e-8.
 constexpr int kBeamVpt = 16;                                   // logits per lane and step
-constexpr int kBeamCap = kMaxBeams + 64 * kBeamVpt;            // keys a wavefront may hold at once
+constexpr int kBeamPend = 128;                                 // keys a wavefront collects before it cuts them to `keep`
+constexpr int kBeamCap = kBeamPend + 64 * kBeamVpt / 2;        // keys a wavefront may hold at once
 constexpr int kBeamKeys = 2048;                                // keys of a row that the second launch joins
 
 struct BeamSched {
@@ -486,18 +487,49 @@ __device__ __forceinline__ u64 beam_key(float x, unsigned v) {
 }
 __device__ __forceinline__ float beam_logit(u64 key) { return float_unflip(~(unsigned)(key >> 32)); }
 
-// The `keep`-th smallest of the n unique keys in LDS (n > keep): bits from the top, one ballot per key and bit.
+// A bound that exactly `keep` of the n unique keys in LDS do not exceed (n > keep): bits from the top, a ballot per 64 keys and
+// bit.  The low half, which only tells equal logits apart, is looked at where they straddle the bound.
+template <int R>
+__device__ __forceinline__ u64 wave_kth_regs(const u64* list, int n, int keep) {
+    const int lane = lane64();
+    unsigned hi[R], lo[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const u64 k = 64 * r + lane < n ? list[64 * r + lane] : ~0ull;
+        hi[r] = (unsigned)(k >> 32);
+        lo[r] = (unsigned)k;
+    }
+    unsigned t = 0;
+    for (int b = 31; b >= 0; --b) {
+        const unsigned c = t | ((1u << b) - 1);
+        int cnt = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) cnt += __popcll(__ballot(hi[r] <= c));
+        if (cnt < keep) t |= 1u << b;
+    }
+    int below = 0, upto = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        below += __popcll(__ballot(hi[r] < t));
+        upto += __popcll(__ballot(hi[r] <= t));
+    }
+    if (upto == keep) return ((u64)t << 32) | ~0u;
+    unsigned u = 0;
+    for (int b = 31; b >= 0; --b) {
+        const unsigned c = u | ((1u << b) - 1);
+        int cnt = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) cnt += __popcll(__ballot(hi[r] == t && lo[r] <= c));
+        if (cnt < keep - below) u |= 1u << b;
+    }
+    return ((u64)t << 32) | u;
+}
 __device__ __forceinline__ u64 wave_kth(const u64* list, int n, int keep) {
+    if (n <= 64) return wave_kth_regs<1>(list, n, keep);
+    if (n <= 128) return wave_kth_regs<2>(list, n, keep);
+    if (n <= 256) return wave_kth_regs<4>(list, n, keep);
     const int lane = lane64();
     u64 t = 0;
-    if (n <= 64) {
-        const u64 k = lane < n ? list[lane] : ~0ull;
-        for (int b = 63; b >= 0; --b) {
-            const u64 c = t | ((1ull << b) - 1);
-            if (__popcll(__ballot(lane < n && k <= c)) < keep) t |= 1ull << b;
-        }
-        return t;
-    }
     for (int b = 63; b >= 0; --b) {
         const u64 c = t | ((1ull << b) - 1);
         int cnt = 0;
@@ -522,9 +554,6 @@ __device__ __forceinline__ int wave_cut(u64* list, int n, u64 kth) {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
     return out;
 }
-
-template <typename T>
-__device__ __forceinline__ float logit(T x) { return (float)x; }
 
 template <typename T>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s) {
@@ -552,75 +581,83 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s)
     const int64_t steps = (granules + 64 * LD - 1) / (64 * LD);
     u64* list = lists[wave];
     int n = 0;
-    u64 thr = ~0ull; // only keys below it can be among the best
+    float thr = -INFINITY; // only logits of at least this can be among the best; set once `keep` better ones are in the list
+    bool full = false;
     float m = -INFINITY;
     double sum = 0.0;
-    for (int64_t st = (int64_t)part * 4 + wave; st < steps; st += (int64_t)s.parts * 4) {
-        float v[kBeamVpt];
-        unsigned best = ~0u;
-        float mx = -INFINITY;
+    const int64_t stride = (int64_t)s.parts * 4;
+    T next[kBeamVpt];
+    auto fetch = [&](int64_t st) {
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
             const int64_t e0 = ((st * LD + i) * 64 + lane) * PER;
             if (e0 + PER <= a.vocab) {
-                T t[PER];
-                __builtin_memcpy(t, x + e0, 16);
-#pragma unroll
-                for (int e = 0; e < PER; ++e) v[i * PER + e] = logit(t[e]);
+                __builtin_memcpy(next + i * PER, x + e0, 16);
             } else {
 #pragma unroll
-                for (int e = 0; e < PER; ++e) {
-                    const int64_t at = e0 + e;
-                    v[i * PER + e] = at < a.vocab ? logit(x[at]) : -INFINITY;
-                }
+                for (int e = 0; e < PER; ++e) next[i * PER + e] = e0 + e < a.vocab ? x[e0 + e] : (T)-INFINITY;
             }
         }
-        bool odd = false; // a NaN
+    };
+    int64_t st = (int64_t)part * 4 + wave;
+    if (st < steps) fetch(st);
+    for (; st < steps; st += stride) {
+        float v[kBeamVpt];
 #pragma unroll
-        for (int i = 0; i < kBeamVpt; ++i) {
-            mx = fmaxf(mx, v[i]);
-            odd |= v[i] != v[i];
-            const unsigned k = v[i] > -INFINITY ? ~float_flip(v[i]) : ~0u;
-            best = min(best, k);
-        }
-        // running maximum and sum of the lane
+        for (int i = 0; i < kBeamVpt; ++i) v[i] = (float)next[i];
+        if (st + stride < steps) fetch(st + stride);
+        float mx = v[0];
+#pragma unroll
+        for (int i = 1; i < kBeamVpt; ++i) mx = fmaxf(mx, v[i]);
+        // running maximum and sum of the lane; a NaN or an infinity makes the sum NaN
         const float mn = fmaxf(m, mx);
-        if (mn > -INFINITY) {
-            float p = 0.f;
+        float p = 0.f;
 #pragma unroll
-            for (int i = 0; i < kBeamVpt; ++i) p += __builtin_amdgcn_exp2f((v[i] - mn) * 1.4426950408889634f);
+        for (int i = 0; i < kBeamVpt; ++i) p += __builtin_amdgcn_exp2f((v[i] - mn) * 1.4426950408889634f);
+        if (mn == -INFINITY) { // (nothing but -inf so far, or a NaN among it)
+            p = 0.f;
+#pragma unroll
+            for (int i = 0; i < kBeamVpt; ++i) p = v[i] == v[i] ? p : v[i];
+            sum += (double)p;
+        } else {
             sum = sum * (double)__builtin_amdgcn_exp2f((m - mn) * 1.4426950408889634f) + (double)p;
         }
-        if (odd) sum = __builtin_nan("");
         m = mn;
-        // candidates.  The keep-th best of the lanes' best logits bounds what can be among the keep best of this step.
-        unsigned lim = (unsigned)(thr >> 32);
-        if (thr == ~0ull) {
+        float lim = thr;
+        if (!full) {
+            // the keep-th best of the lanes' best logits bounds what can be among the keep best of this step
+            const unsigned best = mx > -INFINITY ? ~float_flip(mx) : ~0u;
             unsigned t = 0;
             for (int b = 31; b >= 0; --b) {
                 const unsigned c = t | ((1u << b) - 1);
                 if (__popcll(__ballot(best <= c)) < keep) t |= 1u << b;
             }
-            lim = t;
+            lim = t == ~0u ? -INFINITY : float_unflip(~t);
         }
-        if (!__ballot(best <= lim && best != ~0u)) continue;
+        if (!__ballot(mx >= lim && mx > -INFINITY)) continue;
 #pragma unroll
-        for (int i = 0; i < kBeamVpt; ++i) {
-            const unsigned k = v[i] > -INFINITY ? ~float_flip(v[i]) : ~0u;
-            const int64_t at = ((st * LD + i / PER) * 64 + lane) * PER + i % PER;
-            const u64 key = ((u64)k << 32) | (unsigned)at;
-            const bool in = k != ~0u && k <= lim && key < thr;
-            const u64 mask = __ballot(in);
-            if (!mask) continue;
-            if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = key;
-            n += __popcll(mask);
+        for (int half = 0; half < 2; ++half) {
+            if (n > kBeamPend) n = wave_cut(list, n, wave_kth(list, n, keep));
+#pragma unroll
+            for (int j = 0; j < kBeamVpt / 2; ++j) {
+                const int i = half * (kBeamVpt / 2) + j;
+                const bool in = v[i] >= lim && v[i] > -INFINITY;
+                const u64 mask = __ballot(in);
+                if (!mask) continue;
+                if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = beam_key(v[i], (unsigned)(((st * LD + i / PER) * 64 + lane) * PER + i % PER));
+                n += __popcll(mask);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
-        if (n > keep) {
-            thr = wave_kth(list, n, keep);
-            n = wave_cut(list, n, thr);
+        // a bound for the steps to come; renewed when there is something to gain from it
+        if (n > keep && (!full || n > kBeamPend / 2)) {
+            const u64 kth = wave_kth(list, n, keep);
+            n = wave_cut(list, n, kth);
+            thr = beam_logit(kth);
+            full = true;
         }
     }
+    if (n > keep) n = wave_cut(list, n, wave_kth(list, n, keep));
     // the wavefront's maximum and sum, then the workgroup's
     float M = m;
 #pragma unroll
@@ -665,14 +702,28 @@ constexpr int kBeamJoin = 1024;
 __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSched s) {
     __shared__ u64 val[kMaxBeams * kMaxBeams]; // double_flip of a candidate's value
     __shared__ unsigned tok[kMaxBeams * kMaxBeams];
-    __shared__ u64 lists[kBeamJoin / 64][256];
+    __shared__ int ranks[kMaxBeams * kMaxBeams];
+    __shared__ int valid;
+    __shared__ u64 lists[kBeamJoin / 64][256 + kMaxBeams];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, keep = a.keep, b = blockIdx.x;
+    const int total = a.beams * keep;
+    for (int i = threadIdx.x; i < total; i += kBeamJoin) ranks[i] = 0;
+    if (threadIdx.x == 0) valid = 0;
     for (int w = wave; w < a.beams; w += kBeamJoin / 64) {
         const int64_t row = (int64_t)b * a.beams + w;
+        const u64* keys = s.keys + row * s.parts * keep;
+        const int count = s.parts * keep;
+        // (the loads do not wait for one another: the launch is latency)
+        const bool fin = a.finished && a.finished[row];
         const double score = (double)a.scores[row];
+        float pm = lane < s.parts ? s.maxs[row * s.parts + lane] : -INFINITY;
+        double ps = lane < s.parts ? s.sums[row * s.parts + lane] : 0.0;
+        u64 first[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) first[j] = 64 * j + lane < count ? keys[64 * j + lane] : ~0ull;
         u64* vw = val + w * keep;
         unsigned* tw = tok + w * keep;
-        if (a.finished && a.finished[row]) {
+        if (fin) {
             for (int i = lane; i < keep; i += 64) {
                 vw[i] = i == 0 && score > -INFINITY ? double_flip(score) : ~0ull;
                 tw[i] = (unsigned)a.padToken;
@@ -680,30 +731,30 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSc
             continue;
         }
         // log of the sum of the row's exponentials
-        float M = -INFINITY;
-        for (int p = lane; p < s.parts; p += 64) M = fmaxf(M, s.maxs[row * s.parts + p]);
+        float M = pm;
+        for (int p = lane + 64; p < s.parts; p += 64) M = fmaxf(M, s.maxs[row * s.parts + p]);
 #pragma unroll
         for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
         double S = 0.0;
         for (int p = lane; p < s.parts; p += 64) {
-            const float pm = s.maxs[row * s.parts + p];
-            const double ps = s.sums[row * s.parts + p];
+            if (p >= 64) {
+                pm = s.maxs[row * s.parts + p];
+                ps = s.sums[row * s.parts + p];
+            }
             if (pm > -INFINITY || ps != ps) S += ps * exp((double)pm - (double)M);
         }
 #pragma unroll
         for (int o = 32; o; o >>= 1) S += __shfl_xor(S, o, 64);
         const double lse = (double)M + log(S);
-        // the row's best: keys below the keep-th best of the lanes' best, cut in LDS; in rounds where they do not fit
-        const u64* keys = s.keys + row * s.parts * keep;
-        const int total = s.parts * keep;
+        // the row's best, cut in LDS four times 64 keys at a time
         u64* list = lists[wave];
         int n = 0;
         u64 thr = ~0ull;
-        for (int i0 = 0; i0 < total; i0 += 128) {
+        for (int i0 = 0; i0 < count; i0 += 256) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const int i = i0 + 64 * j + lane;
-                const u64 k = i < total ? keys[i] : ~0ull;
+                const u64 k = i0 == 0 ? first[j] : i < count ? keys[i] : ~0ull;
                 const bool in = k < thr;
                 const u64 mask = __ballot(in);
                 if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = k;
@@ -728,31 +779,33 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSc
         }
     }
     __syncthreads();
-    // rank of each candidate among those of the batch item: by value, then beam, then token
-    const int total = a.beams * keep;
-    int valid = 0;
-    for (int i0 = 0; i0 < total; i0 += kBeamJoin) {
-        const int i = i0 + threadIdx.x;
-        const bool is = i < total && val[min(i, total - 1)] != ~0ull;
-        valid += __syncthreads_count(is);
-        if (!is) continue;
+    // rank of each candidate among those of the batch item: by value, then beam, then token.  A thread compares one candidate
+    // with the candidates of every `share`-th beam
+    const int share = max(1, min(kBeamJoin / total, a.beams));
+    for (int x = threadIdx.x; x < total * share; x += kBeamJoin) {
+        const int i = x / share, g = x - i * share, w = i / keep;
         const u64 v = val[i];
+        if (v == ~0ull) continue;
         const unsigned t = tok[i];
-        const int w = i / keep;
         int rank = 0;
-        for (int j = 0; j < total; ++j) {
-            const u64 o = val[j];
-            const int ow = j / keep;
-            rank += o < v || (o == v && (ow < w || (ow == w && tok[j] < t)));
-            if (rank >= keep) break;
-        }
-        if (rank < keep) {
-            const int64_t at = (int64_t)b * keep + rank;
-            const u64 u = ~v;
-            a.outScores[at] = (float)__builtin_bit_cast(double, (u >> 63) ? (u & ~(1ull << 63)) : ~u);
-            a.parents[at] = w;
-            a.tokens[at] = (int)t;
-        }
+        for (int ow = g; ow < a.beams; ow += share)
+            for (int j = ow * keep; j < (ow + 1) * keep; ++j) {
+                const u64 o = val[j];
+                rank += o < v || (o == v && (ow < w || (ow == w && tok[j] < t)));
+            }
+        if (rank) atomicAdd(&ranks[i], rank);
+        if (g == 0) atomicAdd(&valid, 1);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < total; i += kBeamJoin) {
+        const u64 v = val[i];
+        const int rank = ranks[i];
+        if (v == ~0ull || rank >= keep) continue;
+        const int64_t at = (int64_t)b * keep + rank;
+        const u64 u = ~v;
+        a.outScores[at] = (float)__builtin_bit_cast(double, (u >> 63) ? (u & ~(1ull << 63)) : ~u);
+        a.parents[at] = i / keep;
+        a.tokens[at] = (int)tok[i];
     }
     for (int i = valid + threadIdx.x; i < keep; i += kBeamJoin) { // fewer candidates than asked for
         const int64_t at = (int64_t)b * keep + i;
