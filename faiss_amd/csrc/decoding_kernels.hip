@@ -15,6 +15,11 @@ __device__ __forceinline__ int lane64() {
     return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
 }
 
+// how many bits of the mask stand before this lane's
+__device__ __forceinline__ int lanes_before(unsigned long long mask) {
+    return (int)__builtin_amdgcn_mbcnt_hi((unsigned)(mask >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)mask, 0u));
+}
+
 // ================================================================================================ block tables and slot maps
 // Requests are served in order.  Request b needs take_b = blocks(new) - blocks(old) more blocks (or returns that many); it is
 // granted if the blocks and the slots that the requests up to b ask for together are there.  Both sums only grow with b, so
@@ -635,6 +640,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s)
             lim = t == ~0u ? -INFINITY : float_unflip(~t);
         }
         if (!__ballot(mx >= lim && mx > -INFINITY)) continue;
+        const unsigned first = (unsigned)((st * LD * 64 + lane) * PER); // index of v[0]
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             if (n > kBeamPend) n = wave_cut(list, n, wave_kth(list, n, keep));
@@ -644,13 +650,13 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s)
                 const bool in = v[i] >= lim && v[i] > -INFINITY;
                 const u64 mask = __ballot(in);
                 if (!mask) continue;
-                if (in) list[n + __popcll(mask & ((1ull << lane) - 1))] = beam_key(v[i], (unsigned)(((st * LD + i / PER) * 64 + lane) * PER + i % PER));
+                if (in) list[n + lanes_before(mask)] = beam_key(v[i], first + (unsigned)(64 * PER * (i / PER) + i % PER));
                 n += __popcll(mask);
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
         }
         // a bound for the steps to come; renewed when there is something to gain from it
-        if (n > keep && (!full || n > kBeamPend / 2)) {
+        if (n > keep && (!full || n > keep + max(keep / 2, 8))) {
             const u64 kth = wave_kth(list, n, keep);
             n = wave_cut(list, n, kth);
             thr = beam_logit(kth);
