@@ -28,7 +28,8 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kTile = 64;        // tokens per step of a wavefront
-constexpr float kBias = 14.f;    // see above
+constexpr int kSeg = 64;         // tiles whose blocks and scales are held in LDS
+constexpr float kBias = 6.f, kSlack = 8.f; // see above; both in units of log 2
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // what a launch works on, beside AttendArgs
@@ -40,6 +41,7 @@ struct Sched {
     int wshift;       // work is counted in units of 2^wshift tiles so that its sum fits an int
     int maxSlots;     // partial results that the workspace holds
     int merge;        // 0: no request is split
+    int mergeRows;    // workgroups that join a row tile's rows
     float* partO;     // [maxSlots][rows][dim]
     float2* partML;   // [maxSlots][rows]
 };
@@ -199,13 +201,13 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
     return false;
 }
 
-__device__ __forceinline__ float load_elem(const void* p, int64_t i, int type) {
-    if (type == DT_F16) return (float)((const _Float16*)p)[i];
-    return __builtin_bit_cast(float, (unsigned)((const unsigned short*)p)[i] << 16);
-}
-__device__ __forceinline__ unsigned short to_elem(float x, int type) {
-    if (type == DT_F16) return __builtin_bit_cast(unsigned short, (_Float16)x);
-    return __builtin_bit_cast(unsigned short, (__bf16)x);
+// four adjacent elements of a result (any alignment)
+__device__ __forceinline__ void store4(unsigned short* p, f32x4 x, float f, int type) {
+    unsigned short r[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        r[e] = type == DT_F16 ? __builtin_bit_cast(unsigned short, (_Float16)(x[e] * f)) : __builtin_bit_cast(unsigned short, (__bf16)(x[e] * f));
+    __builtin_memcpy(p, r, 8);
 }
 
 // One work item.  SPLIT: the four wavefronts share the rows and take every fourth tile of the chunk, their results are joined in
@@ -224,6 +226,72 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
     const int rowsAll = it.nq * G;
     const int row0 = it.rt * ROWS + (SPLIT ? 0 : wave * 16 * NT);
 
+    // ---- the tiles of this wavefront
+    const int lastRow = min(rowsAll, row0 + 16 * NT) - 1;
+    int vis = 0, visMin = 0; // tokens that the last / the first row sees
+    if (lastRow >= row0) {
+        vis = a.causal ? max(0, it.len - it.nq + lastRow / G + 1) : it.len;
+        visMin = a.causal ? max(0, it.len - it.nq + row0 / G + 1) : it.len;
+    }
+    const int step = SPLIT ? kWaves : 1;
+    const int tile0 = it.c * it.tiles;
+    int tile = tile0 + (SPLIT ? wave : 0);
+    const int end = min(tile0 + it.tiles, (vis + kTile - 1) / kTile);
+    // what the workgroup's last row sees
+    const int lastAll = min(rowsAll, it.rt * ROWS + ROWS) - 1;
+    const int visAll = a.causal ? max(0, it.len - it.nq + lastAll / G + 1) : it.len;
+    const int endAll = min(tile0 + it.tiles, (visAll + kTile - 1) / kTile);
+    // blocks and scales of a stretch of the context, looked up once: a wait for a block's number in the loop would be a wait for
+    // all loads issued before it
+    __shared__ int pageL[4 * kSeg];
+    __shared__ float scaleL[2][4 * kSeg];
+    const int* tb = a.table + (int64_t)it.b * a.tableStride;
+
+    // block of the 16 tokens 16 u ...: -1 where there is none, -2 where there should be one
+    auto block_of = [&](int u) -> int {
+        if (u >= (it.len + 15) >> 4) return -1;
+        const int col = (u << 4) >> bsShift;
+        if (col >= a.cols) return -2;
+        const int p = tb[col];
+        return (unsigned)p < (unsigned)a.cache.numBlocks ? p : -2;
+    };
+    auto look_up = [&](int seg0) {
+        for (int i = threadIdx.x; i < 4 * min(kSeg, endAll - seg0); i += 256) {
+            const int p = block_of(4 * seg0 + i);
+            float ks = p == -2 ? __builtin_nanf("") : 0.f, vs = ks;
+            if (p >= 0) {
+                ks = a.cache.ks[(int64_t)p * H + it.h];
+                vs = a.cache.vs[(int64_t)p * H + it.h];
+            }
+            pageL[i] = max(p, 0);
+            scaleL[0][i] = ks;
+            scaleL[1][i] = vs;
+        }
+    };
+    // the codes of a tile, on their way or there
+    u32x4 kr[4][NL ? NL : 1];
+    u32x2 kx[4];
+    u32x4 vr[MD];
+    auto fetch_k = [&](int t, int page) {
+        const int off = ((t * kTile + 16 * (n16 >> 2)) & (bs - 1)) + (n16 & 3);
+        const uint8_t* p = a.cache.k + ((int64_t)page * H + it.h) * (int64_t)(bs * D) + (int64_t)off * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int j = 0; j < NL; ++j) kr[i][j] = *(const u32x4*)(p + i * 4 * D + 64 * j + 16 * grp);
+            if constexpr (D % 64) kx[i] = *(const u32x2*)(p + i * 4 * D + 64 * NL + 8 * grp);
+        }
+    };
+    auto fetch_v = [&](int t, int page) { // 16 tokens of a dimension per lane
+        const uint8_t* p = a.cache.v + ((int64_t)page * H + it.h) * (int64_t)(bs * D) + (int64_t)n16 * bs + ((t * kTile + 16 * grp) & (bs - 1));
+#pragma unroll
+        for (int i = 0; i < MD; ++i) vr[i] = *(const u32x4*)(p + (int64_t)i * 16 * bs);
+    };
+    // the first keys are on their way before the queries are looked at
+    look_up(tile0);
+    __syncthreads();
+    if (tile < min(tile0 + kSeg, end)) fetch_k(tile, pageL[(tile - tile0) * 4 + (n16 >> 2)]);
+
     // ---- queries: lane (n16, grp) holds of row n16 the dimensions 64 j + 16 grp + 8 p ... + 7 for step 2 j + p, the bytes that
     // its lane loads of a key.  qs: what a score is multiplied by beside the block's scale, in units of log 2
     half8_t q[NT][KS];
@@ -241,9 +309,13 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             const int d = (D % 64 && k == KS - 1) ? 64 * NL + 8 * grp : 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
+            u32x4 raw; // (any alignment)
+            __builtin_memcpy(&raw, (const unsigned short*)a.q + at + d, 16);
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float v = in ? load_elem(a.q, at + d + e, a.type) : 0.f;
+                const unsigned u = e & 1 ? raw[e >> 1] >> 16 : raw[e >> 1] & 0xffffu;
+                float v = a.type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)u) : __builtin_bit_cast(float, u << 16);
+                v = in ? v : 0.f;
                 x[k][e] = v;
                 const float m = fabsf(v);
                 big = (m > big && m < INFINITY) ? m : big;
@@ -275,60 +347,11 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
     }
     float vref = 0.f, vinv = 0.f; // values are accumulated in units of vref, the largest scale met so far
 
-    // ---- the tiles of this wavefront
-    const int lastRow = min(rowsAll, row0 + 16 * NT) - 1;
-    int vis = 0, visMin = 0; // tokens that the last / the first row sees
-    if (lastRow >= row0) {
-        vis = a.causal ? max(0, it.len - it.nq + lastRow / G + 1) : it.len;
-        visMin = a.causal ? max(0, it.len - it.nq + row0 / G + 1) : it.len;
-    }
-    const int step = SPLIT ? kWaves : 1;
-    int tile = it.c * it.tiles + (SPLIT ? wave : 0);
-    const int end = min(it.c * it.tiles + it.tiles, (vis + kTile - 1) / kTile);
-    const int* tb = a.table + (int64_t)it.b * a.tableStride;
-
-    // block of the 16 tokens 16 u ...: -1 where there is none, -2 where there should be one
-    auto block_of = [&](int u) -> int {
-        if (u >= (it.len + 15) >> 4) return -1;
-        const int col = (u << 4) >> bsShift;
-        if (col >= a.cols) return -2;
-        const int p = tb[col];
-        return (unsigned)p < (unsigned)a.cache.numBlocks ? p : -2;
-    };
-    u32x4 kr[4][NL ? NL : 1];
-    u32x2 kx[4];
-    auto load_k = [&](int t, int page) {
-        const int u = (t << 2) + (n16 >> 2);
-        const int off = ((u << 4) & (bs - 1)) + (n16 & 3);
-        const uint8_t* p = a.cache.k + ((int64_t)(max(page, 0)) * H + it.h) * (int64_t)(bs * D) + (int64_t)off * D;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-            for (int j = 0; j < NL; ++j) kr[i][j] = *(const u32x4*)(p + i * 4 * D + 64 * j + 16 * grp);
-            if constexpr (D % 64) kx[i] = *(const u32x2*)(p + i * 4 * D + 64 * NL + 8 * grp);
-        }
-    };
-    if (tile < end) {
-        int pk = block_of((tile << 2) + (n16 >> 2)), pv = block_of((tile << 2) + grp);
-        load_k(tile, pk);
-        for (; tile < end; tile += step) {
+    auto work = [&](int seg0, int segEnd) {
             const int t0 = tile * kTile;
-            const int64_t sc = (int64_t)max(pv, 0) * H + it.h;
-            float ks = a.cache.ks[sc], vs = a.cache.vs[sc];
-            if (pv < 0) {
-                ks = pv == -1 ? 0.f : __builtin_nanf("");
-                vs = ks;
-            }
-            // values of this tile: 16 tokens of a dimension per lane
-            const uint8_t* vp = a.cache.v + sc * (int64_t)(bs * D) + (int64_t)n16 * bs + ((t0 + 16 * grp) & (bs - 1));
-            u32x4 vr[MD];
-#pragma unroll
-            for (int i = 0; i < MD; ++i) vr[i] = *(const u32x4*)(vp + (int64_t)i * 16 * bs);
             const int next = tile + step;
-            if (next < end) {
-                pk = block_of((next << 2) + (n16 >> 2));
-                pv = block_of((next << 2) + grp);
-            }
+            fetch_v(tile, pageL[(tile - seg0) * 4 + grp]);
+            const float ks = scaleL[0][(tile - seg0) * 4 + grp], vs = scaleL[1][(tile - seg0) * 4 + grp];
             // scores
             f32x4 sc4[NT][4];
 #pragma unroll
@@ -347,7 +370,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
                     for (int t = 0; t < NT; ++t) sc4[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[t][k], sc4[t][i], 0, 0, 0);
                 }
             }
-            if (next < end) load_k(next, pk);
+            if (next < segEnd) fetch_k(next, pageL[(next - seg0) * 4 + (n16 >> 2)]);
 
             // the values' unit
             // (a scale that is no number or has no normal inverse does not become the unit: it must not touch rows that mask it)
@@ -376,7 +399,8 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
                         mx = fmaxf(mx, x);
                     }
                 mx = groups_max(mx);
-                const float mn = fmaxf(m[t], mx);
+                // the reference of the exponentials follows the maximum only when that has grown by more than 2^8
+                const float mn = mx > m[t] + kSlack ? mx : m[t];
                 const float top = mn == -INFINITY ? 0.f : mn;
                 const float sub = top - kBias;
                 const float down = __builtin_amdgcn_exp2f(m[t] - top);
@@ -420,7 +444,17 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
                     o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pr[t][1], o[t][i], 0, 0, 0);
                 }
             }
+            tile = next;
+    };
+    for (int seg0 = tile0; seg0 < endAll; seg0 += kSeg) {
+        const int segEnd = min(seg0 + kSeg, end);
+        if (seg0 != tile0) {
+            __syncthreads(); // (the segment before has been read)
+            look_up(seg0);
+            __syncthreads();
+            if (tile < segEnd) fetch_k(tile, pageL[(tile - seg0) * 4 + (n16 >> 2)]);
         }
+        while (tile < segEnd) work(seg0, segEnd);
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t) l[t] = groups_sum(l[t]);
@@ -470,8 +504,7 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
                 const int qi = (row0 + r) / G, g = (row0 + r) - qi * G;
                 const float inv = L == 0.f ? 0.f : 1.f / L;
                 unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) op[e] = to_elem(O[e] * inv, a.type);
+                store4(op, O, inv, a.type);
                 if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = L == 0.f ? -INFINITY : (M - kBias + __builtin_amdgcn_logf(L)) * kLn2;
             }
         }
@@ -495,64 +528,89 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
                 const float inv = l[t] == 0.f ? 0.f : vref / l[t];
                 unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + 4 * grp;
 #pragma unroll
-                for (int i = 0; i < MD; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) op[16 * i + e] = to_elem(o[t][i][e] * inv, a.type);
+                for (int i = 0; i < MD; ++i) store4(op + 16 * i, o[t][i], inv, a.type);
                 if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = l[t] == 0.f ? -INFINITY : (m[t] - kBias + __builtin_amdgcn_logf(l[t])) * kLn2;
             }
         }
     }
 }
 
-// Joins the chunks of a split request: one workgroup per row.
+// Joins the chunks of a split request: a workgroup takes every mergeRows-th row.  The chunks' weights come first (all loads in flight together), then
+// every group of dim / 4 threads adds up its share of the chunks, eight loads at a time.
+constexpr int kMergeChunks = 1024; // weights held at once
 __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, Sched s) {
     Item it;
-    if (!find_item<true>(a, s, blockIdx.x / s.rows, 0, it)) return;
-    const int r = blockIdx.x % s.rows, D = a.cache.headDim, G = a.heads / a.cache.numHeads;
+    if (!find_item<true>(a, s, blockIdx.x / s.mergeRows, 0, it)) return;
+    const int D = a.cache.headDim, G = a.heads / a.cache.numHeads;
+    for (int r = blockIdx.x % s.mergeRows; r < s.rows; r += s.mergeRows) {
     const int row = it.rt * s.rows + r;
     if (row >= it.nq * G) return;
+    __syncthreads();
     const float2* ml = s.partML + (int64_t)it.slot * s.rows + r;
     const float* po = s.partO + ((int64_t)it.slot * s.rows + r) * D;
-    const int quads = D / 4, parts = 256 / quads; // parts: the chunks are dealt to this many groups of threads
+    const int quads = D / 4, parts = 256 / quads;
     const int part = threadIdx.x / quads, d = 4 * (threadIdx.x - part * quads);
     __shared__ __align__(16) float so[256 * 4];
-    __shared__ float sM[256], sL[256];
-    float M = -INFINITY, L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    if (part < parts) {
-        for (int c = part; c < it.n; c += parts) M = fmaxf(M, ml[(int64_t)c * s.rows].x);
-        for (int c = part; c < it.n; c += parts) {
-            const float2 x = ml[(int64_t)c * s.rows];
-            if (x.x == -INFINITY && x.y == 0.f) continue; // saw nothing, wrote nothing worth reading
-            const float f = __builtin_amdgcn_exp2f(x.x - M);
-            L = __builtin_fmaf(f, x.y, L);
-            const f32x4 v = *(const f32x4*)(po + (int64_t)c * s.rows * D + d);
+    __shared__ float wt[kMergeChunks];
+    __shared__ float red[2][4];
+    float M = -INFINITY;
+    for (int c = threadIdx.x; c < it.n; c += 256) M = fmaxf(M, ml[(int64_t)c * s.rows].x);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(f, v[e], O[e]);
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+    if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+    for (int c0 = 0; c0 < it.n; c0 += kMergeChunks) {
+        const int n = min(it.n - c0, kMergeChunks);
+        __syncthreads();
+        for (int c = threadIdx.x; c < n; c += 256) {
+            const float2 x = ml[(int64_t)(c0 + c) * s.rows];
+            // a chunk that saw nothing has weight zero and no sums; one of which every score was NaN has a NaN sum
+            const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : x.y) : __builtin_amdgcn_exp2f(x.x - M);
+            wt[c] = f;
+            L += f == 0.f ? 0.f : f * x.y;
+        }
+        __syncthreads();
+        if (part < parts) {
+            const float* p = po + (int64_t)c0 * s.rows * D + d;
+            int c = part;
+            for (; c + 7 * parts < n; c += 8 * parts) {
+                f32x4 v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = *(const f32x4*)(p + (int64_t)(c + e * parts) * s.rows * D);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float f = wt[c + e * parts];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) O[j] = f == 0.f ? O[j] : __builtin_fmaf(f, v[e][j], O[j]);
+                }
+            }
+            for (; c < n; c += parts) {
+                const f32x4 v = *(const f32x4*)(p + (int64_t)c * s.rows * D);
+                const float f = wt[c];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) O[j] = f == 0.f ? O[j] : __builtin_fmaf(f, v[j], O[j]);
+            }
         }
     }
-    sM[threadIdx.x] = M;
-    sL[threadIdx.x] = L;
+#pragma unroll
+    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, 64);
+    if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
     *(f32x4*)&so[4 * threadIdx.x] = O;
     __syncthreads();
-    if (threadIdx.x >= quads) return;
-    for (int p = 1; p < parts; ++p) M = fmaxf(M, sM[p * quads + threadIdx.x]);
-    L = 0.f;
-    O = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int p = 0; p < parts; ++p) {
-        const int x = p * quads + threadIdx.x;
-        if (sM[x] == -INFINITY && sL[x] == 0.f) continue;
-        const float f = __builtin_amdgcn_exp2f(sM[x] - M);
-        L = __builtin_fmaf(f, sL[x], L);
+    if (threadIdx.x >= quads) continue;
+    L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    for (int p = 1; p < parts; ++p)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(f, so[4 * x + e], O[e]);
-    }
+        for (int e = 0; e < 4; ++e) O[e] += so[4 * (p * quads + threadIdx.x) + e];
     const int qi = row / G, g = row - qi * G;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) op[e] = to_elem(O[e] * inv, a.type);
+    store4(op, O, inv, a.type);
     if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = L == 0.f ? -INFINITY : (M - kBias + __builtin_amdgcn_logf(L)) * kLn2;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host side
@@ -578,7 +636,7 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         s.rowLo = lo;
         s.rowHi = (int)std::min<int64_t>(hi, INT32_MAX);
         s.minTiles = split ? 4 : 8;
-        s.target = num_cus * (split ? 4 : 2);
+        s.target = num_cus * (split ? (a.cache.headDim <= 64 ? 6 : a.cache.headDim <= 128 ? 4 : 2) : 2);
         const int64_t rowTiles = ((int64_t)a.tokens * G + s.rows - 1) / s.rows + a.batch;
         const int64_t tiles = ((int64_t)a.cols * a.cache.blockSize + kTile) / kTile;
         s.wshift = 0;
@@ -588,7 +646,9 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         const int64_t items = s.merge ? 2 * (int64_t)s.target + 2 * (int64_t)a.cache.numHeads : 0;
         s.maxSlots = (int)std::min<int64_t>(items, INT32_MAX);
         L.grid = rowTiles * a.cache.numHeads + items + 8; // (items are dealt to the XCDs in eight ranges of the same length)
-        L.mergeGrid = s.merge ? std::min<int64_t>(rowTiles * a.cache.numHeads, s.maxSlots / 2) * s.rows : 0;
+        const int64_t groups = std::min<int64_t>(rowTiles * a.cache.numHeads, s.maxSlots / 2);
+        s.mergeRows = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s.rows, most), 8192 / std::max<int64_t>(groups, 1)));
+        L.mergeGrid = s.merge ? groups * s.mergeRows : 0;
         L.bytes = s.merge ? round_up((size_t)s.maxSlots * s.rows * a.cache.headDim * 4, 256) + round_up((size_t)s.maxSlots * s.rows * 8, 256) : 0;
         s.partO = nullptr;
         s.partML = nullptr;
