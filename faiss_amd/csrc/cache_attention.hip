@@ -28,6 +28,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kWaves = 4;
 constexpr int kTile = 64;        // tokens per step of a wavefront
+constexpr float kNoScale = -1000.f;
 constexpr int kSeg = 64;         // tiles whose blocks and scales are held in LDS
 constexpr float kBias = 6.f, kSlack = 8.f; // see above; both in units of log 2
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -38,9 +39,11 @@ struct Sched {
     int rows;         // rows of a work item
     int minTiles;     // fewest 64-token tiles of a chunk
     int target;       // chunks are as long as needed to have about this many work items
+    int slack;        // a request is split only if it is this many times as long as a chunk
     int wshift;       // work is counted in units of 2^wshift tiles so that its sum fits an int
     int maxSlots;     // partial results that the workspace holds
     int merge;        // 0: no request is split
+    int sort;         // of 64 requests, the longest first
     int mergeRows;    // workgroups that join a row tile's rows
     float* partO;     // [maxSlots][rows][dim]
     float2* partML;   // [maxSlots][rows]
@@ -104,11 +107,15 @@ __device__ __forceinline__ void request(const AttendArgs& a, int b, int& len, in
     }
 }
 
+__device__ __forceinline__ int chunks(int lt, int tiles, int slack) {
+    return lt > (long long)tiles * slack ? (lt + tiles - 1) / tiles : 1;
+}
+
 // Deals the work out: chunks of the same number of tiles for every request, so that long and short contexts of a ragged batch
 // cost a workgroup the same.  Every wavefront recomputes this from the lengths (a prefix sum over the batch, one step per 64
 // requests); a table made by a launch of its own would cost more than it saves.  id: work item (MERGE: row group) number.
 template <bool MERGE>
-__device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, int id, int xcd_blocks, Item& it) {
+__device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, int id, Item& it) {
     const int lane = threadIdx.x & 63;
     const int G = a.heads / a.cache.numHeads;
     int sum = 0;
@@ -129,32 +136,21 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
     const long long total = (((long long)sum * a.cache.numHeads) << s.wshift);
     int tiles = (int)min((long long)(1 << 28), (total + s.target - 1) / s.target);
     tiles = max(tiles, s.minTiles);
-    // neighbouring items (the row tiles and chunks of one request and head) on one XCD: it.c / it.rt fastest, items dealt in
-    // eight contiguous ranges because consecutive workgroups go to the eight XCDs in turn
-    int items = 0;
-    if (!MERGE && xcd_blocks) {
-        for (int b0 = 0; b0 < a.batch; b0 += 64) {
-            const int b = b0 + lane;
-            int w = 0;
-            if (b < a.batch) {
-                int len, q0, nq;
-                request(a, b, len, q0, nq);
-                const long long rows = (long long)nq * G;
-                if (rows >= s.rowLo && rows <= s.rowHi) {
-                    const int lt = (int)(((long long)len + kTile - 1) / kTile);
-                    w = (int)((rows + s.rows - 1) / s.rows) * max(1, (lt + tiles - 1) / tiles) * a.cache.numHeads;
-                }
-            }
-            items += __builtin_amdgcn_readlane((int)wave_incl_scan((unsigned)w), 63);
-        }
-        const int per = (items + 7) >> 3;
-        if ((id >> 3) >= per) return false;
-        id = (id & 7) * per + (id >> 3);
-        if (id >= items) return false;
-    }
+    // Consecutive workgroups go to the eight XCDs in turn, so every XCD gets its share of every request; the heads of a row tile
+    // follow one another, the row tiles that see most come first, and of 64 requests the longest.
     int base = 0, sbase = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
-        const int b = b0 + lane;
+        int b = b0 + lane;
+        if (s.sort && b0 + 1 < a.batch) {
+            const int key = b < a.batch ? a.lengths[b] : -1; // (any order would do)
+            int rank = 0;
+            for (int j = 0; j < min(64, a.batch - b0); ++j) {
+                const int o = __builtin_amdgcn_readlane(key, j);
+                rank += o > key || (o == key && j < lane);
+            }
+            if (b < a.batch) b = b0 + rank;
+            b = __builtin_amdgcn_ds_permute(4 * (b - b0), lane) + b0;
+        }
         int w = 0, sl = 0, len = 0, q0 = 0, nq = 0, n = 1, rts = 0;
         if (b < a.batch) {
             request(a, b, len, q0, nq);
@@ -162,7 +158,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
             if (rows >= s.rowLo && rows <= s.rowHi) {
                 rts = (int)((rows + s.rows - 1) / s.rows);
                 const int lt = (int)(((long long)len + kTile - 1) / kTile);
-                n = max(1, (lt + tiles - 1) / tiles);
+                n = chunks(lt, tiles, s.slack);
                 w = rts * n * a.cache.numHeads;
                 sl = n > 1 ? w : 0;
                 if (MERGE) w = n > 1 ? rts * a.cache.numHeads : 0;
@@ -173,25 +169,19 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
         if (hit) {
             const int src = __ffsll((long long)hit) - 1;
             const int k = id - __builtin_amdgcn_readlane(incl - w, src);
-            it.b = b0 + src;
+            it.b = __builtin_amdgcn_readlane(b, src);
             it.n = __builtin_amdgcn_readlane(n, src);
             it.len = __builtin_amdgcn_readlane(len, src);
             it.q0 = __builtin_amdgcn_readlane(q0, src);
             it.nq = __builtin_amdgcn_readlane(nq, src);
             rts = __builtin_amdgcn_readlane(rts, src);
             const int s0 = __builtin_amdgcn_readlane(sincl - sl, src);
-            it.tiles = tiles;
-            if (MERGE) {
-                it.c = 0;
-                it.rt = k % rts;
-                it.h = k / rts;
-                it.slot = s0 + k * it.n;
-            } else {
-                it.c = k % it.n;
-                it.rt = (k / it.n) % rts;
-                it.h = k / (it.n * rts);
-                it.slot = it.n > 1 ? s0 + (k / it.n) * it.n : -1;
-            }
+            it.tiles = (int)((((long long)it.len + kTile - 1) / kTile + it.n - 1) / it.n); // chunks of the same length
+            const int H = a.cache.numHeads, m = MERGE ? 1 : it.n;
+            it.c = k % m;
+            it.h = (k / m) % H;
+            it.rt = rts - 1 - k / (m * H);
+            it.slot = it.n > 1 ? s0 + (k / m) * it.n : -1;
             if (it.slot >= 0 && it.slot + it.n > s.maxSlots) return false; // offsets that overlap: nothing to work in
             return true;
         }
@@ -210,66 +200,235 @@ __device__ __forceinline__ void store4(unsigned short* p, f32x4 x, float f, int 
     __builtin_memcpy(p, r, 8);
 }
 
-// One work item.  SPLIT: the four wavefronts share the rows and take every fourth tile of the chunk, their results are joined in
-// LDS.  Otherwise each has 16 x NT rows of its own and all read the same tiles (through the CU's L1).
-template <int D, int CODE, int NT, bool SPLIT>
-__global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s) {
+// ---- parts of the two kernels.  A wavefront has NT tiles of 16 rows; lane (n16, grp) = (lane % 16, lane / 16) holds of the scores of
+// row n16 of each tile the tokens 16 grp ... + 15 of a step's 64, and of its sums 4 dimensions of every 16.
+template <int NT, int MD>
+struct Rows {
+    float qs[NT];    // what a score is multiplied by beside the block's scale, in units of log 2; not negative
+    int limit[NT];   // tokens the row sees
+    float m[NT], l[NT];
+    float vref;      // values are accumulated in units of 2^vref, the largest scale met so far
+    f32x4 o[NT][MD];
+    __device__ __forceinline__ void reset() {
+        vref = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MD; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+};
+
+// NT tiles of rows from row0 on as fp16 operands.  KEYBYTES: step k's dimensions are the ones of the bytes that a lane of the direct
+// kernel loads of a key, 64 (k / 2) + 16 grp + 8 (k % 2) ...; else 32 k + 8 grp ...
+template <int D, int NT, bool KEYBYTES, int MD>
+__device__ __forceinline__ void load_queries(const AttendArgs& a, const Item& it, int G, int row0, int rowsAll, half8_t (&q)[NT][D / 32], Rows<NT, MD>& w) {
+    const int lane = threadIdx.x & 63, n16 = lane & 15, grp = lane >> 4;
+    constexpr int KS = D / 32;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + n16;
+        const bool in = r < rowsAll;
+        const int qi = in ? r / G : 0, g = in ? r - qi * G : 0;
+        w.limit[t] = !in ? 0 : a.causal ? max(0, it.len - it.nq + qi + 1) : it.len;
+        const int64_t at = (int64_t)(it.q0 + qi) * a.qTokenStride + (int64_t)(it.h * G + g) * a.qHeadStride;
+        float x[KS][8];
+        float big = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            const int d = !KEYBYTES || (D % 64 && k == KS - 1) ? 32 * k + 8 * grp : 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
+            u32x4 raw; // (any alignment)
+            __builtin_memcpy(&raw, (const unsigned short*)a.q + at + d, 16);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const unsigned u = e & 1 ? raw[e >> 1] >> 16 : raw[e >> 1] & 0xffffu;
+                float v = a.type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)u) : __builtin_bit_cast(float, u << 16);
+                v = in ? v : 0.f;
+                x[k][e] = v;
+                const float m = fabsf(v);
+                big = (m > big && m < INFINITY) ? m : big;
+            }
+        }
+        float up = 1.f;
+        w.qs[t] = fabsf(a.scale) * kLog2e;
+        if (a.type == DT_BF16) {
+            big = groups_max(big);
+            // largest element to [2^9, 2^10); both factors stay finite: the exponent of a bf16 number is -133 ... 127
+            const int e = big > 0.f ? min(max(10 - (int)__builtin_amdgcn_frexp_expf(big), -120), 120) : 0;
+            up = __builtin_ldexpf(1.f, e);
+            w.qs[t] *= __builtin_ldexpf(1.f, -e);
+        }
+        if (a.scale < 0.f) up = -up;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) q[t][k][e] = (_Float16)(x[k][e] * up);
+    }
+}
+
+// The scores of 64 tokens become probabilities, fp16 operands of the second product; maxima, sums and accumulators follow.
+// tok0: the lane group's first token; edge: some row does not see all 64; ks, lvs: the key scale and log2 of the value scale of the
+// lane group's block.  A value's scale goes into its probability's exponent, so the sum of the probabilities themselves is the
+// lane's sum times the inverse.  All row tiles are worked on between the same branches: they are independent chains.
+template <int NT, int MD>
+__device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float lvs, int tok0, bool edge, Rows<NT, MD>& w, half8_t (&pr)[NT][2]) {
+    float f[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) f[t] = ks * w.qs[t];
+    if (edge) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[t][i][e] = (tok0 + 4 * i + e) < w.limit[t] ? sc[t][i][e] * f[t] : -INFINITY;
+            f[t] = 1.f;
+        }
+    }
+    const float vnew = fmaxf(w.vref, groups_max(lvs));
+    const float vdown = __builtin_amdgcn_exp2f(w.vref - (vnew == -INFINITY ? 0.f : vnew));
+    w.vref = vnew;
+    const float lv = lvs == kNoScale ? 0.f : lvs - vnew, iv = __builtin_amdgcn_exp2f(-lv);
+    float od[NT];
+    bool change = false;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float mx = fmaxf(sc[t][0][0], sc[t][0][1]);
+#pragma unroll
+        for (int i = 2; i < 16; ++i) mx = fmaxf(mx, sc[t][i >> 2][i & 3]);
+        mx = groups_max(mx * f[t]);
+        mx = __builtin_fmaf(fabsf(mx), 0x1p-22f, mx); // not below the exact products of the fma below, however large they are
+        // the reference of the exponentials follows the maximum only when that has grown by more than 2^8
+        const float mn = mx > w.m[t] + kSlack ? mx : w.m[t];
+        const float top = mn == -INFINITY ? 0.f : mn;
+        const float down = __builtin_amdgcn_exp2f(w.m[t] - top);
+        w.m[t] = mn;
+        const float sub = lv - (top - kBias);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i][e], f[t], sub));
+                sum += p;
+                pr[t][i >> 1][4 * (i & 1) + e] = (_Float16)p;
+            }
+        w.l[t] = __builtin_fmaf(sum, iv, w.l[t] * down);
+        od[t] = down * vdown;
+        change |= od[t] != 1.f;
+    }
+    if (__ballot(change)) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < MD; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[t][i][e] *= od[t];
+    }
+}
+
+// blocks and scales of a stretch of the context, looked up once: a wait for a block's number in the loop would be a wait for all
+// loads issued before it
+struct Stretch {
+    int page[4 * kSeg];
+    float ks[4 * kSeg], lvs[4 * kSeg]; // key scale, log2 of the value scale (kNoScale: the values count as zero)
+};
+__device__ __forceinline__ void look_up(const AttendArgs& a, const Item& it, int seg0, int endAll, int threads, Stretch& z) {
+    const int bs = a.cache.blockSize, shift = 31 - __builtin_clz(bs);
+    const int* tb = a.table + (int64_t)it.b * a.tableStride;
+    for (int i = threadIdx.x; i < 4 * min(kSeg, endAll - seg0); i += threads) {
+        const int u = 4 * seg0 + i; // 16 tokens
+        int p = -1;
+        float ks = 0.f, vs = 0.f;
+        if (u < (it.len + 15) >> 4) { // there should be a block
+            const int col = (u << 4) >> shift;
+            p = col < a.cols ? tb[col] : -1;
+            if ((unsigned)p < (unsigned)a.cache.numBlocks) {
+                ks = a.cache.ks[(int64_t)p * a.cache.numHeads + it.h];
+                vs = a.cache.vs[(int64_t)p * a.cache.numHeads + it.h];
+                // a scale that is negative or no number, of the values also an infinite one, makes the scores NaN: the rows that
+                // see the block become NaN, those that mask it do not
+                if (!(ks >= 0.f) || !(vs >= 0.f && vs < INFINITY)) ks = __builtin_nanf("");
+            } else {
+                p = -1;
+                ks = __builtin_nanf("");
+            }
+        }
+        z.page[i] = max(p, 0);
+        z.ks[i] = ks;
+        z.lvs[i] = vs >= FLT_MIN && vs < INFINITY ? __builtin_amdgcn_logf(vs) : kNoScale;
+    }
+}
+
+// tokens that a row sees
+__device__ __forceinline__ int visible(const AttendArgs& a, const Item& it, int G, int row) {
+    return a.causal ? max(0, it.len - it.nq + row / G + 1) : it.len;
+}
+// the bytes of 16 tokens that lie before the request's end: behind it there may be anything, NaN codes too
+__device__ __forceinline__ u32x4 cut_tokens(u32x4 w, int valid) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int nb = min(max(valid - 4 * i, 0), 4);
+        w[i] &= nb == 4 ? ~0u : (1u << (8 * nb)) - 1u;
+    }
+    return w;
+}
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l == 0.f ? -INFINITY : (m - kBias + __builtin_amdgcn_logf(l)) * kLn2;
+}
+// a row of a wavefront's own: the result, or a chunk's partial sums
+template <int D, int NT, int MD>
+__device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, const Item& it, int G, int row0, int rowsAll, Rows<NT, MD>& w) {
+    const int lane = threadIdx.x & 63, n16 = lane & 15, grp = lane >> 4;
+    const float unit = __builtin_amdgcn_exp2f(w.vref);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int r = row0 + 16 * t + n16;
+        if (r >= rowsAll) continue;
+        if (it.slot >= 0) {
+            const int64_t pr = (int64_t)(it.slot + it.c) * s.rows + (r - it.rt * s.rows);
+#pragma unroll
+            for (int i = 0; i < MD; ++i) {
+                f32x4 x = w.o[t][i];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] *= unit;
+                *(f32x4*)(s.partO + pr * D + 16 * i + 4 * grp) = x;
+            }
+            if (grp == 0) s.partML[pr] = make_float2(w.m[t], w.l[t]);
+        } else {
+            const int qi = r / G, g = r - qi * G;
+            const float inv = w.l[t] == 0.f ? 0.f : unit / w.l[t];
+            unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + 4 * grp;
+#pragma unroll
+            for (int i = 0; i < MD; ++i) store4(op + 16 * i, w.o[t][i], inv, a.type);
+            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.m[t], w.l[t]);
+        }
+    }
+}
+
+// Few rows (single tokens, drafts): bound by the bytes of the cache.  The four wavefronts of a workgroup share the rows and take every
+// fourth tile of the chunk, straight from memory into the registers that feed the matrix instructions; their results are joined in
+// LDS.
+template <int D, int CODE, int NT>
+__global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16; // steps of the first product, row tiles of the second
     constexpr int NL = D / 64;              // 16-byte pieces of a key per lane (and one of 8 bytes if D % 64)
-    constexpr int ROWS = SPLIT ? 16 * NT : 16 * NT * kWaves;
+    constexpr int ROWS = 16 * NT;
     Item it;
-    if (!find_item<false>(a, s, blockIdx.x, 1, it)) return;
+    if (!find_item<false>(a, s, blockIdx.x, it)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n16 = lane & 15, grp = lane >> 4;
     const int H = a.cache.numHeads, G = a.heads / H, bs = a.cache.blockSize;
-    const int bsShift = 31 - __builtin_clz(bs);
-    const int rowsAll = it.nq * G;
-    const int row0 = it.rt * ROWS + (SPLIT ? 0 : wave * 16 * NT);
+    const int rowsAll = it.nq * G, row0 = it.rt * ROWS;
+    const int vis = visible(a, it, G, min(rowsAll, row0 + ROWS) - 1), visMin = visible(a, it, G, row0); // what the last / the first row sees
+    const int tile0 = it.c * it.tiles, end = min(tile0 + it.tiles, (vis + kTile - 1) / kTile);
+    int tile = tile0 + wave;
+    __shared__ Stretch z;
 
-    // ---- the tiles of this wavefront
-    const int lastRow = min(rowsAll, row0 + 16 * NT) - 1;
-    int vis = 0, visMin = 0; // tokens that the last / the first row sees
-    if (lastRow >= row0) {
-        vis = a.causal ? max(0, it.len - it.nq + lastRow / G + 1) : it.len;
-        visMin = a.causal ? max(0, it.len - it.nq + row0 / G + 1) : it.len;
-    }
-    const int step = SPLIT ? kWaves : 1;
-    const int tile0 = it.c * it.tiles;
-    int tile = tile0 + (SPLIT ? wave : 0);
-    const int end = min(tile0 + it.tiles, (vis + kTile - 1) / kTile);
-    // what the workgroup's last row sees
-    const int lastAll = min(rowsAll, it.rt * ROWS + ROWS) - 1;
-    const int visAll = a.causal ? max(0, it.len - it.nq + lastAll / G + 1) : it.len;
-    const int endAll = min(tile0 + it.tiles, (visAll + kTile - 1) / kTile);
-    // blocks and scales of a stretch of the context, looked up once: a wait for a block's number in the loop would be a wait for
-    // all loads issued before it
-    __shared__ int pageL[4 * kSeg];
-    __shared__ float scaleL[2][4 * kSeg];
-    const int* tb = a.table + (int64_t)it.b * a.tableStride;
-
-    // block of the 16 tokens 16 u ...: -1 where there is none, -2 where there should be one
-    auto block_of = [&](int u) -> int {
-        if (u >= (it.len + 15) >> 4) return -1;
-        const int col = (u << 4) >> bsShift;
-        if (col >= a.cols) return -2;
-        const int p = tb[col];
-        return (unsigned)p < (unsigned)a.cache.numBlocks ? p : -2;
-    };
-    auto look_up = [&](int seg0) {
-        for (int i = threadIdx.x; i < 4 * min(kSeg, endAll - seg0); i += 256) {
-            const int p = block_of(4 * seg0 + i);
-            float ks = p == -2 ? __builtin_nanf("") : 0.f, vs = ks;
-            if (p >= 0) {
-                ks = a.cache.ks[(int64_t)p * H + it.h];
-                vs = a.cache.vs[(int64_t)p * H + it.h];
-            }
-            pageL[i] = max(p, 0);
-            scaleL[0][i] = ks;
-            scaleL[1][i] = vs;
-        }
-    };
     // the codes of a tile, on their way or there
-    u32x4 kr[4][NL ? NL : 1];
+    u32x4 kr[4][NL];
     u32x2 kx[4];
     u32x4 vr[MD];
     auto fetch_k = [&](int t, int page) {
@@ -288,251 +447,247 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
         for (int i = 0; i < MD; ++i) vr[i] = *(const u32x4*)(p + (int64_t)i * 16 * bs);
     };
     // the first keys are on their way before the queries are looked at
-    look_up(tile0);
+    look_up(a, it, tile0, end, 256, z);
     __syncthreads();
-    if (tile < min(tile0 + kSeg, end)) fetch_k(tile, pageL[(tile - tile0) * 4 + (n16 >> 2)]);
-
-    // ---- queries: lane (n16, grp) holds of row n16 the dimensions 64 j + 16 grp + 8 p ... + 7 for step 2 j + p, the bytes that
-    // its lane loads of a key.  qs: what a score is multiplied by beside the block's scale, in units of log 2
+    if (tile < min(tile0 + kSeg, end)) fetch_k(tile, z.page[(tile - tile0) * 4 + (n16 >> 2)]);
     half8_t q[NT][KS];
-    float qs[NT];
-    int limit[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int r = row0 + 16 * t + n16;
-        const bool in = r < rowsAll;
-        const int qi = in ? r / G : 0, g = in ? r - qi * G : 0;
-        limit[t] = !in ? 0 : a.causal ? max(0, it.len - it.nq + qi + 1) : it.len;
-        const int64_t at = (int64_t)(it.q0 + qi) * a.qTokenStride + (int64_t)(it.h * G + g) * a.qHeadStride;
-        float x[KS][8];
-        float big = 0.f;
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-            const int d = (D % 64 && k == KS - 1) ? 64 * NL + 8 * grp : 64 * (k >> 1) + 16 * grp + 8 * (k & 1);
-            u32x4 raw; // (any alignment)
-            __builtin_memcpy(&raw, (const unsigned short*)a.q + at + d, 16);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const unsigned u = e & 1 ? raw[e >> 1] >> 16 : raw[e >> 1] & 0xffffu;
-                float v = a.type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)u) : __builtin_bit_cast(float, u << 16);
-                v = in ? v : 0.f;
-                x[k][e] = v;
-                const float m = fabsf(v);
-                big = (m > big && m < INFINITY) ? m : big;
-            }
-        }
-        float up = 1.f;
-        qs[t] = a.scale * kLog2e;
-        if (a.type == DT_BF16) {
-            big = groups_max(big);
-            // largest element to [2^10, 2^11); both factors stay finite: the exponent of a bf16 number is -133 ... 127
-            const int e = big > 0.f ? min(max(10 - (int)__builtin_amdgcn_frexp_expf(big), -120), 120) : 0;
-            up = __builtin_ldexpf(1.f, e);
-            qs[t] *= __builtin_ldexpf(1.f, -e);
-        }
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) q[t][k][e] = (_Float16)(x[k][e] * up);
-    }
+    Rows<NT, MD> w;
+    load_queries<D, NT, true>(a, it, G, row0, rowsAll, q, w);
+    w.reset();
 
-    f32x4 o[NT][MD];
-    float m[NT], l[NT];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        m[t] = -INFINITY;
-        l[t] = 0.f;
-#pragma unroll
-        for (int i = 0; i < MD; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
-    float vref = 0.f, vinv = 0.f; // values are accumulated in units of vref, the largest scale met so far
-
-    auto work = [&](int seg0, int segEnd) {
-            const int t0 = tile * kTile;
-            const int next = tile + step;
-            fetch_v(tile, pageL[(tile - seg0) * 4 + grp]);
-            const float ks = scaleL[0][(tile - seg0) * 4 + grp], vs = scaleL[1][(tile - seg0) * 4 + grp];
-            // scores
-            f32x4 sc4[NT][4];
+    for (int seg0 = tile0; seg0 < end; seg0 += kSeg) {
+        const int segEnd = min(seg0 + kSeg, end);
+        if (seg0 != tile0) {
+            __syncthreads(); // (the stretch before has been read)
+            look_up(a, it, seg0, end, 256, z);
+            __syncthreads();
+            if (tile < segEnd) fetch_k(tile, z.page[(tile - seg0) * 4 + (n16 >> 2)]);
+        }
+        for (; tile < segEnd; tile += kWaves) {
+            const int t0 = tile * kTile, u = (tile - seg0) * 4;
+            fetch_v(tile, z.page[u + grp]);
+            const float ks = z.ks[u + grp], lvs = z.lvs[u + grp];
+            f32x4 sc[NT][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) sc4[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int t = 0; t < NT; ++t) sc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    u32x2 w;
+                    u32x2 c;
                     if ((D % 64) && k == KS - 1)
-                        w = kx[i];
+                        c = kx[i];
                     else
-                        w = (k & 1) ? u32x2{kr[i][k >> 1][2], kr[i][k >> 1][3]} : u32x2{kr[i][k >> 1][0], kr[i][k >> 1][1]};
-                    const half8_t ka = widen<CODE>(w);
+                        c = (k & 1) ? u32x2{kr[i][k >> 1][2], kr[i][k >> 1][3]} : u32x2{kr[i][k >> 1][0], kr[i][k >> 1][1]};
+                    const half8_t ka = widen<CODE>(c);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) sc4[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[t][k], sc4[t][i], 0, 0, 0);
+                    for (int t = 0; t < NT; ++t) sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[t][k], sc[t][i], 0, 0, 0);
                 }
             }
-            if (next < segEnd) fetch_k(next, pageL[(next - seg0) * 4 + (n16 >> 2)]);
-
-            // the values' unit
-            // (a scale that is no number or has no normal inverse does not become the unit: it must not touch rows that mask it)
-            const float va = fabsf(vs);
-            const float vmax = groups_max(va >= FLT_MIN && va <= FLT_MAX ? va : 0.f);
-            float vdown = 1.f;
-            if (vmax > vref) {
-                vdown = vref / vmax;
-                vref = vmax;
-                vinv = 1.f / vmax;
-            }
-            const float vunit = vs * vinv;
-            const bool edge = t0 + kTile > visMin;
+            if (tile + kWaves < segEnd) fetch_k(tile + kWaves, z.page[u + 4 * kWaves + (n16 >> 2)]);
             half8_t pr[NT][2];
+            softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, w, pr);
+            if (t0 + kTile > it.len || __ballot(lvs == kNoScale)) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const float f = ks * qs[t];
-                float mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = sc4[t][i][e] * f;
-                        if (edge) x = (t0 + 16 * grp + 4 * i + e) < limit[t] ? x : -INFINITY;
-                        sc4[t][i][e] = x;
-                        mx = fmaxf(mx, x);
-                    }
-                mx = groups_max(mx);
-                // the reference of the exponentials follows the maximum only when that has grown by more than 2^8
-                const float mn = mx > m[t] + kSlack ? mx : m[t];
-                const float top = mn == -INFINITY ? 0.f : mn;
-                const float sub = top - kBias;
-                const float down = __builtin_amdgcn_exp2f(m[t] - top);
-                m[t] = mn;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float p = __builtin_amdgcn_exp2f(sc4[t][i][e] - sub);
-                        sum += p;
-                        float pv1 = p * vunit;
-                        if (edge) pv1 = p == 0.f ? 0.f : pv1;
-                        pr[t][i >> 1][4 * (i & 1) + e] = (_Float16)pv1;
-                    }
-                l[t] = l[t] * down + sum;
-                const float od = down * vdown;
-                if (__ballot(od != 1.f)) {
-#pragma unroll
-                    for (int i = 0; i < MD; ++i)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) o[t][i][e] *= od;
-                }
-            }
-            if (t0 + kTile > it.len) { // what lies behind the last token may be anything, NaN codes too
-                const int valid = min(max(it.len - (t0 + 16 * grp), 0), 16);
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int nb = min(max(valid - 4 * w, 0), 4);
-                    const unsigned mask = nb == 4 ? ~0u : (1u << (8 * nb)) - 1u;
-#pragma unroll
-                    for (int i = 0; i < MD; ++i) vr[i][w] &= mask;
-                }
+                for (int i = 0; i < MD; ++i) vr[i] = cut_tokens(vr[i], lvs == kNoScale ? 0 : it.len - (t0 + 16 * grp));
             }
 #pragma unroll
             for (int i = 0; i < MD; ++i) {
                 const half8_t a0 = widen<CODE>(u32x2{vr[i][0], vr[i][1]}), a1 = widen<CODE>(u32x2{vr[i][2], vr[i][3]});
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pr[t][0], o[t][i], 0, 0, 0);
-                    o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pr[t][1], o[t][i], 0, 0, 0);
+                    w.o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a0, pr[t][0], w.o[t][i], 0, 0, 0);
+                    w.o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a1, pr[t][1], w.o[t][i], 0, 0, 0);
                 }
             }
-            tile = next;
-    };
-    for (int seg0 = tile0; seg0 < endAll; seg0 += kSeg) {
-        const int segEnd = min(seg0 + kSeg, end);
-        if (seg0 != tile0) {
-            __syncthreads(); // (the segment before has been read)
-            look_up(seg0);
-            __syncthreads();
-            if (tile < segEnd) fetch_k(tile, pageL[(tile - seg0) * 4 + (n16 >> 2)]);
         }
-        while (tile < segEnd) work(seg0, segEnd);
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t) l[t] = groups_sum(l[t]);
+    for (int t = 0; t < NT; ++t) w.l[t] = groups_sum(w.l[t]);
 
-    if constexpr (SPLIT) {
-        constexpr int PITCH = D + 4;
-        __shared__ __align__(16) float sm[kWaves][16 * NT][PITCH];
-        __shared__ float sml[kWaves][16 * NT][2];
+    constexpr int PITCH = D + 4;
+    __shared__ __align__(16) float sm[kWaves][16 * NT][PITCH];
+    __shared__ float sml[kWaves][16 * NT][2];
+    const float unit = __builtin_amdgcn_exp2f(w.vref);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (grp == 0) {
-                sml[wave][16 * t + n16][0] = m[t];
-                sml[wave][16 * t + n16][1] = l[t];
-            }
-#pragma unroll
-            for (int i = 0; i < MD; ++i) {
-                f32x4 x = o[t][i];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] *= vref;
-                *(f32x4*)&sm[wave][16 * t + n16][16 * i + 4 * grp] = x;
-            }
+    for (int t = 0; t < NT; ++t) {
+        if (grp == 0) {
+            sml[wave][16 * t + n16][0] = w.m[t];
+            sml[wave][16 * t + n16][1] = w.l[t];
         }
-        __syncthreads();
-        // a thread joins 4 dimensions of a row
-        for (int x = threadIdx.x; x < 16 * NT * (D / 4); x += 256) {
-            const int r = x / (D / 4), d = 4 * (x - r * (D / 4));
-            if (row0 + r >= rowsAll) break;
-            float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) M = fmaxf(M, sml[w][r][0]);
-            float L = 0.f;
-            f32x4 O = {0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < MD; ++i) {
+            f32x4 x = w.o[t][i];
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                const float mw = sml[w][r][0];
-                const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-                L += f * sml[w][r][1];
-                const f32x4 ow = *(const f32x4*)&sm[w][r][d];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(f, ow[e], O[e]);
-            }
-            if (it.slot >= 0) {
-                const int64_t pr = (int64_t)(it.slot + it.c) * ROWS + r;
-                *(f32x4*)(s.partO + pr * D + d) = O;
-                if (d == 0) s.partML[pr] = make_float2(M, L);
-            } else {
-                const int qi = (row0 + r) / G, g = (row0 + r) - qi * G;
-                const float inv = L == 0.f ? 0.f : 1.f / L;
-                unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
-                store4(op, O, inv, a.type);
-                if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = L == 0.f ? -INFINITY : (M - kBias + __builtin_amdgcn_logf(L)) * kLn2;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int r = row0 + 16 * t + n16;
-            if (r >= rowsAll) continue;
-            if (it.slot >= 0) {
-                const int64_t pr = (int64_t)(it.slot + it.c) * ROWS + (r - it.rt * ROWS);
-#pragma unroll
-                for (int i = 0; i < MD; ++i) {
-                    f32x4 x = o[t][i];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e] *= vref;
-                    *(f32x4*)(s.partO + pr * D + 16 * i + 4 * grp) = x;
-                }
-                if (grp == 0) s.partML[pr] = make_float2(m[t], l[t]);
-            } else {
-                const int qi = r / G, g = r - qi * G;
-                const float inv = l[t] == 0.f ? 0.f : vref / l[t];
-                unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + 4 * grp;
-#pragma unroll
-                for (int i = 0; i < MD; ++i) store4(op + 16 * i, o[t][i], inv, a.type);
-                if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = l[t] == 0.f ? -INFINITY : (m[t] - kBias + __builtin_amdgcn_logf(l[t])) * kLn2;
-            }
+            for (int e = 0; e < 4; ++e) x[e] *= unit;
+            *(f32x4*)&sm[wave][16 * t + n16][16 * i + 4 * grp] = x;
         }
     }
+    __syncthreads();
+    // a thread joins 4 dimensions of a row
+    for (int x = threadIdx.x; x < 16 * NT * (D / 4); x += 256) {
+        const int r = x / (D / 4), d = 4 * (x - r * (D / 4));
+        if (row0 + r >= rowsAll) break;
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) M = fmaxf(M, sml[v][r][0]);
+        float L = 0.f;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) {
+            const float mw = sml[v][r][0];
+            const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
+            L += f * sml[v][r][1];
+            const f32x4 ow = *(const f32x4*)&sm[v][r][d];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(f, ow[e], O[e]);
+        }
+        if (it.slot >= 0) {
+            const int64_t pr = (int64_t)(it.slot + it.c) * ROWS + r;
+            *(f32x4*)(s.partO + pr * D + d) = O;
+            if (d == 0) s.partML[pr] = make_float2(M, L);
+        } else {
+            const int qi = (row0 + r) / G, g = (row0 + r) - qi * G;
+            unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
+            store4(op, O, L == 0.f ? 0.f : 1.f / L, a.type);
+            if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
+        }
+    }
+}
+
+// Many rows (prompts): bound by the arithmetic.  Each of the WAVES wavefronts has rows of its own; a tile's keys and values are loaded
+// and widened to fp16 once for all of them and laid into LDS fragment by fragment, in the order in which the matrix instructions'
+// lanes read them (no bank conflicts on either side).  Two such buffers: the next tile is loaded while one is worked on.
+template <int D, int CODE, int NT, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(AttendArgs a, Sched s) {
+    constexpr int KS = D / 32, MD = D / 16;
+    constexpr int ROWS = 16 * NT * WAVES;
+    constexpr int KP = 4 * ((D + 63) / 64);              // pieces of the keys: 16 tokens x 64 dimensions, a wavefront each
+    constexpr int KW = (KP + WAVES - 1) / WAVES, VW = (MD + WAVES - 1) / WAVES;
+    Item it;
+    if (!find_item<false>(a, s, blockIdx.x, it)) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n16 = lane & 15, grp = lane >> 4;
+    const int H = a.cache.numHeads, G = a.heads / H, bs = a.cache.blockSize;
+    const int rowsAll = it.nq * G, row0 = it.rt * ROWS + wave * 16 * NT;
+    const int lastRow = min(rowsAll, row0 + 16 * NT) - 1;
+    const int vis = lastRow >= row0 ? visible(a, it, G, lastRow) : 0, visMin = lastRow >= row0 ? visible(a, it, G, row0) : 0;
+    const int tile0 = it.c * it.tiles;
+    const int end = min(tile0 + it.tiles, (vis + kTile - 1) / kTile);
+    const int endAll = min(tile0 + it.tiles, (visible(a, it, G, min(rowsAll, it.rt * ROWS + ROWS) - 1) + kTile - 1) / kTile);
+    __shared__ Stretch z;
+    __shared__ __align__(16) half8_t kf[2][4 * KS][64]; // fragment (i, k): tokens 16 g + 4 i + e in row 4 g + e, dimensions 32 k ...
+    __shared__ __align__(16) half8_t vf[2][MD * 2][64]; // fragment (i, h): dimensions 16 i ..., tokens 16 grp + 8 h ...
+
+    u32x4 kr[KW], vr[VW];
+    // (every wavefront loads, also where there is nothing for it: a load under a condition waits for the loads before it)
+    auto fetch = [&](int t, int seg0) {
+        const int u = (t - seg0) * 4;
+        const int kp = z.page[u + (n16 >> 2)], vp = z.page[u + grp];
+        const uint8_t* k = a.cache.k + ((int64_t)kp * H + it.h) * (int64_t)(bs * D) + (((t * kTile + 16 * (n16 >> 2)) & (bs - 1)) + (n16 & 3)) * D;
+        const uint8_t* v = a.cache.v + ((int64_t)vp * H + it.h) * (int64_t)(bs * D) + n16 * bs + ((t * kTile + 16 * grp) & (bs - 1));
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            const int pc = min(wave + j * WAVES, KP - 1);
+            kr[j] = *(const u32x4*)(k + 4 * (pc & 3) * D + min(64 * (pc >> 2) + 16 * grp, D - 16));
+        }
+#pragma unroll
+        for (int j = 0; j < VW; ++j) vr[j] = *(const u32x4*)(v + 16 * min(wave + j * WAVES, MD - 1) * bs);
+    };
+    auto lay = [&](int t, int seg0, int buf) { // what fetch brought
+#pragma unroll
+        for (int j = 0; j < KW; ++j) {
+            const int pc = wave + j * WAVES, i = pc & 3, d = 64 * (pc >> 2) + 16 * grp;
+            if (pc < KP && d < D) {
+                kf[buf][i * KS + d / 32][((d >> 3) & 3) * 16 + n16] = widen<CODE>(u32x2{kr[j][0], kr[j][1]});
+                kf[buf][i * KS + d / 32][(((d >> 3) & 3) + 1) * 16 + n16] = widen<CODE>(u32x2{kr[j][2], kr[j][3]});
+            }
+        }
+        const bool none = z.lvs[(t - seg0) * 4 + grp] == kNoScale, tail = (t + 1) * kTile > it.len || __ballot(none);
+        const int valid = none ? 0 : it.len - (t * kTile + 16 * grp);
+#pragma unroll
+        for (int j = 0; j < VW; ++j) {
+            const int i = wave + j * WAVES;
+            if (i < MD) {
+                const u32x4 c = tail ? cut_tokens(vr[j], valid) : vr[j];
+                vf[buf][2 * i][lane] = widen<CODE>(u32x2{c[0], c[1]});
+                vf[buf][2 * i + 1][lane] = widen<CODE>(u32x2{c[2], c[3]});
+            }
+        }
+    };
+    half8_t q[NT][KS];
+    Rows<NT, MD> w;
+    load_queries<D, NT, false>(a, it, G, row0, rowsAll, q, w);
+    w.reset();
+    for (int seg0 = tile0; seg0 < endAll; seg0 += kSeg) {
+        const int segEnd = min(seg0 + kSeg, endAll);
+        __syncthreads(); // (the stretch before has been read)
+        look_up(a, it, seg0, endAll, 64 * WAVES, z);
+        __syncthreads();
+        fetch(seg0, seg0);
+        lay(seg0, seg0, seg0 & 1);
+        __syncthreads();
+        for (int tile = seg0; tile < segEnd; ++tile) {
+            const int buf = tile & 1, t0 = tile * kTile, u = (tile - seg0) * 4;
+            const bool more = tile + 1 < segEnd;
+            fetch(min(tile + 1, segEnd - 1), seg0);
+            if (tile < end) {
+                const float ks = z.ks[u + grp], lvs = z.lvs[u + grp];
+                f32x4 sc[NT][4];
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                // four fragments at a time, the next four on their way from LDS; the order is pinned, or the compiler waits for
+                // each one right before its use
+                half8_t fr[2][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fr[0][j] = kf[buf][j][lane];
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+                for (int g = 0; g < KS; ++g) {
+                    if (g + 1 < KS) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) fr[(g + 1) & 1][j] = kf[buf][4 * (g + 1) + j][lane];
+                        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = (4 * g + j) / KS, k = (4 * g + j) % KS;
+#pragma unroll
+                        for (int t = 0; t < NT; ++t) sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[g & 1][j], q[t][k], sc[t][i], 0, 0, 0);
+                    }
+                    __builtin_amdgcn_sched_group_barrier(0x8, 4 * NT, 0);
+                }
+                half8_t pr[NT][2];
+                softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, w, pr);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) fr[0][j] = vf[buf][j][lane];
+                __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+                for (int g = 0; g < MD / 2; ++g) {
+                    if (g + 1 < MD / 2) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) fr[(g + 1) & 1][j] = vf[buf][4 * (g + 1) + j][lane];
+                        __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+                    }
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+                                w.o[t][2 * g + j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[g & 1][2 * j + h], pr[t][h], w.o[t][2 * g + j], 0, 0, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x8, 4 * NT, 1);
+                }
+            }
+            if (more) lay(tile + 1, seg0, buf ^ 1);
+            __syncthreads();
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) w.l[t] = groups_sum(w.l[t]);
+    write_rows<D>(a, s, it, G, row0, rowsAll, w);
 }
 
 // Joins the chunks of a split request: a workgroup takes every mergeRows-th row.  The chunks' weights come first (all loads in flight together), then
@@ -540,16 +695,48 @@ __global__ __launch_bounds__(256) void cache_attend_kernel(AttendArgs a, Sched s
 constexpr int kMergeChunks = 1024; // weights held at once
 __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, Sched s) {
     Item it;
-    if (!find_item<true>(a, s, blockIdx.x / s.mergeRows, 0, it)) return;
+    if (!find_item<true>(a, s, blockIdx.x / s.mergeRows, it)) return;
     const int D = a.cache.headDim, G = a.heads / a.cache.numHeads;
+    const int quads = D / 4, parts = 256 / quads;
+    const int part = threadIdx.x / quads, d = 4 * (threadIdx.x - part * quads);
+    if (it.n <= 8) { // few chunks: every group of threads joins a row of its own
+        if (part >= parts) return;
+        for (int r = (blockIdx.x % s.mergeRows) * parts + part; r < s.rows; r += s.mergeRows * parts) {
+            const int row = it.rt * s.rows + r;
+            if (row >= it.nq * G) return;
+            const int64_t at = (int64_t)it.slot * s.rows + r;
+            float2 x[8];
+            f32x4 v[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const int64_t p = at + (int64_t)min(c, it.n - 1) * s.rows;
+                x[c] = s.partML[p];
+                v[c] = *(const f32x4*)(s.partO + p * D + d);
+            }
+            float M = -INFINITY, L = 0.f;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) M = c < it.n ? fmaxf(M, x[c].x) : M;
+            f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+                const float f = c >= it.n ? 0.f : x[c].x == -INFINITY ? (x[c].y == x[c].y ? 0.f : x[c].y) : __builtin_amdgcn_exp2f(x[c].x - M);
+                L += f == 0.f ? 0.f : f * x[c].y;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) O[j] = f == 0.f ? O[j] : __builtin_fmaf(f, v[c][j], O[j]);
+            }
+            const int qi = row / G, g = row - qi * G;
+            unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
+            store4(op, O, L == 0.f ? 0.f : 1.f / L, a.type);
+            if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
+        }
+        return;
+    }
     for (int r = blockIdx.x % s.mergeRows; r < s.rows; r += s.mergeRows) {
     const int row = it.rt * s.rows + r;
     if (row >= it.nq * G) return;
     __syncthreads();
     const float2* ml = s.partML + (int64_t)it.slot * s.rows + r;
     const float* po = s.partO + ((int64_t)it.slot * s.rows + r) * D;
-    const int quads = D / 4, parts = 256 / quads;
-    const int part = threadIdx.x / quads, d = 4 * (threadIdx.x - part * quads);
     __shared__ __align__(16) float so[256 * 4];
     __shared__ float wt[kMergeChunks];
     __shared__ float red[2][4];
@@ -609,7 +796,7 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
     const float inv = L == 0.f ? 0.f : 1.f / L;
     unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
     store4(op, O, inv, a.type);
-    if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = L == 0.f ? -INFINITY : (M - kBias + __builtin_amdgcn_logf(L)) * kLn2;
+    if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
     }
 }
 
@@ -617,27 +804,29 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
 // rows of a work item and the requests it serves
 struct Launch {
     Sched s;
-    int nt;
-    bool split;
+    int nt, waves;
     int64_t grid, mergeGrid;
     size_t bytes;
 };
 
 int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
-    const int G = a.heads / a.cache.numHeads;
+    const int G = a.heads / a.cache.numHeads, D = a.cache.headDim;
     const int64_t most = (int64_t)a.maxQueries * G;
     int n = 0;
-    auto add = [&](int nt, bool split, int lo, int64_t hi) {
+    auto add = [&](int nt, int waves, int lo, int64_t hi) { // waves 0: the direct kernel
         Launch& L = out[n++];
         L.nt = nt;
-        L.split = split;
+        L.waves = waves;
         Sched& s = L.s;
-        s.rows = 16 * nt * (split ? 1 : kWaves);
+        s.rows = 16 * nt * (waves ? waves : 1);
         s.rowLo = lo;
         s.rowHi = (int)std::min<int64_t>(hi, INT32_MAX);
-        s.minTiles = split ? 4 : 8;
-        s.target = num_cus * (split ? (a.cache.headDim <= 64 ? 6 : a.cache.headDim <= 128 ? 4 : 2) : 2);
-        const int64_t rowTiles = ((int64_t)a.tokens * G + s.rows - 1) / s.rows + a.batch;
+        s.minTiles = waves ? 8 : 4;
+        // twice as many chunks as there are workgroups at work at a time
+        s.target = num_cus * (waves ? 8 / waves : D <= 64 ? 6 : D <= 128 ? 4 : 2);
+        s.slack = waves ? 2 : 1;
+        s.sort = waves != 0;
+        const int64_t rowTiles = std::min(((int64_t)a.tokens * G + s.rows - 1) / s.rows + a.batch, (int64_t)a.batch * ((s.rowHi + (int64_t)s.rows - 1) / s.rows));
         const int64_t tiles = ((int64_t)a.cols * a.cache.blockSize + kTile) / kTile;
         s.wshift = 0;
         while (((rowTiles * tiles) >> s.wshift) + a.batch > (int64_t)1 << 30) ++s.wshift;
@@ -645,41 +834,41 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         // a request with n > 1 chunks has at most twice its share of the total in them
         const int64_t items = s.merge ? 2 * (int64_t)s.target + 2 * (int64_t)a.cache.numHeads : 0;
         s.maxSlots = (int)std::min<int64_t>(items, INT32_MAX);
-        L.grid = rowTiles * a.cache.numHeads + items + 8; // (items are dealt to the XCDs in eight ranges of the same length)
+        L.grid = rowTiles * a.cache.numHeads + items;
         const int64_t groups = std::min<int64_t>(rowTiles * a.cache.numHeads, s.maxSlots / 2);
-        s.mergeRows = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s.rows, most), 8192 / std::max<int64_t>(groups, 1)));
+        s.mergeRows = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s.rows, most), 2048 / std::max<int64_t>(groups, 1)));
         L.mergeGrid = s.merge ? groups * s.mergeRows : 0;
-        L.bytes = s.merge ? round_up((size_t)s.maxSlots * s.rows * a.cache.headDim * 4, 256) + round_up((size_t)s.maxSlots * s.rows * 8, 256) : 0;
+        L.bytes = s.merge ? round_up((size_t)s.maxSlots * s.rows * D * 4, 256) + round_up((size_t)s.maxSlots * s.rows * 8, 256) : 0;
         s.partO = nullptr;
         s.partML = nullptr;
     };
     // 256 dimensions and 32 rows do not fit the registers of a wavefront
-    const int wide = a.cache.headDim > 192 ? 1 : 2;
+    const int wide = D > 192 ? 1 : 2;
     // few rows (single tokens, drafts): the wavefronts of a workgroup split the tokens; many rows: they split the rows
     if (most <= 16) {
-        add(1, true, 1, INT64_MAX);
+        add(1, 0, 1, INT64_MAX);
     } else if (most <= 32) {
-        add(wide, true, 1, INT64_MAX);
+        add(wide, 0, 1, INT64_MAX);
     } else {
-        if (a.queryOffsets && G <= 32) add(G <= 16 ? 1 : wide, true, 1, G <= 16 ? 16 : 32);
-        add(wide, false, n ? out[0].s.rowHi + 1 : 1, INT64_MAX);
+        if (a.queryOffsets && G <= 32) add(G <= 16 ? 1 : wide, 0, 1, G <= 16 ? 16 : 32);
+        // 128 rows of a workgroup, two of them on a CU, or 256
+        add(wide, D > 128 || most > 128 ? 8 : 4, n ? out[0].s.rowHi + 1 : 1, INT64_MAX);
     }
     return n;
 }
 
 template <int D, int CODE>
 void launch_one(const AttendArgs& a, const Launch& L, hipStream_t stream) {
-    const dim3 grid((unsigned)L.grid), block(256);
-    // (one row tile without a split of the tokens: only where two do not fit)
-    if (L.split && L.nt == 1)
-        cache_attend_kernel<D, CODE, 1, true><<<grid, block, 0, stream>>>(a, L.s);
-    else if constexpr (D > 192)
-        cache_attend_kernel<D, CODE, 1, false><<<grid, block, 0, stream>>>(a, L.s);
-    else {
-        if (L.split)
-            cache_attend_kernel<D, CODE, 2, true><<<grid, block, 0, stream>>>(a, L.s);
-        else
-            cache_attend_kernel<D, CODE, 2, false><<<grid, block, 0, stream>>>(a, L.s);
+    const dim3 grid((unsigned)L.grid);
+    constexpr int WIDE = D > 192 ? 1 : 2;
+    if (L.waves == 8) {
+        cache_attend_rows_kernel<D, CODE, WIDE, 8><<<grid, 512, 0, stream>>>(a, L.s);
+    } else if (L.waves == 4) {
+        if constexpr (D <= 128) cache_attend_rows_kernel<D, CODE, WIDE, 4><<<grid, 256, 0, stream>>>(a, L.s);
+    } else if (L.nt == 1) {
+        cache_attend_direct_kernel<D, CODE, 1><<<grid, 256, 0, stream>>>(a, L.s);
+    } else {
+        if constexpr (D <= 192) cache_attend_direct_kernel<D, CODE, 2><<<grid, 256, 0, stream>>>(a, L.s);
     }
     HIP_CHECK(hipGetLastError());
 }
