@@ -183,12 +183,12 @@ def load_library():
         # faiss_amd/decoding.py
         "faiss_amd_plan_blocks": (i32, [vp, vp, vp]),
         "faiss_amd_PagedCache_add": (i32, [vp, vp, vp, vp]),
-        "faiss_amd_PagedCache_reconstruct": (i32, [vp, vp, i32, vp, i32, vp, vp, vp]),
+        "faiss_amd_PagedCache_reconstruct": (i32, [vp, vp, i32, vp, i32, vp, vp, i32, vp]),
         "faiss_amd_PagedCache_attend": (i32, [vp, vp, vp, vp]),
         "faiss_amd_PagedCache_attend_workspace": (i32, [vp, vp, vp, P(sz)]),
         "faiss_amd_beam_select": (i32, [vp, vp, vp]),
         "faiss_amd_beam_select_workspace": (i32, [vp, vp, P(sz)]),
-        "faiss_amd_reorder_beams": (i32, [vp, i32, vp, vp, i32, i32, i32, vp]),
+        "faiss_amd_reorder_beams": (i32, [vp, i32, vp, vp, i32, i32, i32, i32, vp]),
         "faiss_amd_fork_blocks": (i32, [vp, i32, vp, vp, vp]),
     }
     for name, (res, args) in protos.items():

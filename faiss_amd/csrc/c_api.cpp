@@ -1094,9 +1094,9 @@ int faiss_amd_PagedCache_add(FaissAmdGpuResources* res, const FaissAmdPagedCache
     FA_CATCH
 }
 int faiss_amd_PagedCache_reconstruct(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, int n, const int* blocks, int type,
-                                     void* keys, void* values, void* stream) {
+                                     void* keys, void* values, int pointersChecked, void* stream) {
     FA_TRY
-    cache_reconstruct(G(res), cache, n, blocks, type, keys, values, (hipStream_t)stream);
+    cache_reconstruct(G(res), cache, n, blocks, type, keys, values, pointersChecked, (hipStream_t)stream);
     FA_CATCH
 }
 int faiss_amd_PagedCache_attend(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdAttendParams* args, void* stream) {
@@ -1123,9 +1123,9 @@ int faiss_amd_beam_select_workspace(FaissAmdGpuResources* res, const FaissAmdBea
     FA_CATCH
 }
 int faiss_amd_reorder_beams(FaissAmdGpuResources* res, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams,
-                            int keep, void* stream) {
+                            int keep, int pointersChecked, void* stream) {
     FA_TRY
-    reorder_beams(G(res), n, states, parents, batch, beams, keep, (hipStream_t)stream);
+    reorder_beams(G(res), n, states, parents, batch, beams, keep, pointersChecked, (hipStream_t)stream);
     FA_CATCH
 }
 int faiss_amd_fork_blocks(FaissAmdGpuResources* res, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* args,

@@ -36,7 +36,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // what a launch works on, beside AttendArgs
 struct Sched {
     int rowLo, rowHi; // serve the requests with rowLo <= queries * group <= rowHi
-    int rows;         // rows of a work item
+    int rows, rowShift; // rows of a work item, 2^rowShift
     int minTiles;     // fewest 64-token tiles of a chunk
     int target;       // chunks are as long as needed to have about this many work items
     int slack;        // a request is split only if it is this many times as long as a chunk
@@ -107,8 +107,9 @@ __device__ __forceinline__ void request(const AttendArgs& a, int b, int& len, in
     }
 }
 
+__device__ __forceinline__ int tiles_of(int len) { return (int)(((unsigned)len + kTile - 1) / kTile); }
 __device__ __forceinline__ int chunks(int lt, int tiles, int slack) {
-    return lt > (long long)tiles * slack ? (lt + tiles - 1) / tiles : 1;
+    return (unsigned)lt > (unsigned)tiles * slack ? (lt + tiles - 1) / tiles : 1;
 }
 
 // Deals the work out: chunks of the same number of tiles for every request, so that long and short contexts of a ragged batch
@@ -118,6 +119,11 @@ template <bool MERGE>
 __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, int id, Item& it) {
     const int lane = threadIdx.x & 63;
     const int G = a.heads / a.cache.numHeads;
+    // (tokens x heads fits an int, and the host chose wshift for the sums)
+    auto row_tiles = [&](int nq) {
+        const int rows = nq * G;
+        return rows >= s.rowLo && rows <= s.rowHi ? (rows + s.rows - 1) >> s.rowShift : 0;
+    };
     int sum = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 64) {
         const int b = b0 + lane;
@@ -125,17 +131,14 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
         if (b < a.batch) {
             int len, q0, nq;
             request(a, b, len, q0, nq);
-            const long long rows = (long long)nq * G;
-            if (rows >= s.rowLo && rows <= s.rowHi) {
-                const long long work = ((rows + s.rows - 1) / s.rows) * (((long long)len + kTile - 1) / kTile);
-                w = (int)((work + (1ll << s.wshift) - 1) >> s.wshift);
-            }
+            const long long work = (long long)row_tiles(nq) * tiles_of(len);
+            w = (int)((work + (1ll << s.wshift) - 1) >> s.wshift);
         }
         sum += __builtin_amdgcn_readlane((int)wave_incl_scan((unsigned)w), 63);
     }
-    const long long total = (((long long)sum * a.cache.numHeads) << s.wshift);
-    int tiles = (int)min((long long)(1 << 28), (total + s.target - 1) / s.target);
-    tiles = max(tiles, s.minTiles);
+    // (a division of floats: the same in every wavefront, and what it is off by is within the slack of maxSlots)
+    const float share = ceilf((float)sum * (float)a.cache.numHeads * __builtin_ldexpf(1.f, s.wshift) / (float)s.target);
+    const int tiles = max((int)fminf(share, 0x1p28f), s.minTiles);
     // Consecutive workgroups go to the eight XCDs in turn, so every XCD gets its share of every request; the heads of a row tile
     // follow one another, the row tiles that see most come first, and of 64 requests the longest.
     int base = 0, sbase = 0;
@@ -154,15 +157,11 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
         int w = 0, sl = 0, len = 0, q0 = 0, nq = 0, n = 1, rts = 0;
         if (b < a.batch) {
             request(a, b, len, q0, nq);
-            const long long rows = (long long)nq * G;
-            if (rows >= s.rowLo && rows <= s.rowHi) {
-                rts = (int)((rows + s.rows - 1) / s.rows);
-                const int lt = (int)(((long long)len + kTile - 1) / kTile);
-                n = chunks(lt, tiles, s.slack);
-                w = rts * n * a.cache.numHeads;
-                sl = n > 1 ? w : 0;
-                if (MERGE) w = n > 1 ? rts * a.cache.numHeads : 0;
-            }
+            rts = row_tiles(nq);
+            n = chunks(tiles_of(len), tiles, s.slack);
+            w = rts * n * a.cache.numHeads;
+            sl = n > 1 ? w : 0;
+            if (MERGE) w = n > 1 ? rts * a.cache.numHeads : 0;
         }
         const int incl = base + (int)wave_incl_scan((unsigned)w), sincl = sbase + (int)wave_incl_scan((unsigned)sl);
         const unsigned long long hit = __ballot(id < incl);
@@ -176,7 +175,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
             it.nq = __builtin_amdgcn_readlane(nq, src);
             rts = __builtin_amdgcn_readlane(rts, src);
             const int s0 = __builtin_amdgcn_readlane(sincl - sl, src);
-            it.tiles = (int)((((long long)it.len + kTile - 1) / kTile + it.n - 1) / it.n); // chunks of the same length
+            it.tiles = it.n > 1 ? (tiles_of(it.len) + it.n - 1) / it.n : tiles_of(it.len); // chunks of the same length
             const int H = a.cache.numHeads, m = MERGE ? 1 : it.n;
             it.c = k % m;
             it.h = (k / m) % H;
@@ -819,15 +818,19 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         L.waves = waves;
         Sched& s = L.s;
         s.rows = 16 * nt * (waves ? waves : 1);
+        s.rowShift = 0;
+        while ((1 << s.rowShift) < s.rows) ++s.rowShift;
         s.rowLo = lo;
         s.rowHi = (int)std::min<int64_t>(hi, INT32_MAX);
-        s.minTiles = waves ? 8 : 4;
-        // twice as many chunks as there are workgroups at work at a time
-        s.target = num_cus * (waves ? 8 / waves : D <= 64 ? 6 : D <= 128 ? 4 : 2);
+        // Direct: twice as many chunks as there are workgroups at work at a time, one and a half times with one workgroup on a CU
+        // (131071 tokens, 256 dimensions: 256 / 384 / 512 / 768 chunks 57 / 48 / 56 / 57 us)
+        s.target = waves ? num_cus * 8 / waves : num_cus * (D <= 64 ? 12 : D <= 128 ? 8 : 3) / 2;
         s.slack = waves ? 2 : 1;
         s.sort = waves != 0;
         const int64_t rowTiles = std::min(((int64_t)a.tokens * G + s.rows - 1) / s.rows + a.batch, (int64_t)a.batch * ((s.rowHi + (int64_t)s.rows - 1) / s.rows));
         const int64_t tiles = ((int64_t)a.cols * a.cache.blockSize + kTile) / kTile;
+        // a split costs a launch to join it (4 us), a tile of a wavefront 1 us: contexts of up to 16 tiles are not split
+        s.minTiles = waves || tiles > 16 ? 8 : 16;
         s.wshift = 0;
         while (((rowTiles * tiles) >> s.wshift) + a.batch > (int64_t)1 << 30) ++s.wshift;
         s.merge = tiles > s.minTiles;
@@ -842,7 +845,7 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         s.partO = nullptr;
         s.partML = nullptr;
     };
-    // 256 dimensions and 32 rows do not fit the registers of a wavefront
+    // 256 dimensions and 32 rows do not fit the registers of a wavefront (nor 192, where two of them share a SIMD)
     const int wide = D > 192 ? 1 : 2;
     // few rows (single tokens, drafts): the wavefronts of a workgroup split the tokens; many rows: they split the rows
     if (most <= 16) {
@@ -852,7 +855,7 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
     } else {
         if (a.queryOffsets && G <= 32) add(G <= 16 ? 1 : wide, 0, 1, G <= 16 ? 16 : 32);
         // 128 rows of a workgroup, two of them on a CU, or 256
-        add(wide, D > 128 || most > 128 ? 8 : 4, n ? out[0].s.rowHi + 1 : 1, INT64_MAX);
+        add(D > 128 ? 1 : 2, D > 128 || most > 128 ? 8 : 4, n ? out[0].s.rowHi + 1 : 1, INT64_MAX);
     }
     return n;
 }
@@ -860,11 +863,10 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
 template <int D, int CODE>
 void launch_one(const AttendArgs& a, const Launch& L, hipStream_t stream) {
     const dim3 grid((unsigned)L.grid);
-    constexpr int WIDE = D > 192 ? 1 : 2;
     if (L.waves == 8) {
-        cache_attend_rows_kernel<D, CODE, WIDE, 8><<<grid, 512, 0, stream>>>(a, L.s);
+        cache_attend_rows_kernel<D, CODE, (D > 128 ? 1 : 2), 8><<<grid, 512, 0, stream>>>(a, L.s);
     } else if (L.waves == 4) {
-        if constexpr (D <= 128) cache_attend_rows_kernel<D, CODE, WIDE, 4><<<grid, 256, 0, stream>>>(a, L.s);
+        if constexpr (D <= 128) cache_attend_rows_kernel<D, CODE, 2, 4><<<grid, 256, 0, stream>>>(a, L.s);
     } else if (L.nt == 1) {
         cache_attend_direct_kernel<D, CODE, 1><<<grid, 256, 0, stream>>>(a, L.s);
     } else {

@@ -8,9 +8,10 @@
 namespace faiss_amd {
 namespace {
 
-// memory of the resources' device
-void on_device(const GpuResources& r, const void* p, const char* what) {
+// memory of the resources' device; checked: the caller has looked
+void on_device(const GpuResources& r, const void* p, const char* what, int checked) {
     if (!p) FA_THROW_MSG(std::string(what) + " must be provided (passed null)");
+    if (checked) return;
     hipPointerAttribute_t a;
     if (hipPointerGetAttributes(&a, p) != hipSuccess) {
         (void)hipGetLastError();
@@ -60,11 +61,11 @@ CacheView view(const FaissAmdPagedCache* c) {
     v.headDim = c->headDim;
     return v;
 }
-void check_memory(const GpuResources& r, const CacheView& v) {
-    on_device(r, v.k, "cache keys");
-    on_device(r, v.v, "cache values");
-    on_device(r, v.ks, "cache keyScales");
-    on_device(r, v.vs, "cache valueScales");
+void check_memory(const GpuResources& r, const CacheView& v, int checked) {
+    on_device(r, v.k, "cache keys", checked);
+    on_device(r, v.v, "cache values", checked);
+    on_device(r, v.ks, "cache keyScales", checked);
+    on_device(r, v.vs, "cache valueScales", checked);
     aligned(v.k, 16, "cache keys");
     aligned(v.v, 16, "cache values");
     aligned(v.ks, 4, "cache keyScales");
@@ -83,21 +84,22 @@ void plan_blocks(const GpuResources* r, const FaissAmdPlanBlocksParams* p, hipSt
                         "plan_blocks: number of blocks out of range");
     FA_THROW_IF_NOT_MSG((int64_t)p->numColumns * p->blockSize < ((int64_t)1 << 31), "plan_blocks: table too wide");
     FA_THROW_IF_NOT_MSG(p->tableStride >= p->numColumns && (!p->ownedTable || p->ownedStride >= p->numColumns), "plan_blocks: rows of the table overlap");
+    const int checked = p->pointersChecked;
     DeviceScope scope(r);
     if (p->batch > 0) {
-        if (p->numColumns > 0) on_device(*r, p->blockTable, "blockTable");
-        if (p->ownedTable) on_device(*r, p->ownedTable, "ownedTable");
-        on_device(*r, p->lengths, "lengths");
-        on_device(*r, p->newLengths, "newLengths");
-        on_device(*r, p->lengthsOut, "lengthsOut");
-        on_device(*r, p->granted, "granted");
+        if (p->numColumns > 0) on_device(*r, p->blockTable, "blockTable", checked);
+        if (p->ownedTable) on_device(*r, p->ownedTable, "ownedTable", checked);
+        on_device(*r, p->lengths, "lengths", checked);
+        on_device(*r, p->newLengths, "newLengths", checked);
+        on_device(*r, p->lengthsOut, "lengthsOut", checked);
+        on_device(*r, p->granted, "granted", checked);
     }
-    on_device(*r, p->freeRing, "freeRing");
-    on_device(*r, p->freeState, "freeState");
-    on_device(*r, p->freeStateOut, "freeStateOut");
-    on_device(*r, p->queryOffsets, "queryOffsets");
-    on_device(*r, p->workspace, "workspace");
-    if (p->maxTokens > 0) on_device(*r, p->slots, "slots");
+    on_device(*r, p->freeRing, "freeRing", checked);
+    on_device(*r, p->freeState, "freeState", checked);
+    on_device(*r, p->freeStateOut, "freeStateOut", checked);
+    on_device(*r, p->queryOffsets, "queryOffsets", checked);
+    on_device(*r, p->workspace, "workspace", checked);
+    if (p->maxTokens > 0) on_device(*r, p->slots, "slots", checked);
     PlanArgs a;
     a.table = p->blockTable;
     a.owned = p->ownedTable;
@@ -127,12 +129,13 @@ void cache_add(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAm
     FA_THROW_IF_NOT_MSG(p, "null arguments");
     FA_THROW_IF_NOT_MSG(half_type(p->type), "add: keys and values must be float16 or bfloat16");
     FA_THROW_IF_NOT_MSG(p->tokens >= 0, "add: negative number of tokens");
+    const int checked = p->pointersChecked;
     DeviceScope scope(r);
     if (p->tokens == 0) return;
-    check_memory(*r, a.cache);
-    on_device(*r, p->keys, "keys");
-    on_device(*r, p->values, "values");
-    on_device(*r, p->slots, "slots");
+    check_memory(*r, a.cache, checked);
+    on_device(*r, p->keys, "keys", checked);
+    on_device(*r, p->values, "values", checked);
+    on_device(*r, p->slots, "slots", checked);
     aligned(p->keys, 2, "keys");
     aligned(p->values, 2, "values");
     a.key = p->keys;
@@ -147,17 +150,17 @@ void cache_add(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAm
     launch_cache_add(a, stream);
 }
 
-void cache_reconstruct(const GpuResources* r, const FaissAmdPagedCache* c, int n, const int* blocks, int type, void* keys, void* values, hipStream_t stream) {
+void cache_reconstruct(const GpuResources* r, const FaissAmdPagedCache* c, int n, const int* blocks, int type, void* keys, void* values, int checked, hipStream_t stream) {
     ReconstructArgs a;
     a.cache = view(c);
     FA_THROW_IF_NOT_MSG(type == DT_F32 || half_type(type), "reconstruct: type must be float32, float16 or bfloat16");
     FA_THROW_IF_NOT_MSG(n >= 0, "reconstruct: negative number of blocks");
     DeviceScope scope(r);
     if (n == 0) return;
-    check_memory(*r, a.cache);
-    on_device(*r, blocks, "blocks");
-    on_device(*r, keys, "keys");
-    on_device(*r, values, "values");
+    check_memory(*r, a.cache, checked);
+    on_device(*r, blocks, "blocks", checked);
+    on_device(*r, keys, "keys", checked);
+    on_device(*r, values, "values", checked);
     aligned(keys, 16, "keys");
     aligned(values, 16, "values");
     a.blocks = blocks;
@@ -201,6 +204,7 @@ void cache_attend(const GpuResources* r, const FaissAmdPagedCache* c, const Fais
     a.scale = p->scale;
     a.workspace = p->workspace;
     a.workspaceBytes = p->workspaceBytes;
+    const int checked = p->pointersChecked;
     DeviceScope scope(r);
     const size_t need = cache_attend_workspace(a, r->num_cus);
     if (bytes) {
@@ -208,18 +212,18 @@ void cache_attend(const GpuResources* r, const FaissAmdPagedCache* c, const Fais
         return;
     }
     if (p->batch == 0 || p->tokens == 0) return;
-    check_memory(*r, a.cache);
-    on_device(*r, p->queries, "queries");
-    on_device(*r, p->out, "out");
+    check_memory(*r, a.cache, checked);
+    on_device(*r, p->queries, "queries", checked);
+    on_device(*r, p->out, "out", checked);
     aligned(p->queries, 2, "queries");
     aligned(p->out, 2, "out");
-    if (p->lse) on_device(*r, p->lse, "lse");
-    if (p->numColumns > 0) on_device(*r, p->blockTable, "blockTable");
-    on_device(*r, p->lengths, "lengths");
-    if (p->queryOffsets) on_device(*r, p->queryOffsets, "queryOffsets");
+    if (p->lse) on_device(*r, p->lse, "lse", checked);
+    if (p->numColumns > 0) on_device(*r, p->blockTable, "blockTable", checked);
+    on_device(*r, p->lengths, "lengths", checked);
+    if (p->queryOffsets) on_device(*r, p->queryOffsets, "queryOffsets", checked);
     if (need) {
         FA_THROW_IF_NOT_MSG(p->workspaceBytes >= need, "attend: workspace too small");
-        on_device(*r, p->workspace, "workspace");
+        on_device(*r, p->workspace, "workspace", checked);
         aligned(p->workspace, 256, "workspace");
     }
     launch_cache_attend(a, r->num_cus, stream);
@@ -249,6 +253,7 @@ void beam_select(const GpuResources* r, const FaissAmdBeamSelectParams* p, hipSt
     a.type = p->type;
     a.workspace = p->workspace;
     a.workspaceBytes = p->workspaceBytes;
+    const int checked = p->pointersChecked;
     DeviceScope scope(r);
     const size_t need = beam_select_workspace(a, r->num_cus);
     if (bytes) {
@@ -256,34 +261,34 @@ void beam_select(const GpuResources* r, const FaissAmdBeamSelectParams* p, hipSt
         return;
     }
     if (p->batch == 0) return;
-    on_device(*r, p->logits, "logits");
+    on_device(*r, p->logits, "logits", checked);
     aligned(p->logits, type_size(p->type), "logits");
-    on_device(*r, p->scores, "scores");
-    if (p->finished) on_device(*r, p->finished, "finished");
-    on_device(*r, p->outScores, "outScores");
-    on_device(*r, p->outParents, "outParents");
-    on_device(*r, p->outTokens, "outTokens");
+    on_device(*r, p->scores, "scores", checked);
+    if (p->finished) on_device(*r, p->finished, "finished", checked);
+    on_device(*r, p->outScores, "outScores", checked);
+    on_device(*r, p->outParents, "outParents", checked);
+    on_device(*r, p->outTokens, "outTokens", checked);
     FA_THROW_IF_NOT_MSG(p->workspaceBytes >= need, "beam_select: workspace too small");
-    on_device(*r, p->workspace, "workspace");
+    on_device(*r, p->workspace, "workspace", checked);
     aligned(p->workspace, 256, "workspace");
     launch_beam_select(a, r->num_cus, stream);
 }
 
-void reorder_beams(const GpuResources* r, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams, int keep, hipStream_t stream) {
+void reorder_beams(const GpuResources* r, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams, int keep, int checked, hipStream_t stream) {
     FA_THROW_IF_NOT_MSG(n >= 0 && batch >= 0 && beams >= 1 && keep >= 0, "reorder_beams: negative size");
     FA_THROW_IF_NOT_MSG((int64_t)batch * keep < ((int64_t)1 << 31) && (int64_t)batch * beams < ((int64_t)1 << 31), "reorder_beams: too many rows");
     DeviceScope scope(r);
     if (n == 0 || batch == 0 || keep == 0) return;
     FA_THROW_IF_NOT_MSG(states, "reorder_beams: null states");
-    on_device(*r, parents, "parents");
+    on_device(*r, parents, "parents", checked);
     std::vector<ReorderState> st((size_t)n);
     for (int i = 0; i < n; ++i) {
         const FaissAmdBeamState& s = states[i];
         FA_THROW_IF_NOT_MSG(s.rowBytes >= 0 && s.batchBytes >= 0 && s.beamBytes >= 0, "reorder_beams: negative stride");
         st[i] = {s.in, s.out, s.batchBytes, s.beamBytes, s.rowBytes};
         if (s.rowBytes == 0) continue;
-        on_device(*r, s.in, "a state's input");
-        on_device(*r, s.out, "a state's output");
+        on_device(*r, s.in, "a state's input", checked);
+        on_device(*r, s.out, "a state's output", checked);
         const uintptr_t i0 = (uintptr_t)s.in, i1 = i0 + (uintptr_t)((batch - 1) * s.batchBytes + (beams - 1) * s.beamBytes + s.rowBytes);
         const uintptr_t o0 = (uintptr_t)s.out, o1 = o0 + (uintptr_t)((int64_t)batch * keep * s.rowBytes);
         FA_THROW_IF_NOT_MSG(o1 <= i0 || i1 <= o0, "reorder_beams: a state's output overlaps its input");
@@ -304,19 +309,20 @@ void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches,
         FA_THROW_IF_NOT_MSG(v[i].blockSize == v[0].blockSize && v[i].numBlocks == v[0].numBlocks, "fork_blocks: caches of different blocks");
     }
     FA_THROW_IF_NOT_MSG((int64_t)p->numColumns * v[0].blockSize < ((int64_t)1 << 31), "fork_blocks: table too wide");
+    const int checked = p->pointersChecked;
     DeviceScope scope(r);
     if (p->batch == 0) return;
-    for (int i = 0; i < n; ++i) check_memory(*r, v[i]);
+    for (int i = 0; i < n; ++i) check_memory(*r, v[i], checked);
     if (p->numColumns > 0) {
-        on_device(*r, p->blockTable, "blockTable");
-        on_device(*r, p->tableOut, "tableOut");
+        on_device(*r, p->blockTable, "blockTable", checked);
+        on_device(*r, p->tableOut, "tableOut", checked);
         FA_THROW_IF_NOT_MSG(p->tableOut != p->blockTable, "fork_blocks: outputs overlap inputs");
     }
-    on_device(*r, p->lengths, "lengths");
-    on_device(*r, p->spare, "spare");
-    on_device(*r, p->parents, "parents");
-    on_device(*r, p->lengthsOut, "lengthsOut");
-    on_device(*r, p->spareOut, "spareOut");
+    on_device(*r, p->lengths, "lengths", checked);
+    on_device(*r, p->spare, "spare", checked);
+    on_device(*r, p->parents, "parents", checked);
+    on_device(*r, p->lengthsOut, "lengthsOut", checked);
+    on_device(*r, p->spareOut, "spareOut", checked);
     FA_THROW_IF_NOT_MSG(p->lengthsOut != p->lengths && p->spareOut != p->spare, "fork_blocks: outputs overlap inputs");
     ForkArgs a;
     a.table = p->blockTable;

@@ -132,11 +132,11 @@ namespace faiss_amd {
 class GpuResources;
 void plan_blocks(const GpuResources* r, const FaissAmdPlanBlocksParams* p, hipStream_t stream);
 void cache_add(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAmdCacheAddParams* p, hipStream_t stream);
-void cache_reconstruct(const GpuResources* r, const FaissAmdPagedCache* c, int n, const int* blocks, int type, void* keys, void* values, hipStream_t stream);
+void cache_reconstruct(const GpuResources* r, const FaissAmdPagedCache* c, int n, const int* blocks, int type, void* keys, void* values, int checked, hipStream_t stream);
 // bytes: no launch, the workspace that the call needs instead
 void cache_attend(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAmdAttendParams* p, hipStream_t stream, size_t* bytes);
 void beam_select(const GpuResources* r, const FaissAmdBeamSelectParams* p, hipStream_t stream, size_t* bytes);
-void reorder_beams(const GpuResources* r, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams, int keep, hipStream_t stream);
+void reorder_beams(const GpuResources* r, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams, int keep, int checked, hipStream_t stream);
 void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* p, hipStream_t stream);
 
 } // namespace faiss_amd

@@ -99,8 +99,126 @@ __device__ __forceinline__ int plan_slot(const PlanArgs& a, const PlanScratch& s
     return (unsigned)p < (unsigned)a.numBlocks ? p * bs + (pos - col * bs) : -1;
 }
 
-// ALL: table and slots too, for calls of few tokens -- one workgroup and one launch
-template <bool ALL>
+// All of it in one workgroup, for batches of up to a thread per request: sums of 32 bits (a request asks for no more than one block
+// or slot beyond what there is -- it is refused then either way), what the requests hold is kept in LDS, and the blocks and slots
+// of the call are dealt to the threads one by one.
+constexpr int kPlanSmallTokens = 1 << 20; // (1024 requests of them fit 32 bits)
+struct PlanLds {
+    int oldLen[kPlanThreads], newLen[kPlanThreads];
+    int take[kPlanThreads + 1], give[kPlanThreads + 1], off[kPlanThreads + 1]; // where a request's blocks and slots begin
+};
+// last request that begins at or before t
+__device__ __forceinline__ int plan_owner(const int* start, int n, int t) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (start[mid] <= t)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+__device__ __forceinline__ int wg_scan(int x, int* part) { // inclusive, every thread calls it
+    const int lane = lane64(), wave = threadIdx.x >> 6;
+    x = (int)wave_incl_scan((unsigned)x);
+    __syncthreads();
+    if (lane == 63) part[wave] = x;
+    __syncthreads();
+    int before = lane < wave ? part[lane] : 0; // (at most 16 wavefronts)
+    before = __builtin_amdgcn_readlane((int)wave_incl_scan((unsigned)before), 63);
+    return x + before;
+}
+
+// FILL: the table and the slots too (few tokens); else what plan_fill_kernel goes by
+template <bool FILL>
+__global__ __launch_bounds__(kPlanThreads) void plan_small_kernel(PlanArgs a) {
+    __shared__ PlanLds z;
+    __shared__ int part[kPlanThreads / 64], top[2];
+    const int b = threadIdx.x, bs = a.blockSize, N = a.numBlocks;
+    const unsigned cap = (unsigned)a.cols * (unsigned)bs;
+    int oldLen = 0, newLen = 0;
+    if (b < a.batch) {
+        oldLen = a.lengths[b];
+        newLen = a.newLengths[b];
+    }
+    long long h0 = a.state[0];
+    const long long count = min(max((long long)a.state[1], 0ll), (long long)N);
+    if (h0 < 0 || h0 >= N) h0 = ((h0 % N) + N) % N;
+    const int head = (int)h0;
+    if (b < 2) top[b] = 0;
+    const bool ok = b < a.batch && (unsigned)oldLen <= cap && (unsigned)newLen <= cap;
+    const int have = ok ? (int)(((unsigned)oldLen + bs - 1) / bs) : 0, want = ok ? (int)(((unsigned)newLen + bs - 1) / bs) : 0;
+    const int tok = ok ? min(max(newLen - oldLen, 0), a.maxTokens + 1) : 0, need = min(max(want - have, 0), a.maxTokens + 1);
+    const int ct = wg_scan(need, part), cn = wg_scan(tok, part);
+    const bool granted = ok && (tok == 0 || (ct <= count && cn <= a.maxTokens));
+    if (granted && tok > 0) {
+        atomicMax(&top[0], ct);
+        atomicMax(&top[1], cn);
+    }
+    const int mine = granted ? max(have - want, 0) : 0;
+    const int give = wg_scan(mine, part); // (its barriers order the maxima)
+    const int taken = top[0], placed = top[1];
+    if (b < a.batch) {
+        z.oldLen[b] = oldLen;
+        z.newLen[b] = newLen;
+        // (a refused request begins where the granted ones end: nothing is its own)
+        z.take[b] = min(ct - need, taken);
+        z.off[b] = min(cn - tok, placed);
+        z.give[b] = give - mine;
+        a.granted[b] = granted;
+        a.lengthsOut[b] = granted ? newLen : oldLen;
+        a.queryOffsets[b] = z.off[b];
+        if (b == a.batch - 1) {
+            z.give[a.batch] = give;
+            z.take[a.batch] = taken;
+            z.off[a.batch] = placed;
+        }
+    }
+    if (a.batch == 0 && b == 0) z.give[0] = z.take[0] = z.off[0] = 0;
+    __syncthreads();
+    const int given = z.give[a.batch];
+    if (b == 0) {
+        a.queryOffsets[a.batch] = placed;
+        a.stateOut[0] = ring_at(head, taken, N);
+        a.stateOut[1] = min(count - taken + given, (long long)N);
+    }
+    if (!FILL) {
+        const PlanScratch s = plan_scratch(a.scratch, a.batch);
+        if (b < a.batch) {
+            s.oldLen[b] = oldLen;
+            s.newLen[b] = newLen;
+            s.takeStart[b] = z.take[b];
+            s.giveStart[b] = z.give[b];
+        }
+        if (b == 0) {
+            s.head[0] = head;
+            s.head[1] = (int)count;
+        }
+        return;
+    }
+    for (int t = threadIdx.x; t < taken; t += kPlanThreads) {
+        const int r = plan_owner(z.take, a.batch, t), col = (z.oldLen[r] + bs - 1) / bs + (t - z.take[r]);
+        const int p = a.ring[ring_at(head, t, N)];
+        a.table[(int64_t)r * a.tableStride + col] = p;
+        if (a.owned) a.owned[(int64_t)r * a.ownedStride + col] = p;
+    }
+    for (int t = threadIdx.x; t < given; t += kPlanThreads) {
+        const int r = plan_owner(z.give, a.batch, t), col = (z.newLen[r] + bs - 1) / bs + (t - z.give[r]);
+        a.ring[ring_at(head, (u64)count + t, N)] = a.owned ? a.owned[(int64_t)r * a.ownedStride + col] : a.table[(int64_t)r * a.tableStride + col];
+    }
+    for (int t = threadIdx.x; t < a.maxTokens; t += kPlanThreads) {
+        int slot = -1;
+        if (t < placed) {
+            const int r = plan_owner(z.off, a.batch, t), pos = z.oldLen[r] + (t - z.off[r]), col = pos / bs, first = (z.oldLen[r] + bs - 1) / bs;
+            const int p = col >= first ? a.ring[ring_at(head, z.take[r] + (col - first), N)] : a.table[(int64_t)r * a.tableStride + col];
+            if ((unsigned)p < (unsigned)N) slot = p * bs + (pos - col * bs);
+        }
+        a.slots[t] = slot;
+    }
+}
+
+// batches of any size
 __global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(PlanArgs a) {
     __shared__ u64 part[kPlanThreads / 64][2];
     __shared__ u64 tot[2];
@@ -171,10 +289,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(PlanArgs a) {
         a.stateOut[0] = ring_at((int)h0, taken, a.numBlocks);
         a.stateOut[1] = min(count - (long long)taken + (long long)giveBase, (long long)a.numBlocks);
     }
-    if (!ALL) return;
-    __syncthreads();
-    for (int b = threadIdx.x >> 6; b < a.batch; b += kPlanThreads / 64) plan_fill_blocks(a, s, b, threadIdx.x & 63, 64);
-    for (int t = threadIdx.x; t < a.maxTokens; t += kPlanThreads) a.slots[t] = plan_slot(a, s, t);
 }
 
 constexpr int kPlanSlots = 1024; // per workgroup
@@ -840,7 +954,22 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderTable tab, int
     uint8_t* out = (uint8_t*)s.out + row * s.rowBytes + at;
     const bool none = parent < 0 || parent >= beams; // such a row becomes zero
     const uint8_t* in = (const uint8_t*)s.in + (int64_t)b * s.inBatchBytes + (int64_t)(none ? 0 : parent) * s.inBeamBytes + at;
-    for (int64_t i = threadIdx.x; i < len; i += 256) out[i] = none ? 0 : in[i];
+    // rows of any length lie anywhere: 16 bytes at a time where the output is aligned (the loads need not be), single ones around
+    const int head = (int)min(len, (int64_t)((16 - ((uintptr_t)out & 15)) & 15)), mid = (int)(len - head) / 16, done = head + 16 * mid;
+    u32x4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int i = threadIdx.x + 256 * j;
+        v[j] = u32x4{0u, 0u, 0u, 0u};
+        if (i < mid && !none) __builtin_memcpy(&v[j], in + head + 16 * i, 16);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int i = threadIdx.x + 256 * j;
+        if (i < mid) *(u32x4*)(out + head + 16 * i) = v[j];
+    }
+    const int edge = threadIdx.x < 16 ? threadIdx.x : done + threadIdx.x - 16;
+    if (threadIdx.x < 16 ? edge < head : edge < len) out[edge] = none ? 0 : in[edge];
 }
 
 struct ForkTable {
@@ -901,13 +1030,18 @@ void beam_sched(const BeamArgs& a, int num_cus, BeamSched& s, size_t& bytes) {
 size_t plan_scratch_ints(int batch) { return (size_t)batch * 4 + 2; }
 
 void launch_plan_blocks(const PlanArgs& a, hipStream_t stream) {
-    if (a.maxTokens <= 4 * kPlanThreads && a.batch <= kPlanThreads) {
-        plan_scan_kernel<true><<<1, kPlanThreads, 0, stream>>>(a);
-    } else {
-        plan_scan_kernel<false><<<1, kPlanThreads, 0, stream>>>(a);
-        HIP_CHECK(hipGetLastError());
-        plan_fill_kernel<<<(unsigned)(a.batch + div_up(a.maxTokens, kPlanSlots)), 256, 0, stream>>>(a);
-    }
+    // (cols: what a request returns is summed in 32 bits too)
+    const bool small = a.batch <= kPlanThreads && a.maxTokens <= kPlanSmallTokens && a.cols <= 1 << 20;
+    const bool fill = small && a.maxTokens <= 4 * kPlanThreads;
+    if (fill)
+        plan_small_kernel<true><<<1, kPlanThreads, 0, stream>>>(a);
+    else if (small)
+        plan_small_kernel<false><<<1, kPlanThreads, 0, stream>>>(a);
+    else
+        plan_scan_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+    HIP_CHECK(hipGetLastError());
+    if (fill) return;
+    plan_fill_kernel<<<(unsigned)(a.batch + div_up(a.maxTokens, kPlanSlots)), 256, 0, stream>>>(a);
     HIP_CHECK(hipGetLastError());
 }
 

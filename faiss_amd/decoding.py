@@ -37,25 +37,25 @@ class _PlanStruct(ctypes.Structure):
     _fields_ = [("blockTable", _P), ("ownedTable", _P), ("tableStride", _I64), ("ownedStride", _I64), ("lengths", _P),
                 ("newLengths", _P), ("freeRing", _P), ("freeState", _P), ("lengthsOut", _P), ("freeStateOut", _P),
                 ("queryOffsets", _P), ("slots", _P), ("granted", _P), ("workspace", _P), ("batch", _I), ("numColumns", _I),
-                ("numBlocks", _I), ("blockSize", _I), ("maxTokens", _I)]
+                ("numBlocks", _I), ("blockSize", _I), ("maxTokens", _I), ("pointersChecked", _I)]
 
 
 class _AddStruct(ctypes.Structure):
     _fields_ = [("keys", _P), ("values", _P), ("keyTokenStride", _I64), ("keyHeadStride", _I64), ("valueTokenStride", _I64),
-                ("valueHeadStride", _I64), ("slots", _P), ("tokens", _I), ("type", _I)]
+                ("valueHeadStride", _I64), ("slots", _P), ("tokens", _I), ("type", _I), ("pointersChecked", _I)]
 
 
 class _AttendStruct(ctypes.Structure):
     _fields_ = [("queries", _P), ("out", _P), ("lse", _P), ("queryTokenStride", _I64), ("queryHeadStride", _I64),
                 ("outTokenStride", _I64), ("outHeadStride", _I64), ("blockTable", _P), ("tableStride", _I64), ("lengths", _P),
                 ("queryOffsets", _P), ("batch", _I), ("tokens", _I), ("heads", _I), ("numColumns", _I), ("maxQueries", _I),
-                ("type", _I), ("causal", _I), ("scale", _F), ("workspace", _P), ("workspaceBytes", _SZ)]
+                ("type", _I), ("causal", _I), ("pointersChecked", _I), ("scale", _F), ("workspace", _P), ("workspaceBytes", _SZ)]
 
 
 class _BeamStruct(ctypes.Structure):
     _fields_ = [("logits", _P), ("batchStride", _I64), ("beamStride", _I64), ("scores", _P), ("finished", _P), ("outScores", _P),
                 ("outParents", _P), ("outTokens", _P), ("vocab", _I64), ("batch", _I), ("beams", _I), ("keep", _I),
-                ("padToken", _I), ("type", _I), ("workspace", _P), ("workspaceBytes", _SZ)]
+                ("padToken", _I), ("type", _I), ("pointersChecked", _I), ("workspace", _P), ("workspaceBytes", _SZ)]
 
 
 class _StateStruct(ctypes.Structure):
@@ -64,7 +64,7 @@ class _StateStruct(ctypes.Structure):
 
 class _ForkStruct(ctypes.Structure):
     _fields_ = [("blockTable", _P), ("tableStride", _I64), ("lengths", _P), ("spare", _P), ("parents", _P), ("tableOut", _P),
-                ("lengthsOut", _P), ("spareOut", _P), ("batch", _I), ("beams", _I), ("numColumns", _I)]
+                ("lengthsOut", _P), ("spareOut", _P), ("batch", _I), ("beams", _I), ("numColumns", _I), ("pointersChecked", _I)]
 
 
 _byref = ctypes.byref
@@ -110,8 +110,16 @@ def _dense_last(t, name):
         raise ValueError("the last dimension of %s must be dense" % name)
 
 
+try:  # the same number without a Stream object around it (a microsecond of every call)
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # a torch without CUDA / HIP
+
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
+
+
 def _stream(res):
-    return torch.cuda.current_stream(res.device).cuda_stream
+    return _raw_stream(res.device)
 
 
 def _device(res):
@@ -139,24 +147,24 @@ def plan_blocks(res, block_table, lengths, new_lengths, free_ring, free_state, b
         if owned_table.shape != block_table.shape:
             raise ValueError("owned_table must have the shape of block_table")
     dev = _device(res)
-    if lengths_out is None:
-        lengths_out = torch.empty(n, dtype=torch.int32, device=dev)
-    else:
+    if lengths_out is not None:
         _same_length(_tensor(res, lengths_out, "lengths_out", torch.int32, 1), n, "lengths_out")
     if free_state_out is None:
         free_state_out = torch.empty(2, dtype=torch.int64, device=dev)
     else:
         _same_length(_tensor(res, free_state_out, "free_state_out", torch.int64, 1), 2, "free_state_out")
     max_tokens = int(max_tokens)
-    # offsets, grants and scratch in one allocation
-    ints = torch.empty(6 * n + 3, dtype=torch.int32, device=dev)
-    offsets, granted, scratch = ints[:n + 1], ints[n + 1:2 * n + 1], ints[2 * n + 1:]
-    slots = torch.empty(max(max_tokens, 0), dtype=torch.int32, device=dev)
+    # everything that is made here in one allocation
+    made = 0 if lengths_out is not None else n
+    offsets, granted, scratch, slots, own = torch.empty(6 * n + 3 + max(max_tokens, 0) + made, dtype=torch.int32, device=dev).split(
+        [n + 1, n, 4 * n + 2, max(max_tokens, 0), made])
+    if lengths_out is None:
+        lengths_out = own
     a = _PlanStruct(block_table.data_ptr() or None, owned_table.data_ptr() if owned_table is not None else None,
                     _row_stride(block_table), _row_stride(owned_table) if owned_table is not None else 0, lengths.data_ptr() or None,
                     new_lengths.data_ptr() or None, free_ring.data_ptr() or None, free_state.data_ptr(), lengths_out.data_ptr() or None,
                     free_state_out.data_ptr(), offsets.data_ptr(), slots.data_ptr() or None, granted.data_ptr(), scratch.data_ptr(),
-                    n, cols, free_ring.shape[0], int(block_size), max_tokens)
+                    n, cols, free_ring.shape[0], int(block_size), max_tokens, 1)
     _check(res._lib.faiss_amd_plan_blocks(res._h, _byref(a), _stream(res)))
     return BlockPlan(lengths_out, free_state_out, offsets, slots, granted)
 
@@ -206,6 +214,7 @@ class PagedCache:
         self._s = _CacheStruct(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), _CODE_OF[k.dtype], n, b, h, d)
         self._ref = _byref(self._s)
         self._lib = load_library()
+        self._workspaces = {}
 
     def add(self, k, v, slots):
         """store the tokens k, v [tokens, num_heads, head_dim] (float16 / bfloat16) at slots [tokens] (int32; -1: skipped)"""
@@ -221,7 +230,7 @@ class PagedCache:
         _same_length(v, n, "v")
         _same_length(_tensor(res, slots, "slots", torch.int32, 1), n, "slots")
         a = _AddStruct(k.data_ptr() or None, v.data_ptr() or None, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                       slots.data_ptr() or None, n, _HALF[k.dtype])
+                       slots.data_ptr() or None, n, _HALF[k.dtype], 1)
         _check(self._lib.faiss_amd_PagedCache_add(res._h, self._ref, _byref(a), _stream(res)))
 
     def reconstruct(self, blocks, dtype=torch.float32):
@@ -233,7 +242,7 @@ class PagedCache:
         shape = (blocks.shape[0], self.num_heads, self.block_size, self.head_dim)
         k, v = torch.empty(shape, dtype=dtype, device=blocks.device), torch.empty(shape, dtype=dtype, device=blocks.device)
         _check(self._lib.faiss_amd_PagedCache_reconstruct(res._h, self._ref, shape[0], blocks.data_ptr() or None, _FLOAT[dtype],
-                                                          k.data_ptr() or None, v.data_ptr() or None, _stream(res)))
+                                                          k.data_ptr() or None, v.data_ptr() or None, 1, _stream(res)))
         return k, v
 
     def attend(self, q, block_table, lengths, query_offsets=None, scale=None, causal=True, max_queries=None, out=None,
@@ -276,14 +285,21 @@ class PagedCache:
         a = _AttendStruct(q.data_ptr() or None, out.data_ptr() or None, lse.data_ptr() if return_lse else None, q.stride(0), q.stride(1),
                           out.stride(0), out.stride(1), block_table.data_ptr() or None, _row_stride(block_table), lengths.data_ptr() or None,
                           query_offsets.data_ptr() if query_offsets is not None else None, n, t, h, block_table.shape[1],
-                          max(most, 0), _HALF[q.dtype], 1 if causal else 0, 1.0 / math.sqrt(d) if scale is None else float(scale),
+                          max(most, 0), _HALF[q.dtype], 1 if causal else 0, 1, 1.0 / math.sqrt(d) if scale is None else float(scale),
                           None, 0)
         lib, ref = self._lib, _byref(a)
-        size = _SZ(0)
-        _check(lib.faiss_amd_PagedCache_attend_workspace(res._h, self._ref, ref, _byref(size)))
-        if size.value:
-            ws = torch.empty(size.value, dtype=torch.uint8, device=q.device)
-            a.workspace, a.workspaceBytes = ws.data_ptr(), size.value
+        # (the size follows from these numbers alone)
+        sizes = (n, t, h, block_table.shape[1], a.maxQueries, query_offsets is None)
+        need = self._workspaces.get(sizes)
+        if need is None:
+            size = _SZ(0)
+            _check(lib.faiss_amd_PagedCache_attend_workspace(res._h, self._ref, ref, _byref(size)))
+            if len(self._workspaces) > 1000:
+                self._workspaces.clear()
+            need = self._workspaces[sizes] = size.value
+        if need:
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+            a.workspace, a.workspaceBytes = ws.data_ptr(), need
         _check(lib.faiss_amd_PagedCache_attend(res._h, self._ref, ref, _stream(res)))
         return (out, lse) if return_lse else out
 
@@ -315,12 +331,19 @@ def beam_select(res, logits, scores, num_beams, finished=None, pad_token=0):
     parents, tokens = which[0], which[1]
     a = _BeamStruct(logits.data_ptr() or None, logits.stride(0), logits.stride(1), scores.data_ptr() or None,
                     finished.data_ptr() if finished is not None else None, out.data_ptr() or None, parents.data_ptr() or None,
-                    tokens.data_ptr() or None, v, n, w, k, int(pad_token), _FLOAT[logits.dtype], None, 0)
+                    tokens.data_ptr() or None, v, n, w, k, int(pad_token), _FLOAT[logits.dtype], 1, None, 0)
     lib, ref = res._lib, _byref(a)
-    size = _SZ(0)
-    _check(lib.faiss_amd_beam_select_workspace(res._h, ref, _byref(size)))
-    ws = torch.empty(size.value, dtype=torch.uint8, device=dev)
-    a.workspace, a.workspaceBytes = ws.data_ptr() or None, size.value
+    # (the size follows from these numbers alone)
+    known = res.__dict__.setdefault("_beam_workspaces", {})
+    need = known.get((n, w, v, k))
+    if need is None:
+        size = _SZ(0)
+        _check(lib.faiss_amd_beam_select_workspace(res._h, ref, _byref(size)))
+        if len(known) > 1000:
+            known.clear()
+        need = known[n, w, v, k] = size.value
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspaceBytes = ws.data_ptr() or None, need
     _check(lib.faiss_amd_beam_select(res._h, ref, _stream(res)))
     return out, parents, tokens
 
@@ -340,15 +363,19 @@ def reorder_beams(res, states, parents):
             w = t.shape[1]
         if t.shape[1] != w or w < 1:
             raise ValueError("the states must have the same number of beams")
-        if not t[:1, :1].is_contiguous():
-            raise ValueError("the rows of states[%d] must be dense" % i)
+        if t.numel() and not t.is_contiguous():
+            width = 1
+            for m, st in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
+                if m > 1 and st != width:
+                    raise ValueError("the rows of states[%d] must be dense" % i)
+                width *= m
         out = torch.empty((n, k) + tuple(t.shape[2:]), dtype=t.dtype, device=t.device)
         outs.append(out)
         size = t.element_size()
         arr[i] = _StateStruct(t.data_ptr() or None, out.data_ptr() or None, t.stride(0) * size, t.stride(1) * size,
                               math.prod(t.shape[2:]) * size)
     if outs:
-        _check(res._lib.faiss_amd_reorder_beams(res._h, len(outs), arr, parents.data_ptr() or None, n, w, k, _stream(res)))
+        _check(res._lib.faiss_amd_reorder_beams(res._h, len(outs), arr, parents.data_ptr() or None, n, w, k, 1, _stream(res)))
     return outs
 
 
@@ -375,7 +402,7 @@ def fork_blocks(res, caches, block_table, lengths, spare, parents):
                        torch.empty(rows, dtype=torch.int32, device=dev))
     arr = (_CacheStruct * len(caches))(*[c._s for c in caches])
     a = _ForkStruct(block_table.data_ptr() or None, _row_stride(block_table), lengths.data_ptr() or None, spare.data_ptr() or None,
-                    parents.data_ptr() or None, table.data_ptr() or None, lens.data_ptr() or None, sp.data_ptr() or None, n, w, cols)
+                    parents.data_ptr() or None, table.data_ptr() or None, lens.data_ptr() or None, sp.data_ptr() or None, n, w, cols, 1)
     if rows:
         _check(res._lib.faiss_amd_fork_blocks(res._h, len(caches), arr, _byref(a), _stream(res)))
     return table, lens, sp

@@ -486,7 +486,9 @@ int faiss_amd_GpuIndexIVF_list_major_rule(const FaissAmdIndex* index, int64_t n,
  *                              values [numBlocks][numHeads][headDim][blockSize], one byte each, 16-byte aligned
  *                              keyScales, valueScales [numBlocks][numHeads]; a value is code * scale.
  *      code: 0 = int8, 1 = e4m3; blockSize: 16, 32, 64, 128, 256; headDim: 64, 96, 128, 192, 256; numBlocks * blockSize < 2^31.
- *      Types of other operands: 1 = F32, 2 = F16, 3 = BF16 (DistanceDataType). */
+ *      Types of other operands: 1 = F32, 2 = F16, 3 = BF16 (DistanceDataType).
+ *      pointersChecked: 0 = every pointer is looked up (0.4 us each) and refused if it is no memory of res's device; otherwise the
+ *      caller has done so, as the Python mirror has, and only null pointers are refused. */
 typedef struct FaissAmdPagedCache {
     void *keys, *values;
     float *keyScales, *valueScales;
@@ -513,7 +515,7 @@ typedef struct FaissAmdPlanBlocksParams {
     int* lengthsOut;
     int64_t* freeStateOut;
     int *queryOffsets, *slots, *granted, *workspace;
-    int batch, numColumns, numBlocks, blockSize, maxTokens;
+    int batch, numColumns, numBlocks, blockSize, maxTokens, pointersChecked;
 } FaissAmdPlanBlocksParams;
 int faiss_amd_plan_blocks(FaissAmdGpuResources* res, const FaissAmdPlanBlocksParams* args, void* stream);
 
@@ -527,13 +529,13 @@ typedef struct FaissAmdCacheAddParams {
     const void *keys, *values;
     int64_t keyTokenStride, keyHeadStride, valueTokenStride, valueHeadStride;
     const int* slots;
-    int tokens, type;
+    int tokens, type, pointersChecked;
 } FaissAmdCacheAddParams;
 int faiss_amd_PagedCache_add(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdCacheAddParams* args, void* stream);
 
 /* Reads blocks back: keys, values [n][numHeads][blockSize][headDim] of the given type; NaN for a block id out of range. */
 int faiss_amd_PagedCache_reconstruct(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, int n, const int* blocks, int type,
-                                     void* keys, void* values, void* stream);
+                                     void* keys, void* values, int pointersChecked, void* stream);
 
 /* Attention: out[r][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q[r][h] . k_j), query head h over key-value head
  * h / (heads / numHeads).  Request b's queries are the rows queryOffsets[b] ... queryOffsets[b + 1] - 1 (NULL: row b; offsets
@@ -551,7 +553,7 @@ typedef struct FaissAmdAttendParams {
     const int* blockTable;
     int64_t tableStride;
     const int *lengths, *queryOffsets;
-    int batch, tokens, heads, numColumns, maxQueries, type, causal;
+    int batch, tokens, heads, numColumns, maxQueries, type, causal, pointersChecked;
     float scale;
     void* workspace;
     size_t workspaceBytes;
@@ -573,7 +575,7 @@ typedef struct FaissAmdBeamSelectParams {
     float* outScores;
     int *outParents, *outTokens;
     int64_t vocab;
-    int batch, beams, keep, padToken, type;
+    int batch, beams, keep, padToken, type, pointersChecked;
     void* workspace;
     size_t workspaceBytes;
 } FaissAmdBeamSelectParams;
@@ -588,7 +590,7 @@ typedef struct FaissAmdBeamState {
     int64_t batchBytes, beamBytes, rowBytes; /* strides of `in` */
 } FaissAmdBeamState;
 int faiss_amd_reorder_beams(FaissAmdGpuResources* res, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams,
-                            int keep, void* stream);
+                            int keep, int pointersChecked, void* stream);
 
 /* Reorders beams over paged caches (`caches`: host array of n, all layers that the table leads to): row b * beams + j takes over
  * the blocks of row b * beams + parents[b][j] (its own if that is out of range).  Full blocks are shared; a partly filled last
@@ -601,7 +603,7 @@ typedef struct FaissAmdForkBlocksParams {
     int64_t tableStride;
     const int *lengths, *spare, *parents;
     int *tableOut, *lengthsOut, *spareOut;
-    int batch, beams, numColumns;
+    int batch, beams, numColumns, pointersChecked;
 } FaissAmdForkBlocksParams;
 int faiss_amd_fork_blocks(FaissAmdGpuResources* res, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* args, void* stream);
 

@@ -38,7 +38,7 @@ def test_a_cache_of_another_kind_is_refused(kw, say):
     assert say in _attend(_cache(**kw))
     add = decoding._AddStruct(type=3, tokens=1)
     assert say in _error("faiss_amd_PagedCache_add", None, ctypes.byref(_cache(**kw)), ctypes.byref(add), None)
-    assert say in _error("faiss_amd_PagedCache_reconstruct", None, ctypes.byref(_cache(**kw)), 1, None, 1, None, None, None)
+    assert say in _error("faiss_amd_PagedCache_reconstruct", None, ctypes.byref(_cache(**kw)), 1, None, 1, None, None, 0, None)
 
 
 @pytest.mark.parametrize("kw, say", [
@@ -80,9 +80,9 @@ def test_plan_blocks_refuses(kw, say):
 
 
 def test_reorder_and_fork_refuse():
-    assert "null resources" in _error("faiss_amd_reorder_beams", None, 1, None, None, 1, 2, 2, None)
-    assert "negative" in _error("faiss_amd_reorder_beams", None, -1, None, None, 1, 2, 2, None)
-    assert "negative" in _error("faiss_amd_reorder_beams", None, 1, None, None, 1, 0, 2, None)
+    assert "null resources" in _error("faiss_amd_reorder_beams", None, 1, None, None, 1, 2, 2, 0, None)
+    assert "negative" in _error("faiss_amd_reorder_beams", None, -1, None, None, 1, 2, 2, 0, None)
+    assert "negative" in _error("faiss_amd_reorder_beams", None, 1, None, None, 1, 0, 2, 0, None)
     fork = dict(tableStride=4, batch=1, beams=2, numColumns=4)
     two = (decoding._CacheStruct * 2)(_cache(), _cache(blockSize=32))
     for kw, n, c, say in ((dict(), 1, two, "null resources"), (dict(), 2, two, "different blocks"), (dict(), 0, two, "at least one"),

@@ -778,7 +778,7 @@ def test_refusals_on_the_device(res):
     import ctypes
     lib = faiss_amd.load_library()
     host = torch.zeros(64, dtype=I32)
-    assert lib.faiss_amd_PagedCache_reconstruct(res._h, c._ref, 1, host.data_ptr(), 1, q.data_ptr(), q.data_ptr(), None) == -2
+    assert lib.faiss_amd_PagedCache_reconstruct(res._h, c._ref, 1, host.data_ptr(), 1, q.data_ptr(), q.data_ptr(), 0, None) == -2
     assert b"device memory" in lib.faiss_amd_get_last_error() or b"resources' device" in lib.faiss_amd_get_last_error()
-    a = decoding._BeamStruct(q.data_ptr(), 8, 8, t.data_ptr(), None, q.data_ptr(), q.data_ptr(), q.data_ptr(), 8, 1, 1, 1, 0, 2, q.data_ptr(), 1)
+    a = decoding._BeamStruct(q.data_ptr(), 8, 8, t.data_ptr(), None, q.data_ptr(), q.data_ptr(), q.data_ptr(), 8, 1, 1, 1, 0, 2, 0, q.data_ptr(), 1)
     assert lib.faiss_amd_beam_select(res._h, ctypes.byref(a), None) == -2 and b"workspace" in lib.faiss_amd_get_last_error()
