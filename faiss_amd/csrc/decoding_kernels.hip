@@ -936,13 +936,15 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSc
 }
 
 // ================================================================================================ reordering by parent
-struct ReorderTable {
-    ReorderState st[kMaxReorderStates];
-    int first[kMaxReorderStates + 1]; // workgroups of a row before state i
+template <int CAP>
+struct ReorderTable { // (a kernel's argument: a launch of few states carries few)
+    ReorderState st[CAP];
+    int first[CAP + 1]; // workgroups of a row before state i
 };
 constexpr int kReorderBytes = 16384; // of a row per workgroup
 
-__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderTable tab, int n, const int* parents, int beams, int keep) {
+template <int CAP>
+__global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderTable<CAP> tab, int n, const int* parents, int beams, int keep) {
     const int chunk = blockIdx.y;
     int lo = 0;
     while (lo + 1 < n && tab.first[lo + 1] <= chunk) ++lo;
@@ -1116,23 +1118,31 @@ void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream) {
     HIP_CHECK(hipGetLastError());
 }
 
-void launch_beam_reorder(const ReorderState* states, int n, const int* parents, int batch, int beams, int keep, hipStream_t stream) {
-    const int64_t rows = (int64_t)batch * keep;
-    if (rows == 0) return;
-    ReorderTable tab;
-    int k = 0;
+template <int CAP>
+static void launch_reorder(const ReorderState* states, int n, const int* parents, int64_t rows, int beams, int keep, hipStream_t stream) {
+    ReorderTable<CAP> tab;
     int64_t first = 0;
     for (int i = 0; i < n; ++i) {
-        if (states[i].rowBytes == 0) continue;
-        tab.st[k] = states[i];
-        tab.first[k++] = (int)first;
+        tab.st[i] = states[i];
+        tab.first[i] = (int)first;
         first += (states[i].rowBytes + kReorderBytes - 1) / kReorderBytes;
         FA_THROW_IF_NOT_MSG(first <= 65535, "reorder: rows too long for one call");
     }
-    if (k == 0) return;
-    tab.first[k] = (int)first;
-    beam_reorder_kernel<<<dim3((unsigned)rows, (unsigned)first), 256, 0, stream>>>(tab, k, parents, beams, keep);
+    tab.first[n] = (int)first;
+    beam_reorder_kernel<CAP><<<dim3((unsigned)rows, (unsigned)first), 256, 0, stream>>>(tab, n, parents, beams, keep);
     HIP_CHECK(hipGetLastError());
+}
+void launch_beam_reorder(const ReorderState* states, int n, const int* parents, int batch, int beams, int keep, hipStream_t stream) {
+    const int64_t rows = (int64_t)batch * keep;
+    ReorderState some[kMaxReorderStates];
+    int k = 0;
+    for (int i = 0; i < n; ++i)
+        if (states[i].rowBytes > 0) some[k++] = states[i];
+    if (rows == 0 || k == 0) return;
+    if (k <= 8)
+        launch_reorder<8>(some, k, parents, rows, beams, keep, stream);
+    else
+        launch_reorder<kMaxReorderStates>(some, k, parents, rows, beams, keep, stream);
 }
 
 void launch_fork_blocks(const ForkArgs& a, const CacheView* caches, int n, hipStream_t stream) {

@@ -353,28 +353,34 @@ def reorder_beams(res, states, parents):
     (parents [batch, num] int32; a row whose parent is out of range becomes zero).  A state's rows must be dense."""
     _tensor(res, parents, "parents", torch.int32, 2)
     n, k = parents.shape
-    arr = (_StateStruct * len(states))()
-    outs, w = [], None
+    outs, flat, w = [], [], None
     for i, t in enumerate(states):
-        _tensor(res, t, "states[%d]" % i, dense=False)
-        if t.dim() < 2 or t.shape[0] != n:
+        _tensor(res, t, "a state", dense=False)
+        shape = t.shape
+        if len(shape) < 2 or shape[0] != n:
             raise ValueError("states[%d] must be [%d, beams, ...]" % (i, n))
         if w is None:
-            w = t.shape[1]
-        if t.shape[1] != w or w < 1:
+            w = shape[1]
+        if shape[1] != w or w < 1:
             raise ValueError("the states must have the same number of beams")
-        if t.numel() and not t.is_contiguous():
-            width = 1
-            for m, st in zip(reversed(t.shape[2:]), reversed(t.stride()[2:])):
-                if m > 1 and st != width:
-                    raise ValueError("the rows of states[%d] must be dense" % i)
-                width *= m
-        out = torch.empty((n, k) + tuple(t.shape[2:]), dtype=t.dtype, device=t.device)
-        outs.append(out)
+        row = shape[2:]
         size = t.element_size()
-        arr[i] = _StateStruct(t.data_ptr() or None, out.data_ptr() or None, t.stride(0) * size, t.stride(1) * size,
-                              math.prod(t.shape[2:]) * size)
+        width = math.prod(row) * size
+        if t.is_contiguous():
+            batch, beam = w * width, width
+        else:
+            dense = 1
+            for m, st in zip(reversed(row), reversed(t.stride()[2:])):
+                if m > 1 and st != dense and t.numel():
+                    raise ValueError("the rows of states[%d] must be dense" % i)
+                dense *= m
+            batch, beam = t.stride(0) * size, t.stride(1) * size
+        out = t.new_empty((n, k) + row)
+        outs.append(out)
+        flat += (t.data_ptr(), out.data_ptr(), batch, beam, width)
     if outs:
+        # (the array of FaissAmdBeamState as what it is, five 64-bit numbers each)
+        arr = (_I64 * len(flat))(*flat)
         _check(res._lib.faiss_amd_reorder_beams(res._h, len(outs), arr, parents.data_ptr() or None, n, w, k, 1, _stream(res)))
     return outs
 
