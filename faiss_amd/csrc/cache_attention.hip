@@ -271,12 +271,21 @@ __device__ __forceinline__ void load_queries(const AttendArgs& a, const Item& it
 // tok0: the lane group's first token; edge: some row does not see all 64; ks, lvs: the key scale and log2 of the value scale of the
 // lane group's block.  A value's scale goes into its probability's exponent, so the sum of the probabilities themselves is the
 // lane's sum times the inverse.  All row tiles are worked on between the same branches: they are independent chains.
+// nan: which of the lane group's 16 tokens have a value of code NaN that was taken out (edge steps only): rows that see one are NaN.
 template <int NT, int MD>
-__device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float lvs, int tok0, bool edge, Rows<NT, MD>& w, half8_t (&pr)[NT][2]) {
+__device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float lvs, int tok0, bool edge, unsigned nan, Rows<NT, MD>& w, half8_t (&pr)[NT][2]) {
     float f[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) f[t] = ks * w.qs[t];
     if (edge) {
+        if (__ballot(nan != 0)) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[t][i][e] = (nan >> (4 * i + e)) & 1 ? __builtin_nanf("") : sc[t][i][e];
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -347,9 +356,9 @@ __device__ __forceinline__ void look_up(const AttendArgs& a, const Item& it, int
             if ((unsigned)p < (unsigned)a.cache.numBlocks) {
                 ks = a.cache.ks[(int64_t)p * a.cache.numHeads + it.h];
                 vs = a.cache.vs[(int64_t)p * a.cache.numHeads + it.h];
-                // a scale that is negative or no number, of the values also an infinite one, makes the scores NaN: the rows that
+                // a scale that is negative, infinite or no number makes the scores NaN: the rows that
                 // see the block become NaN, those that mask it do not
-                if (!(ks >= 0.f) || !(vs >= 0.f && vs < INFINITY)) ks = __builtin_nanf("");
+                if (!(ks >= 0.f && ks < INFINITY && vs >= 0.f && vs < INFINITY)) ks = __builtin_nanf("");
             } else {
                 p = -1;
                 ks = __builtin_nanf("");
@@ -373,6 +382,21 @@ __device__ __forceinline__ u32x4 cut_tokens(u32x4 w, int valid) {
         w[i] &= nb == 4 ? ~0u : (1u << (8 * nb)) - 1u;
     }
     return w;
+}
+// The 16 tokens of a word quadruple with a NaN code (e4m3 0x7f, 0xff), which are taken out.  Zero times NaN is NaN: a value of
+// that code would reach the rows that mask its token too.
+template <int CODE>
+__device__ __forceinline__ unsigned take_nan(u32x4& w) {
+    unsigned m = 0;
+    if constexpr (CODE == CACHE_E4M3) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned f = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+            m |= ((f >> 7 & 1u) | (f >> 14 & 2u) | (f >> 21 & 4u) | (f >> 28 & 8u)) << (4 * i);
+            w[i] &= ~((f >> 7) * 0xffu);
+        }
+    }
+    return m;
 }
 __device__ __forceinline__ float log_sum(float m, float l) {
     return l == 0.f ? -INFINITY : (m - kBias + __builtin_amdgcn_logf(l)) * kLn2;
@@ -485,7 +509,14 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
             }
             if (tile + kWaves < segEnd) fetch_k(tile + kWaves, z.page[u + 4 * kWaves + (n16 >> 2)]);
             half8_t pr[NT][2];
-            softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, w, pr);
+            unsigned nan = 0;
+            if (CODE == CACHE_E4M3 && visMin < it.len && t0 + kTile > visMin) { // some rows mask tokens that others see
+#pragma unroll
+                for (int i = 0; i < MD; ++i) nan |= take_nan<CODE>(vr[i]);
+#pragma unroll
+                for (int o = 8; o; o >>= 1) nan |= (unsigned)__shfl_xor((int)nan, o, 64);
+            }
+            softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, nan, w, pr);
             if (t0 + kTile > it.len || __ballot(lvs == kNoScale)) {
 #pragma unroll
                 for (int i = 0; i < MD; ++i) vr[i] = cut_tokens(vr[i], lvs == kNoScale ? 0 : it.len - (t0 + 16 * grp));
@@ -578,6 +609,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
     __shared__ __align__(16) half8_t kf[2][4 * KS][64]; // fragment (i, k): tokens 16 g + 4 i + e in row 4 g + e, dimensions 32 k ...
     __shared__ __align__(16) half8_t vf[2][MD * 2][64]; // fragment (i, h): dimensions 16 i ..., tokens 16 grp + 8 h ...
 
+    __shared__ unsigned nanL[3][4]; // tokens with NaN codes of a tile's four groups; of this tile, the next, and one being cleared
+    const int visMinAll = visible(a, it, G, it.rt * ROWS);
+
     u32x4 kr[KW], vr[VW];
     // (every wavefront loads, also where there is nothing for it: a load under a condition waits for the loads before it)
     auto fetch = [&](int t, int seg0) {
@@ -608,7 +642,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
         for (int j = 0; j < VW; ++j) {
             const int i = wave + j * WAVES;
             if (i < MD) {
-                const u32x4 c = tail ? cut_tokens(vr[j], valid) : vr[j];
+                u32x4 c = tail ? cut_tokens(vr[j], valid) : vr[j];
+                if (CODE == CACHE_E4M3 && visMinAll < it.len && (t + 1) * kTile > visMinAll) { // some rows mask tokens that others see
+                    const unsigned nan = take_nan<CODE>(c);
+                    if (nan) atomicOr(&nanL[t % 3][grp], nan);
+                }
                 vf[buf][2 * i][lane] = widen<CODE>(u32x2{c[0], c[1]});
                 vf[buf][2 * i + 1][lane] = widen<CODE>(u32x2{c[2], c[3]});
             }
@@ -622,6 +660,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
         const int segEnd = min(seg0 + kSeg, endAll);
         __syncthreads(); // (the stretch before has been read)
         look_up(a, it, seg0, endAll, 64 * WAVES, z);
+        if (threadIdx.x < 12) nanL[threadIdx.x >> 2][threadIdx.x & 3] = 0;
         __syncthreads();
         fetch(seg0, seg0);
         lay(seg0, seg0, seg0 & 1);
@@ -630,6 +669,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
             const int buf = tile & 1, t0 = tile * kTile, u = (tile - seg0) * 4;
             const bool more = tile + 1 < segEnd;
             fetch(min(tile + 1, segEnd - 1), seg0);
+            if (threadIdx.x < 4) nanL[(tile + 2) % 3][threadIdx.x] = 0;
             if (tile < end) {
                 const float ks = z.ks[u + grp], lvs = z.lvs[u + grp];
                 f32x4 sc[NT][4];
@@ -659,7 +699,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
                     __builtin_amdgcn_sched_group_barrier(0x8, 4 * NT, 0);
                 }
                 half8_t pr[NT][2];
-                softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, w, pr);
+                softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, CODE == CACHE_E4M3 ? nanL[tile % 3][grp] : 0u, w, pr);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) fr[0][j] = vf[buf][j][lane];
                 __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);

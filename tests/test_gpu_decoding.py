@@ -216,6 +216,47 @@ def test_attend_masked_scales(res):
         assert not bool(torch.isfinite(got[32:]).all(-1).any())
 
 
+@pytest.mark.parametrize("nq, g", [(5, 2), (200, 1)])
+def test_attend_masked_nan_codes(res, nq, g):
+    """a NaN code of a key or a value reaches the rows that see its token, and no others"""
+    lens = [300]
+    c, table = paged(res, lens, 16, 1, 64, "e4m3", 3)
+    q = torch.randn((nq, g, 64), device="cuda").bfloat16()
+    offs = ints([0, nq])
+    want, _, tol = reference(c, q, table, lens, [0, nq], 1 / 8, True)
+    at = 300 - 3  # seen by the last three rows
+    page, off = int(table[0, at // 16]), at % 16
+    for codes, where in ((c.k_codes, (page, 0, off, 7)), (c.v_codes, (page, 0, 50, off))):
+        raw = codes.view(torch.uint8)
+        old = int(raw[where])
+        for code in (0x7f, 0xff):
+            raw[where] = code
+            got = c.attend(q, table, ints(lens), query_offsets=offs)
+            check(got[:nq - 3], None, want[:nq - 3], None, tol[:nq - 3])
+            assert bool(got[nq - 3:, :, 50].isnan().all())
+        raw[where] = old
+
+
+def test_attend_zero_and_negative_scales(res):
+    """values of a zero scale are zero whatever their codes; a negative scale counts as no number"""
+    lens = [100, 100]
+    c, table = paged(res, lens, 16, 2, 64, "int8", 4)
+    c.v_scales[table[0, 1].long()] = 0.0
+    c.k_scales[table[0, 2].long()] = 0.0
+    for nq in (1, 40):
+        q = torch.randn((2 * nq, 4, 64), device="cuda").half()
+        offs = ints([0, nq, 2 * nq])
+        want, _, tol = reference(c, q, table, lens, [0, nq, 2 * nq], 1 / 8, True)
+        check(c.attend(q, table, ints(lens), query_offsets=offs), None, want, None, tol)
+        for s in (c.k_scales, c.v_scales):
+            old = s.clone()
+            s[table[1, 0].long()] *= -1
+            got = c.attend(q, table, ints(lens), query_offsets=offs)
+            s.copy_(old)
+            check(got[:nq], None, want[:nq], None, tol[:nq])
+            assert bool(got[nq:].isnan().all())
+
+
 def test_attend_bad_blocks_and_lengths(res):
     """a row that reaches a block that does not exist is NaN; the others are what they were"""
     lens = [100, 100, 100, 100]
