@@ -674,11 +674,12 @@ __device__ __forceinline__ int wave_cut(u64* list, int n, u64 kth) {
     return out;
 }
 
-template <typename T>
+template <typename T, int ROUND>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s) {
     constexpr int PER = 16 / sizeof(T); // logits of a 16-byte load
     constexpr int LD = kBeamVpt / PER;
     __shared__ __align__(16) u64 lists[4][kBeamCap];
+    __shared__ unsigned short groups[4][64 * ROUND];
     __shared__ double ss[4];
     __shared__ float sm[4];
     __shared__ int sn[4];
@@ -700,77 +701,105 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s)
     const int64_t steps = (granules + 64 * LD - 1) / (64 * LD);
     u64* list = lists[wave];
     int n = 0;
-    float thr = -INFINITY; // only logits of at least this can be among the best; set once `keep` better ones are in the list
-    bool full = false;
+    float thr = -FLT_MAX; // only logits of at least this can be among the best (-inf is no candidate)
+    bool full = false;    // the list holds `keep` logits that are no smaller
     float m = -INFINITY;
     double sum = 0.0;
     const int64_t stride = (int64_t)s.parts * 4;
-    T next[kBeamVpt];
-    auto fetch = [&](int64_t st) {
+    auto fetch = [&](int64_t st, int l, T (&to)[kBeamVpt]) { // the logits of a lane in a step
 #pragma unroll
         for (int i = 0; i < LD; ++i) {
-            const int64_t e0 = ((st * LD + i) * 64 + lane) * PER;
+            const int64_t e0 = ((st * LD + i) * 64 + l) * PER;
             if (e0 + PER <= a.vocab) {
-                __builtin_memcpy(next + i * PER, x + e0, 16);
+                __builtin_memcpy(to + i * PER, x + e0, 16);
             } else {
 #pragma unroll
-                for (int e = 0; e < PER; ++e) next[i * PER + e] = e0 + e < a.vocab ? x[e0 + e] : (T)-INFINITY;
+                for (int e = 0; e < PER; ++e) to[i * PER + e] = e0 + e < a.vocab ? x[e0 + e] : (T)-INFINITY;
             }
         }
     };
+    T next[kBeamVpt];
     int64_t st = (int64_t)part * 4 + wave;
-    if (st < steps) fetch(st);
-    for (; st < steps; st += stride) {
-        float v[kBeamVpt];
+    if (st < steps) fetch(st, lane, next);
+    // ROUND steps at a time: their sums and the largest logit of every lane in every step; then, from what is still in the
+    // caches, the few lanes' logits again whose largest can be among the best
+    for (; st < steps; st += ROUND * stride) {
+        float best[ROUND];
 #pragma unroll
-        for (int i = 0; i < kBeamVpt; ++i) v[i] = (float)next[i];
-        if (st + stride < steps) fetch(st + stride);
-        float mx = v[0];
+        for (int j = 0; j < ROUND; ++j) {
+            best[j] = -INFINITY;
+            if (st + j * stride < steps) {
+                float v[kBeamVpt];
 #pragma unroll
-        for (int i = 1; i < kBeamVpt; ++i) mx = fmaxf(mx, v[i]);
-        // running maximum and sum of the lane; a NaN or an infinity makes the sum NaN
-        const float mn = fmaxf(m, mx);
-        float p = 0.f;
+                for (int i = 0; i < kBeamVpt; ++i) v[i] = (float)next[i];
+                if (st + (j + 1) * stride < steps) fetch(st + (j + 1) * stride, lane, next);
+                float mx = v[0];
 #pragma unroll
-        for (int i = 0; i < kBeamVpt; ++i) p += __builtin_amdgcn_exp2f((v[i] - mn) * 1.4426950408889634f);
-        if (mn == -INFINITY) { // (nothing but -inf so far, or a NaN among it)
-            p = 0.f;
+                for (int i = 1; i < kBeamVpt; ++i) mx = fmaxf(mx, v[i]);
+                best[j] = mx;
+                // running maximum and sum of the lane; a NaN or an infinity makes the sum NaN
+                const float mn = fmaxf(m, mx);
+                float p = 0.f;
 #pragma unroll
-            for (int i = 0; i < kBeamVpt; ++i) p = v[i] == v[i] ? p : v[i];
-            sum += (double)p;
-        } else {
-            sum = sum * (double)__builtin_amdgcn_exp2f((m - mn) * 1.4426950408889634f) + (double)p;
+                for (int i = 0; i < kBeamVpt; ++i) p += __builtin_amdgcn_exp2f((v[i] - mn) * 1.4426950408889634f);
+                if (mn == -INFINITY) { // (nothing but -inf so far, or a NaN among it)
+                    p = 0.f;
+#pragma unroll
+                    for (int i = 0; i < kBeamVpt; ++i) p = v[i] == v[i] ? p : v[i];
+                    sum += (double)p;
+                } else {
+                    sum = sum * (double)__builtin_amdgcn_exp2f((m - mn) * 1.4426950408889634f) + (double)p;
+                }
+                m = mn;
+            }
         }
-        m = mn;
-        float lim = thr;
         if (!full) {
-            // the keep-th best of the lanes' best logits bounds what can be among the keep best of this step
-            const unsigned best = mx > -INFINITY ? ~float_flip(mx) : ~0u;
-            unsigned t = 0;
-            for (int b = 31; b >= 0; --b) {
+            // the keep-th best of the lanes' best logits (of their upper 16 bits, rounded down) bounds the keep best
+            unsigned k[ROUND], t = 0;
+#pragma unroll
+            for (int j = 0; j < ROUND; ++j) k[j] = best[j] > -INFINITY ? ~float_flip(best[j]) >> 16 : 0xffffu;
+            for (int b = 15; b >= 0; --b) {
                 const unsigned c = t | ((1u << b) - 1);
-                if (__popcll(__ballot(best <= c)) < keep) t |= 1u << b;
-            }
-            lim = t == ~0u ? -INFINITY : float_unflip(~t);
-        }
-        if (!__ballot(mx >= lim && mx > -INFINITY)) continue;
-        const unsigned first = (unsigned)((st * LD * 64 + lane) * PER); // index of v[0]
+                int cnt = 0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (n > kBeamPend) n = wave_cut(list, n, wave_kth(list, n, keep));
-#pragma unroll
-            for (int j = 0; j < kBeamVpt / 2; ++j) {
-                const int i = half * (kBeamVpt / 2) + j;
-                const bool in = v[i] >= lim && v[i] > -INFINITY;
-                const u64 mask = __ballot(in);
-                if (!mask) continue;
-                if (in) list[n + lanes_before(mask)] = beam_key(v[i], first + (unsigned)(64 * PER * (i / PER) + i % PER));
-                n += __popcll(mask);
+                for (int j = 0; j < ROUND; ++j) cnt += __popcll(__ballot(k[j] <= c));
+                if (cnt < keep) t |= 1u << b;
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            thr = fmaxf(float_unflip(~((t << 16) | 0xffffu)), -FLT_MAX); // (NaN where there are fewer: -FLT_MAX)
         }
-        // a bound for the steps to come; renewed when there is something to gain from it
-        if (n > keep && (!full || n > keep + max(keep / 2, 8))) {
+        int ng = 0;
+#pragma unroll
+        for (int j = 0; j < ROUND; ++j) {
+            const u64 mask = __ballot(best[j] >= thr);
+            if (best[j] >= thr) groups[wave][ng + lanes_before(mask)] = (unsigned short)(64 * j + lane);
+            ng += __popcll(mask);
+        }
+        if (!ng) continue;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+        for (int g0 = 0; g0 < ng; g0 += 64) {
+            const bool is = g0 + lane < ng;
+            const int g = groups[wave][min(g0 + lane, ng - 1)];
+            const int64_t gs = st + (g >> 6) * stride;
+            T again[kBeamVpt];
+            fetch(gs, g & 63, again);
+            const unsigned first = (unsigned)((gs * LD * 64 + (g & 63)) * PER); // index of the first of them
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (n > kBeamPend) n = wave_cut(list, n, wave_kth(list, n, keep));
+#pragma unroll
+                for (int j = 0; j < kBeamVpt / 2; ++j) {
+                    const int i = half * (kBeamVpt / 2) + j;
+                    const float v = (float)again[i];
+                    const bool in = is && v >= thr;
+                    const u64 mask = __ballot(in);
+                    if (!mask) continue;
+                    if (in) list[n + lanes_before(mask)] = beam_key(v, first + (unsigned)(64 * PER * (i / PER) + i % PER));
+                    n += __popcll(mask);
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");
+            }
+        }
+        if (n > keep) {
             const u64 kth = wave_kth(list, n, keep);
             n = wave_cut(list, n, kth);
             thr = beam_logit(kth);
@@ -1100,6 +1129,16 @@ size_t beam_select_workspace(const BeamArgs& a, int num_cus) {
     beam_sched(a, num_cus, s, bytes);
     return bytes;
 }
+template <typename T>
+static void launch_beam_scan(const BeamArgs& a, const BeamSched& s, unsigned grid, hipStream_t stream) {
+    // eight steps between two selections, one where a wavefront has no more than two (4 x 32000 logits: 7.9 us against 10.5;
+    // 512 x 128001: 54 us with one, 43 with eight)
+    const int64_t step = 64 * kBeamVpt, per = 4 * (int64_t)s.parts * step;
+    if (a.vocab <= 2 * per)
+        beam_scan_kernel<T, 1><<<grid, 256, 0, stream>>>(a, s);
+    else
+        beam_scan_kernel<T, 8><<<grid, 256, 0, stream>>>(a, s);
+}
 void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream) {
     if (a.batch == 0) return;
     BeamSched s;
@@ -1108,11 +1147,11 @@ void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream) {
     const int64_t grid = (int64_t)a.batch * a.beams * s.parts;
     FA_THROW_IF_NOT_MSG(grid < ((int64_t)1 << 31), "beam_select: too many rows for one call");
     if (a.type == DT_F32)
-        beam_scan_kernel<float><<<(unsigned)grid, 256, 0, stream>>>(a, s);
+        launch_beam_scan<float>(a, s, (unsigned)grid, stream);
     else if (a.type == DT_F16)
-        beam_scan_kernel<_Float16><<<(unsigned)grid, 256, 0, stream>>>(a, s);
+        launch_beam_scan<_Float16>(a, s, (unsigned)grid, stream);
     else
-        beam_scan_kernel<__bf16><<<(unsigned)grid, 256, 0, stream>>>(a, s);
+        launch_beam_scan<__bf16>(a, s, (unsigned)grid, stream);
     HIP_CHECK(hipGetLastError());
     beam_join_kernel<<<a.batch, kBeamJoin, 0, stream>>>(a, s);
     HIP_CHECK(hipGetLastError());
