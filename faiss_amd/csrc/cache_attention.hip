@@ -340,7 +340,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
 // blocks and scales of a stretch of the context, looked up once: a wait for a block's number in the loop would be a wait for all
 // loads issued before it
 struct Stretch {
-    int page[4 * kSeg];
+    unsigned at[4 * kSeg]; // where the block's codes of this head begin, in 512 bytes (a block has a multiple of them)
     float ks[4 * kSeg], lvs[4 * kSeg]; // key scale, log2 of the value scale (kNoScale: the values count as zero)
 };
 __device__ __forceinline__ void look_up(const AttendArgs& a, const Item& it, int seg0, int endAll, int threads, Stretch& z) {
@@ -364,7 +364,7 @@ __device__ __forceinline__ void look_up(const AttendArgs& a, const Item& it, int
                 ks = __builtin_nanf("");
             }
         }
-        z.page[i] = max(p, 0);
+        z.at[i] = (unsigned)((((int64_t)max(p, 0) * a.cache.numHeads + it.h) * (bs * a.cache.headDim)) >> 9);
         z.ks[i] = ks;
         z.lvs[i] = vs >= FLT_MIN && vs < INFINITY ? __builtin_amdgcn_logf(vs) : kNoScale;
     }
@@ -454,9 +454,9 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
     u32x4 kr[4][NL];
     u32x2 kx[4];
     u32x4 vr[MD];
-    auto fetch_k = [&](int t, int page) {
+    auto fetch_k = [&](int t, unsigned at) {
         const int off = ((t * kTile + 16 * (n16 >> 2)) & (bs - 1)) + (n16 & 3);
-        const uint8_t* p = a.cache.k + ((int64_t)page * H + it.h) * (int64_t)(bs * D) + (int64_t)off * D;
+        const uint8_t* p = a.cache.k + ((uint64_t)at << 9) + off * D;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
@@ -464,15 +464,15 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
             if constexpr (D % 64) kx[i] = *(const u32x2*)(p + i * 4 * D + 64 * NL + 8 * grp);
         }
     };
-    auto fetch_v = [&](int t, int page) { // 16 tokens of a dimension per lane
-        const uint8_t* p = a.cache.v + ((int64_t)page * H + it.h) * (int64_t)(bs * D) + (int64_t)n16 * bs + ((t * kTile + 16 * grp) & (bs - 1));
+    auto fetch_v = [&](int t, unsigned at) { // 16 tokens of a dimension per lane
+        const uint8_t* p = a.cache.v + ((uint64_t)at << 9) + n16 * bs + ((t * kTile + 16 * grp) & (bs - 1));
 #pragma unroll
-        for (int i = 0; i < MD; ++i) vr[i] = *(const u32x4*)(p + (int64_t)i * 16 * bs);
+        for (int i = 0; i < MD; ++i) vr[i] = *(const u32x4*)(p + i * 16 * bs);
     };
     // the first keys are on their way before the queries are looked at
     look_up(a, it, tile0, end, 256, z);
     __syncthreads();
-    if (tile < min(tile0 + kSeg, end)) fetch_k(tile, z.page[(tile - tile0) * 4 + (n16 >> 2)]);
+    if (tile < min(tile0 + kSeg, end)) fetch_k(tile, z.at[(tile - tile0) * 4 + (n16 >> 2)]);
     half8_t q[NT][KS];
     Rows<NT, MD> w;
     load_queries<D, NT, true>(a, it, G, row0, rowsAll, q, w);
@@ -484,11 +484,11 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
             __syncthreads(); // (the stretch before has been read)
             look_up(a, it, seg0, end, 256, z);
             __syncthreads();
-            if (tile < segEnd) fetch_k(tile, z.page[(tile - seg0) * 4 + (n16 >> 2)]);
+            if (tile < segEnd) fetch_k(tile, z.at[(tile - seg0) * 4 + (n16 >> 2)]);
         }
         for (; tile < segEnd; tile += kWaves) {
             const int t0 = tile * kTile, u = (tile - seg0) * 4;
-            fetch_v(tile, z.page[u + grp]);
+            fetch_v(tile, z.at[u + grp]);
             const float ks = z.ks[u + grp], lvs = z.lvs[u + grp];
             f32x4 sc[NT][4];
 #pragma unroll
@@ -507,7 +507,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
                     for (int t = 0; t < NT; ++t) sc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka, q[t][k], sc[t][i], 0, 0, 0);
                 }
             }
-            if (tile + kWaves < segEnd) fetch_k(tile + kWaves, z.page[u + 4 * kWaves + (n16 >> 2)]);
+            if (tile + kWaves < segEnd) fetch_k(tile + kWaves, z.at[u + 4 * kWaves + (n16 >> 2)]);
             half8_t pr[NT][2];
             unsigned nan = 0;
             if (CODE == CACHE_E4M3 && visMin < it.len && t0 + kTile > visMin) { // some rows mask tokens that others see
@@ -616,9 +616,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
     // (every wavefront loads, also where there is nothing for it: a load under a condition waits for the loads before it)
     auto fetch = [&](int t, int seg0) {
         const int u = (t - seg0) * 4;
-        const int kp = z.page[u + (n16 >> 2)], vp = z.page[u + grp];
-        const uint8_t* k = a.cache.k + ((int64_t)kp * H + it.h) * (int64_t)(bs * D) + (((t * kTile + 16 * (n16 >> 2)) & (bs - 1)) + (n16 & 3)) * D;
-        const uint8_t* v = a.cache.v + ((int64_t)vp * H + it.h) * (int64_t)(bs * D) + n16 * bs + ((t * kTile + 16 * grp) & (bs - 1));
+        const uint8_t* k = a.cache.k + ((uint64_t)z.at[u + (n16 >> 2)] << 9) + (((t * kTile + 16 * (n16 >> 2)) & (bs - 1)) + (n16 & 3)) * D;
+        const uint8_t* v = a.cache.v + ((uint64_t)z.at[u + grp] << 9) + n16 * bs + ((t * kTile + 16 * grp) & (bs - 1));
 #pragma unroll
         for (int j = 0; j < KW; ++j) {
             const int pc = min(wave + j * WAVES, KP - 1);

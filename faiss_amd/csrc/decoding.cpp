@@ -49,6 +49,8 @@ CacheView view(const FaissAmdPagedCache* c) {
                         "head dimension must be 64, 96, 128, 192 or 256");
     FA_THROW_IF_NOT_MSG(c->numHeads >= 1 && c->numHeads <= 32767, "number of heads out of range");
     FA_THROW_IF_NOT_MSG(c->numBlocks >= 1 && (int64_t)c->numBlocks * c->blockSize < ((int64_t)1 << 31), "number of blocks out of range");
+    // (the attention counts a block's place in units of 512 bytes)
+    FA_THROW_IF_NOT_MSG((double)c->numBlocks * c->numHeads * c->blockSize * c->headDim < 2e12, "cache too large");
     CacheView v;
     v.k = (uint8_t*)c->keys;
     v.v = (uint8_t*)c->values;
