@@ -421,6 +421,23 @@ def test_add_nothing_and_many(res):
     add_both(res, c, x, x.flip(0), torch.randperm(1120, generator=g)[:1000].tolist())  # no order at all
 
 
+@pytest.mark.parametrize("bs, d, n", [(16, 64, 3000), (128, 256, 1500), (64, 96, 1025)])
+def test_add_long_calls_and_odd_addresses(res, bs, d, n):
+    """calls of more than a thousand tokens, whose workgroups share the scan for a block's tokens; rows that start anywhere"""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n)
+    blocks = -(-n // bs) + 3
+    for code in ("e4m3", "int8"):
+        c = decoding.PagedCache(res, blocks, bs, 3, d, code)
+        x = torch.randn((n, 2, 3, d + 3), generator=g, device="cuda").half()
+        k, v = x[:, 0, :, 1:d + 1], x[:, 1, :, 2:d + 2]
+        o = torch.Generator()
+        o.manual_seed(bs)
+        # runs of a block's slots, and a tail in no order that comes back to their blocks
+        slots = [2 * bs + i for i in range(n - 70)] + torch.randint(0, blocks * bs, (70,), generator=o).tolist()
+        add_both(res, c, k, v, slots)
+
+
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
 def test_reconstruct(res, code):
     for bs, h, d in ((16, 3, 64), (64, 2, 96), (256, 1, 256)):
