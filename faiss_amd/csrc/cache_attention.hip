@@ -5,15 +5,19 @@
 //
 // Both products run on v_mfma_f32_16x16x32_f16: every 8-bit code is an fp16 number exactly (e4m3: 4 significant bits, 2^-9 ...
 // 448; int8: integers), fp16 queries are taken as they are, and bf16 queries are shifted by a power of two per row so that their
-// largest element lies at 2^10 -- fp16 then holds 24 binades below it exactly, what is lost is 2^-35 of the row's largest element.
-// Scores, the running maximum and sum and the accumulators are fp32.  Probabilities are rounded to fp16 (2^-12 relative) after a
-// bias of 2^14 in the exponent: they keep their full precision down to 2^-28 of the row's largest, and vanish below 2^-38.
+// largest element lies in [2^9, 2^10) -- fp16 then holds 23 binades below it exactly, what is lost is 2^-34 of the row's largest
+// element.  Scores, the running reference and sum and the accumulators are fp32.  A probability is rounded to fp16 (2^-11 relative)
+// together with its value's scale, in units in which the largest such product of the row lies between 2^6 and 2^14: it keeps its
+// precision down to 2^-20 of that, and vanishes below 2^-31.
 //
 // Layout: one wavefront computes S^T = K Q^T for 64 tokens and 16 x NT rows, and O^T += V^T P^T.  Tokens are dealt to the rows of
 // the four 16 x 16 score tiles such that lane group g (lanes 16 g ... 16 g + 15) receives exactly the scores of the 16 tokens
 // 16 g ... 16 g + 15 of the tile, in order: converted to fp16 they ARE the B operand of the second product, whose A operand
-// (V^T: dimension x token) is 16 adjacent bytes of the values' layout.  Nothing goes through LDS or across lanes but the row
-// maximum; a block of 16 tokens, the smallest, is one lane group, so a scale is one factor per lane.
+// (V^T: dimension x token) is 16 adjacent bytes of the values' layout.  Nothing goes across lanes but the row maximum; a block of
+// 16 tokens, the smallest, is one lane group, so a scale is one factor per lane.
+//
+// Two kernels feed these products: straight from memory for few rows (bound by the cache's bytes), through LDS for many (bound by
+// the arithmetic); a third joins the chunks of split contexts.
 #include "decoding.h"
 #include <algorithm>
 
@@ -205,14 +209,15 @@ template <int NT, int MD>
 struct Rows {
     float qs[NT];    // what a score is multiplied by beside the block's scale, in units of log 2; not negative
     int limit[NT];   // tokens the row sees
-    float m[NT], l[NT];
-    float vref;      // values are accumulated in units of 2^vref, the largest scale met so far
-    f32x4 o[NT][MD];
+    float top[NT];   // reference of the exponents, log2 of a probability times its value's scale
+    float l[NT];     // sum of the probabilities, in units of 2^(top - vref - kBias)
+    float vref;      // log2 of the largest value scale met so far
+    f32x4 o[NT][MD]; // sums of probability times value, in units of 2^(top - kBias)
     __device__ __forceinline__ void reset() {
-        vref = -INFINITY;
+        vref = kNoScale;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            m[t] = -INFINITY;
+            top[t] = -INFINITY;
             l[t] = 0.f;
 #pragma unroll
             for (int i = 0; i < MD; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -270,7 +275,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs& a, const Item& it
 // The scores of 64 tokens become probabilities, fp16 operands of the second product; maxima, sums and accumulators follow.
 // tok0: the lane group's first token; edge: some row does not see all 64; ks, lvs: the key scale and log2 of the value scale of the
 // lane group's block.  A value's scale goes into its probability's exponent, so the sum of the probabilities themselves is the
-// lane's sum times the inverse.  All row tiles are worked on between the same branches: they are independent chains.
+// lane's sum times the inverse of its scale.  All row tiles are worked on between the same branches: they are independent chains.
 // nan: which of the lane group's 16 tokens have a value of code NaN that was taken out (edge steps only): rows that see one are NaN.
 template <int NT, int MD>
 __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float lvs, int tok0, bool edge, unsigned nan, Rows<NT, MD>& w, half8_t (&pr)[NT][2]) {
@@ -295,10 +300,11 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
             f[t] = 1.f;
         }
     }
-    const float vnew = fmaxf(w.vref, groups_max(lvs));
-    const float vdown = __builtin_amdgcn_exp2f(w.vref - (vnew == -INFINITY ? 0.f : vnew));
+    const float vnew = fmaxf(w.vref, groups_max(lvs)), vold = w.vref;
     w.vref = vnew;
-    const float lv = lvs == kNoScale ? 0.f : lvs - vnew, iv = __builtin_amdgcn_exp2f(-lv);
+    // the exponent of the lane's value scale: where there is none the probability is needed for the sum alone, and 2^-100 of the
+    // largest is as good as less
+    const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f), iv = __builtin_amdgcn_exp2f(vnew - lv);
     float od[NT];
     bool change = false;
 #pragma unroll
@@ -306,13 +312,15 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
         float mx = fmaxf(sc[t][0][0], sc[t][0][1]);
 #pragma unroll
         for (int i = 2; i < 16; ++i) mx = fmaxf(mx, sc[t][i >> 2][i & 3]);
-        mx = groups_max(mx * f[t]);
-        mx = __builtin_fmaf(fabsf(mx), 0x1p-22f, mx); // not below the exact products of the fma below, however large they are
-        // the reference of the exponentials follows the maximum only when that has grown by more than 2^8
-        const float mn = mx > w.m[t] + kSlack ? mx : w.m[t];
-        const float top = mn == -INFINITY ? 0.f : mn;
-        const float down = __builtin_amdgcn_exp2f(w.m[t] - top);
-        w.m[t] = mn;
+        mx *= f[t];
+        // (2^-22: not below the exact products and sums of the fma below, however large they are)
+        mx = groups_max(__builtin_fmaf(fabsf(mx), 0x1p-22f, mx) + lv);
+        // the reference follows the maximum only when that has grown by more than 2^8.  It is that of probability and scale
+        // together: what a probability loses in fp16 is then small beside the row's largest term, whatever the scales
+        const float was = w.top[t], now = mx > was + kSlack ? mx : was;
+        const float top = now == -INFINITY ? 0.f : now;
+        w.top[t] = now;
+        od[t] = __builtin_amdgcn_exp2f(was - top);
         const float sub = lv - (top - kBias);
         float sum = 0.f;
 #pragma unroll
@@ -323,8 +331,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
                 sum += p;
                 pr[t][i >> 1][4 * (i & 1) + e] = (_Float16)p;
             }
-        w.l[t] = __builtin_fmaf(sum, iv, w.l[t] * down);
-        od[t] = down * vdown;
+        w.l[t] = __builtin_fmaf(sum, iv, w.l[t] * __builtin_amdgcn_exp2f((was - vold) - (top - vnew)));
         change |= od[t] != 1.f;
     }
     if (__ballot(change)) {
@@ -419,21 +426,25 @@ __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, 
                 for (int e = 0; e < 4; ++e) x[e] *= unit;
                 *(f32x4*)(s.partO + pr * D + 16 * i + 4 * grp) = x;
             }
-            if (grp == 0) s.partML[pr] = make_float2(w.m[t], w.l[t]);
+            if (grp == 0) s.partML[pr] = make_float2(w.top[t] - w.vref, w.l[t]);
         } else {
             const int qi = r / G, g = r - qi * G;
             const float inv = w.l[t] == 0.f ? 0.f : unit / w.l[t];
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + 4 * grp;
 #pragma unroll
             for (int i = 0; i < MD; ++i) store4(op + 16 * i, w.o[t][i], inv, a.type);
-            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.m[t], w.l[t]);
+            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.top[t] - w.vref, w.l[t]);
         }
     }
 }
 
 // Few rows (single tokens, drafts): bound by the bytes of the cache.  The four wavefronts of a workgroup share the rows and take every
 // fourth tile of the chunk, straight from memory into the registers that feed the matrix instructions; their results are joined in
-// LDS.
+// LDS.  A tile's values are asked for before its scores are computed and the next tile's keys before its softmax; what a wait would
+// hold up is looked up beforehand (Stretch).
+// 64 contexts of 4096 ... 16384 tokens, 8 heads of 128, e4m3: 260 us, 5.1 TB/s, as fast as a large copy; 3 of 131071, one head of 256,
+// int8: 47 us, 4.3 TB/s (one wavefront per SIMD: 357 registers); 1 of 1000: 11.7 us, a chain of dependent loads (lengths, blocks,
+// scales, keys, values).  With the block numbers loaded in the loop 295, 82 and 11.4 us.
 template <int D, int CODE, int NT>
 __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16; // steps of the first product, row tiles of the second
@@ -542,7 +553,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         if (grp == 0) {
-            sml[wave][16 * t + n16][0] = w.m[t];
+            sml[wave][16 * t + n16][0] = w.top[t] - w.vref;
             sml[wave][16 * t + n16][1] = w.l[t];
         }
 #pragma unroll
@@ -588,6 +599,9 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 // Many rows (prompts): bound by the arithmetic.  Each of the WAVES wavefronts has rows of its own; a tile's keys and values are loaded
 // and widened to fp16 once for all of them and laid into LDS fragment by fragment, in the order in which the matrix instructions'
 // lanes read them (no bank conflicts on either side).  Two such buffers: the next tile is loaded while one is worked on.
+// 2048 queries each behind 8192 tokens, four requests, 16 heads over 4 of 128, e4m3: 581 us, 830 TFLOP/s in the matrix pipe (33 % of
+// its rate; 317 other vector instructions and 32 exponentials beside 64 matrix instructions per wavefront and tile, two wavefronts
+// per SIMD).  Ragged prompts: 364 us; the same rows straight from memory, as above, 745 us.
 template <int D, int CODE, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16;

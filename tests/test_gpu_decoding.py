@@ -1,7 +1,8 @@
 """GPU tests of the decoding operators (faiss_amd/decoding.py) against plain implementations in 64 bits.
 
 Tolerances of the attention, per output element.  With A = sum_j p_j |v_j| / sum_j p_j:
-  * probabilities are rounded to fp16: at most 2^-11 of each, together 2^-11 A;
+  * probabilities (times their value's scale) are rounded to fp16: at most 2^-11 of each, together 2^-11 A, and where they are
+    below fp16's normal numbers by 2^-25 in units in which the row's largest is at least 2^6: 2^-31 max_j p_j s_j per code;
   * a score's fp32 sum over D products and its scaling are off by at most (D + 8) 2^-24 B, B = scale max_j sum_d |q_d k_jd| (and
     2 steps for the exponential), which changes numerator and denominator by that factor: 2 ((D + 8) B + 4) 2^-24 A;
   * sums over N tokens in fp32: lanes add 16 at a time, matrix steps 32, chunks are joined: less than (N / 16 + 300) 2^-24 A;
@@ -52,6 +53,7 @@ def reference(cache, q, table, lens, offs, scale, causal):
     tol = torch.zeros_like(out)
     kk = cache.k_codes.double() * cache.k_scales.double()[:, :, None, None]
     vv = (cache.v_codes.double() * cache.v_scales.double()[:, :, None, None]).transpose(2, 3)
+    vc, vs = cache.v_codes.double().abs().transpose(2, 3), cache.v_scales.double()
     for b, n in enumerate(lens):
         a, e = (offs[b], offs[b + 1]) if offs is not None else (b, b + 1)
         nq = e - a
@@ -59,6 +61,7 @@ def reference(cache, q, table, lens, offs, scale, causal):
         for h in range(hk):
             k = kk[pages, h].reshape(-1, d)[:n]
             v = vv[pages, h].reshape(-1, d)[:n]
+            codes, each = vc[pages, h].reshape(-1, d)[:n], vs[pages, h].repeat_interleave(bs)[:n]
             g = hq // hk
             x = q[a:e, h * g:(h + 1) * g].double().reshape(nq * g, d)
             z = x @ k.T * scale
@@ -69,19 +72,20 @@ def reference(cache, q, table, lens, offs, scale, causal):
             z = z.masked_fill(torch.arange(n, device=q.device)[None] >= see, -math.inf)
             empty = see <= 0
             if n == 0:
-                o, l, big = x * 0, x[:, 0] * 0 - math.inf, x * 0
+                o, l, big, low = x * 0, x[:, 0] * 0 - math.inf, x * 0, x * 0
             else:
                 m = z.amax(-1, keepdim=True)
                 p = torch.where(empty, torch.zeros_like(z), (z - m).exp())
                 s = p.sum(-1, keepdim=True)
                 o = torch.where(empty, torch.zeros_like(x), p @ v / s)
                 big = torch.where(empty, torch.zeros_like(x), p @ v.abs() / s)
+                low = torch.where(empty, torch.zeros_like(x), 2 ** -31 * (p * each).amax(-1, keepdim=True) * codes.sum(0) / s)
                 l = torch.where(empty[:, 0], torch.full_like(s[:, 0], -math.inf), m[:, 0] + s[:, 0].log())
             eps = torch.finfo(q.dtype).eps / 2
             f = 2 ** -11 + 2 * ((d + 8) * size + 4) * 2 ** -24 + (n / 16 + 300) * 2 ** -24
             out[a:e, h * g:(h + 1) * g] = o.reshape(nq, g, d)
             lse[a:e, h * g:(h + 1) * g] = l.reshape(nq, g)
-            tol[a:e, h * g:(h + 1) * g] = ((f * big) * (1 + eps) + eps * o.abs() + torch.finfo(q.dtype).smallest_normal * eps).reshape(nq, g, d)
+            tol[a:e, h * g:(h + 1) * g] = ((f * big + low) * (1 + eps) + eps * o.abs() + torch.finfo(q.dtype).smallest_normal * eps).reshape(nq, g, d)
     return out, lse, tol
 
 
@@ -168,6 +172,11 @@ def test_attend_strides_padding_and_scale(res):
     q = qkv[:, 1]
     odd = torch.randn((70, 8, 67), device="cuda").bfloat16()[:, :, 1:65]  # rows on odd addresses
     offs = [0, 40, 41, 58]
+    near = torch.full((70, 8, 67), 7.0, device="cuda").bfloat16()
+    c.attend(q, table, ints(lens), query_offsets=ints(offs), out=near[:, :, 1:65])  # out on odd addresses
+    want, _, tol = reference(c, q[:58], table, lens, offs, 1 / 8, True)
+    check(near[:58, :, 1:65], None, want, None, tol)
+    assert bool((near[58:] == 7).all()) and bool((near[:, :, 0] == 7).all()) and bool((near[:, :, 65:] == 7).all())
     for x, sc in ((q, 0.3), (odd, 0.0), (q.transpose(0, 1).contiguous().transpose(0, 1), -0.125)):
         out = torch.full((8, 70, 64), 7.0, device="cuda").bfloat16().transpose(0, 1)
         got = c.attend(x, wide[:, :table.shape[1]], ints(lens), query_offsets=ints(offs), scale=sc, out=out)
@@ -235,6 +244,33 @@ def test_attend_masked_nan_codes(res, nq, g):
             check(got[:nq - 3], None, want[:nq - 3], None, tol[:nq - 3])
             assert bool(got[nq - 3:, :, 50].isnan().all())
         raw[where] = old
+
+
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_attend_scales_far_apart(res, code, nq):
+    """blocks whose value scales lie up to 2^90 apart, and rows that see next to nothing of the large ones (probability and scale
+    share an fp32 exponent of 2^-126 ..., which is where the limit of 2^100 comes from)"""
+    lens = [160]
+    c, table = paged(res, lens, 16, 1, 64, code, 5)
+    far = [2.0 ** e for e in (-3, -45, 20, -30, 0, -40, 45, -20, -40, 5)]
+    for i, x in enumerate(far):
+        c.v_scales[int(table[0, i])] = x
+    g = torch.Generator(device="cuda")
+    g.manual_seed(nq)
+    q = (torch.randn((nq, 4, 64), generator=g, device="cuda") * 2).half()
+    for scale, lift in ((1 / 8, None), (1 / 8, 3), (1 / 8, 7), (4.0, 1)):
+        old = c.k_codes.clone()
+        if lift is not None:  # one block has nearly all the probability
+            c.k_codes.view(torch.uint8)[int(table[0, lift])] = (q[0, 0].float() * 8).round().clamp(-100, 100).to(c.k_codes.dtype).view(torch.uint8)
+        offs = ints([0, nq])
+        want, wl, tol = reference(c, q, table, lens, [0, nq], scale, False)
+        got, lse = c.attend(q, table, ints(lens), query_offsets=offs, scale=scale, causal=False, return_lse=True)
+        # (beyond the type's range both are infinite)
+        fits = want.abs() < torch.finfo(q.dtype).max * 0.999
+        assert bool(((got.double() - want).abs() <= tol)[fits].all()), (code, scale, lift)
+        assert bool((lse.double() - wl).abs().max() < 2 ** -9)
+        c.k_codes.copy_(old)
 
 
 def test_attend_zero_and_negative_scales(res):
