@@ -442,9 +442,9 @@ __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, 
 // fourth tile of the chunk, straight from memory into the registers that feed the matrix instructions; their results are joined in
 // LDS.  A tile's values are asked for before its scores are computed and the next tile's keys before its softmax; what a wait would
 // hold up is looked up beforehand (Stretch).
-// 64 contexts of 4096 ... 16384 tokens, 8 heads of 128, e4m3: 260 us, 5.1 TB/s, as fast as a large copy; 3 of 131071, one head of 256,
-// int8: 47 us, 4.3 TB/s (one wavefront per SIMD: 357 registers); 1 of 1000: 11.7 us, a chain of dependent loads (lengths, blocks,
-// scales, keys, values).  With the block numbers loaded in the loop 295, 82 and 11.4 us.
+// 64 ragged contexts of up to 16384 tokens, 8 heads of 128, e4m3 (1.34 GB): 263 us, 5.1 TB/s, as fast as a large copy; 3 of 131071,
+// one head of 256, int8 (0.2 GB): 48 us, 4.2 TB/s (358 registers: one wavefront per SIMD); 1 of 1000: 12 us, a chain of dependent
+// loads (lengths, blocks, scales, keys, values).
 template <int D, int CODE, int NT>
 __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16; // steps of the first product, row tiles of the second
@@ -599,9 +599,9 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 // Many rows (prompts): bound by the arithmetic.  Each of the WAVES wavefronts has rows of its own; a tile's keys and values are loaded
 // and widened to fp16 once for all of them and laid into LDS fragment by fragment, in the order in which the matrix instructions'
 // lanes read them (no bank conflicts on either side).  Two such buffers: the next tile is loaded while one is worked on.
-// 2048 queries each behind 8192 tokens, four requests, 16 heads over 4 of 128, e4m3: 581 us, 830 TFLOP/s in the matrix pipe (33 % of
-// its rate; 317 other vector instructions and 32 exponentials beside 64 matrix instructions per wavefront and tile, two wavefronts
-// per SIMD).  Ragged prompts: 364 us; the same rows straight from memory, as above, 745 us.
+// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 597 us, 810 TFLOP/s.  The matrix
+// pipe is busy 33 % of the time: beside 64 matrix instructions a wavefront issues 318 other vector instructions per tile (37 of them
+// transcendental), and 245 registers leave two wavefronts per SIMD.  Ragged prompts: 364 - 370 us; straight from memory, as above, 745.
 template <int D, int CODE, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16;

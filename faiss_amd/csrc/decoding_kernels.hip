@@ -26,7 +26,7 @@ __device__ __forceinline__ int lanes_before(unsigned long long mask) {
 // the granted requests that add tokens are a prefix of those that ask, and where a request's blocks and slots begin is an
 // exclusive prefix sum: one pass.  Free blocks wait in a ring: taken from its front, returned behind its end -- the two ranges
 // cannot meet (all blocks together fit the ring), so nothing has to be ordered between requests.  256 requests, a token each: 8 us
-// in one workgroup, a chain of dependent loads; 64 prompts over 384003 slots: 5.6 + 7.8 us.
+// in one workgroup, a chain of dependent loads; 64 prompts over 384003 slots: 5.6 + 7 us.
 constexpr int kPlanThreads = 1024;
 
 struct PlanScratch { // per request
@@ -387,8 +387,8 @@ __device__ __forceinline__ u32x2 encode8(u32x4 raw, int type, float inv) {
 // predecessor's the workgroup scans the call's slots for all tokens of that block: if none comes earlier it serves them (a block's
 // tokens may stand anywhere in the call; of several tokens for one slot the last wins), else another workgroup does.
 // Keys are written as 8 dimensions of a token, values as 4 tokens of 8 dimensions: 4 x 4 bytes are transposed in registers, so
-// that both layouts get words.  16389 tokens of 8 x 128, int8, blocks of 64: 44 us (100 MB, 20 us at the rate of a copy; 15 us of
-// it are the scan over the slots), element by element with a wavefront per unit 1137 us; 256 tokens of as many blocks: 9.1 us.
+// that both layouts get words.  16389 tokens of 8 x 128, int8, blocks of 64: 44 us (100 MB, 20 us at the rate of a copy), element by
+// element 1137 us; 256 tokens of as many blocks: 9.2 us.
 template <int CODE, bool VEC, int NT, int SG>
 __global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk) {
     const CacheView& c = a.cache;
@@ -550,7 +550,7 @@ __device__ __forceinline__ void store8(T* p, unsigned lo, unsigned hi, float sca
 }
 
 // a workgroup per (block, head), the keys or the values of it (blockIdx.y); the values' bytes are transposed as cache_add_kernel does.
-// Bound by memory: 308 blocks of 8 x 64 x 128 to fp16 in 19 us (5.1 TB/s)
+// Bound by memory: 262 blocks of 8 x 64 x 128, keys and values, to fp16 in 19 us (103 MB, 5.4 TB/s)
 template <int CODE, typename T>
 __global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs a) {
     const CacheView& c = a.cache;
@@ -591,8 +591,8 @@ __global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs 
 // keeps the `keep` best (logit, lowest v) of every piece of a row beside its maximum and sum of exponentials; a second launch
 // joins the pieces of a row, then the rows of a batch item.  The exponentials' sum is accumulated in 64 bits and candidates of
 // different beams are compared as 64-bit values: they come in the order of the exact values unless those agree to ~1e-8.
-// 512 rows of 128001 bf16 logits, 16 kept: 43 us (131 MB, 3.0 TB/s; bound by the vector instructions, a quarter of them exponentials)
-// and 9 us for the join; 4 rows of 32000: 7.9 + 5.1 us.
+// 512 rows of 128001 bf16 logits, 16 kept: 43 us (131 MB, 3.0 TB/s) and 9 us for the join; 4 rows of 32000:
+// 7.9 + 5.1 us.  13 vector instructions per logit keep the SIMDs busy for half of the time; neither they nor the memory are full.
 constexpr int kBeamVpt = 16;                                   // logits per lane and step
 constexpr int kBeamPend = 128;                                 // keys a wavefront collects before it cuts them to `keep`
 constexpr int kBeamCap = kBeamPend + 64 * kBeamVpt / 2;        // keys a wavefront may hold at once
