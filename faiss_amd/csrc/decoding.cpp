@@ -130,7 +130,7 @@ void cache_add(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAm
     a.cache = view(c);
     FA_THROW_IF_NOT_MSG(p, "null arguments");
     FA_THROW_IF_NOT_MSG(half_type(p->type), "add: keys and values must be float16 or bfloat16");
-    FA_THROW_IF_NOT_MSG(p->tokens >= 0, "add: negative number of tokens");
+    FA_THROW_IF_NOT_MSG(p->tokens >= 0 && p->tokens <= 1 << 30, "add: number of tokens out of range");
     const int checked = p->pointersChecked;
     DeviceScope scope(r);
     if (p->tokens == 0) return;
@@ -140,6 +140,7 @@ void cache_add(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAm
     on_device(*r, p->slots, "slots", checked);
     aligned(p->keys, 2, "keys");
     aligned(p->values, 2, "values");
+    if (p->tokens > kAddScan) on_device(*r, p->workspace, "workspace", checked);
     a.key = p->keys;
     a.value = p->values;
     a.keyTokenStride = p->keyTokenStride;
@@ -147,6 +148,7 @@ void cache_add(const GpuResources* r, const FaissAmdPagedCache* c, const FaissAm
     a.valueTokenStride = p->valueTokenStride;
     a.valueHeadStride = p->valueHeadStride;
     a.slots = p->slots;
+    a.workspace = p->workspace;
     a.tokens = p->tokens;
     a.type = p->type;
     launch_cache_add(a, stream);

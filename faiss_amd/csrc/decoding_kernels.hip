@@ -383,41 +383,72 @@ __device__ __forceinline__ u32x2 encode8(u32x4 raw, int type, float inv) {
     return u32x2{encode4<CODE>(x[0], x[1], x[2], x[3]), encode4<CODE>(x[4], x[5], x[6], x[7])};
 }
 
-// blockIdx.y: SG units, a unit being the keys or the values of a head, each with NT threads.  blockIdx.x: `chunk` tokens of the call.  Where a token's block differs from its
-// predecessor's the workgroup scans the call's slots for all tokens of that block: if none comes earlier it serves them (a block's
-// tokens may stand anywhere in the call; of several tokens for one slot the last wins), else another workgroup does.
+// The blocks of a call: found[0] of them, found[1 + i] (in no particular order: they are independent), and where the tokens of block
+// b begin and end, spans[2 * b] and spans[2 * b + 1].  Two launches, since the entries of the call's blocks, and only those, are set
+// (FIRST) before the tokens meet in them.
+template <bool FIRST>
+__global__ __launch_bounds__(256) void add_blocks_kernel(AddArgs a) {
+    const int j = blockIdx.x * 256 + threadIdx.x;
+    int* spans = a.workspace;
+    int* found = a.workspace + 2 * (int64_t)a.cache.numBlocks;
+    if (FIRST && j == 0) found[0] = 0;
+    if (j >= a.tokens) return;
+    const int shift = 31 - __builtin_clz(a.cache.blockSize);
+    const int mine = a.slots[j], block = mine >> shift;
+    if (mine < 0 || block >= a.cache.numBlocks) return;
+    const bool begins = j == 0 || a.slots[j - 1] >> shift != block, ends = j == a.tokens - 1 || a.slots[j + 1] >> shift != block;
+    if (FIRST) {
+        if (begins) spans[2 * block] = 0x7fffffff, spans[2 * block + 1] = -1;
+    } else {
+        if (begins && atomicMin(&spans[2 * block], j) == 0x7fffffff) found[1 + atomicAdd(found, 1)] = block;
+        if (ends) atomicMax(&spans[2 * block + 1], j);
+    }
+}
+
+// blockIdx.y: the keys or the values of a head.  A workgroup of few tokens (LISTED false) looks at token blockIdx.x: where its block
+// differs from its predecessor's it scans the call's slots for all tokens of that block: if none comes earlier it serves them (a
+// block's tokens may stand anywhere in the call; of several tokens for one slot the last wins), else another workgroup does.  Many
+// tokens would be scanned too often (131072 tokens in blocks of 64: 1078 us): for them the blocks are listed first, and a
+// workgroup takes every gridDim.x-th, and scans from its first token to its last.
 // Keys are written as 8 dimensions of a token, values as 4 tokens of 8 dimensions: 4 x 4 bytes are transposed in registers, so
-// that both layouts get words.  16389 tokens of 8 x 128, int8, blocks of 64: 44 us (100 MB, 20 us at the rate of a copy), element by
-// element 1137 us; 256 tokens of as many blocks: 9.2 us.
-template <int CODE, bool VEC, int NT, int SG>
-__global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk) {
+// that both layouts get words.  16384 tokens of 8 x 128, int8, blocks of 64: 32 us with the list (100 MB, 20 us at the rate of a
+// copy), 65536: 109 us; 256 tokens of as many blocks of 16: 8.5 us.  4096 tokens of as many blocks of 64 take 240 us: a value's code
+// is a byte in a line of its own.
+template <int CODE, bool VEC, int NT, bool LISTED>
+__global__ __launch_bounds__(NT) void cache_add_kernel(AddArgs a) {
     const CacheView& c = a.cache;
     const int bs = c.blockSize, D = c.headDim, H = c.numHeads, oct = D / 8;
     const int64_t nslots = (int64_t)c.numBlocks * bs;
-    const int lane = threadIdx.x & 63, sub = threadIdx.x / NT, tid = threadIdx.x - sub * NT;
+    const int lane = threadIdx.x & 63, tid = threadIdx.x;
     __shared__ __align__(16) int token[kMaxBlockSize];
     __shared__ int earlier;
-    __shared__ unsigned part[SG][NT / 64];
-    const int t0 = blockIdx.x * chunk, t1 = min(t0 + chunk, a.tokens);
-    // a lane per token of the chunk (every wavefront the same): does a run of one block's tokens begin here?
+    __shared__ unsigned part[NT / 64];
     const int shift = 31 - __builtin_clz(bs);
-    const int mine = t0 + lane < t1 ? a.slots[t0 + lane] : -1, prev = t0 + lane < t1 && t0 + lane > 0 ? a.slots[t0 + lane - 1] : -1;
-    u64 begins = __ballot(mine >= 0 && mine < nslots && (prev < 0 || (prev >> shift) != (mine >> shift)));
-    for (; begins; begins &= begins - 1) {
-        const int me = t0 + __ffsll((long long)begins) - 1;
-        const int block = __builtin_amdgcn_readlane(mine, me - t0) >> shift;
+    const int* found = a.workspace + 2 * (int64_t)c.numBlocks;
+    const int count = LISTED ? found[0] : a.tokens;
+    for (int n = blockIdx.x; n < count; n += gridDim.x) {
+        int block, me = n, to = a.tokens;
+        if constexpr (LISTED) {
+            block = found[1 + n];
+            me = a.workspace[2 * block];
+            to = a.workspace[2 * block + 1] + 1;
+        } else {
+            const int mine = a.slots[n];
+            block = mine >> shift;
+            if (mine < 0 || mine >= nslots || (n > 0 && a.slots[n - 1] >> shift == block)) continue;
+        }
         __syncthreads();
-        for (int i = threadIdx.x; i < bs; i += NT * SG) token[i] = -1;
+        for (int i = threadIdx.x; i < bs; i += NT) token[i] = -1;
         if (threadIdx.x == 0) earlier = 0;
         __syncthreads();
         const int first = block * bs;
-        for (int j0 = threadIdx.x; j0 < a.tokens; j0 += 8 * NT * SG) { // eight loads in flight: the scan is latency, not bytes
+        for (int j0 = (LISTED ? me : 0) + threadIdx.x; j0 < to; j0 += 8 * NT) { // eight loads in flight: the scan is latency, not bytes
             int s[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = j0 + NT * SG * e < a.tokens ? a.slots[j0 + NT * SG * e] : -1;
+            for (int e = 0; e < 8; ++e) s[e] = j0 + NT * e < to ? a.slots[j0 + NT * e] : -1;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const int j = j0 + NT * SG * e;
+                const int j = j0 + NT * e;
                 const unsigned o = (unsigned)(s[e] - first); // (-1 - first >= bs as an unsigned number)
                 if (o < (unsigned)bs) {
                     atomicMax(&token[o], j);
@@ -428,10 +459,9 @@ __global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk
         __syncthreads();
         if (earlier) continue;
         const bool fresh = token[0] >= 0;
-        const int unit = blockIdx.y * SG + sub;
-        const bool live = unit < 2 * H;
+        const int unit = blockIdx.y;
         const bool isV = unit >= H;
-        const int h = !live ? 0 : isV ? unit - H : unit;
+        const int h = isV ? unit - H : unit;
         const void* x = isV ? a.value : a.key;
         const int64_t ts = isV ? a.valueTokenStride : a.keyTokenStride, base = (int64_t)h * (isV ? a.valueHeadStride : a.keyHeadStride);
         // a thread's piece: 4 tokens x 8 dimensions; neighbours hold the next dimensions (keys), the next tokens (values)
@@ -441,23 +471,29 @@ __global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk
             q = isV ? i & (quads - 1) : (int)((i * recip) >> 16);
             o = isV ? i >> (shift - 2) : i - q * oct;
         };
-        auto load = [&](int q, int o, u32x4 (&raw)[4]) {
+        auto load = [&](int q, int o, u32x4 (&raw)[4]) { // (false: none of the four is in the call)
             const int4 t = *(const int4*)&token[4 * q];
             const int tt[4] = {t.x, t.y, t.z, t.w};
+            if (max(max(tt[0], tt[1]), max(tt[2], tt[3])) < 0) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) raw[e] = elems8<VEC>(x, base + max(tt[e], t0) * ts + 8 * o);
+                for (int e = 0; e < 4; ++e) raw[e] = u32x4{0u, 0u, 0u, 0u};
+                return false;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) raw[e] = elems8<VEC>(x, base + max(tt[e], me) * ts + 8 * o);
             if (min(min(tt[0], tt[1]), min(tt[2], tt[3])) < 0) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) raw[e] = tt[e] >= 0 ? raw[e] : u32x4{0u, 0u, 0u, 0u};
             }
+            return true;
         };
         // largest element: sixteen bits without the sign order like the numbers
         u32x4 raw[4];
         u16x2 most = {0, 0};
-        for (int i = tid; i < (live ? pieces : 0); i += NT) {
+        for (int i = tid; i < pieces; i += NT) {
             int q, o;
             piece(i, q, o);
-            load(q, o, raw);
+            if (!load(q, o, raw)) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -466,11 +502,11 @@ __global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk
         unsigned big = max(most[0], most[1]);
 #pragma unroll
         for (int o = 32; o; o >>= 1) big = max(big, (unsigned)__shfl_xor((int)big, o, 64));
-        if (lane == 0) part[sub][tid >> 6] = big;
+        if (lane == 0) part[tid >> 6] = big;
         float* sp = (isV ? c.vs : c.ks) + (int64_t)block * H + h;
         const float old = *sp;
         __syncthreads(); // (and every thread has read the old scale)
-        for (int w = 0; w < NT / 64; ++w) big = max(big, part[sub][w]);
+        for (int w = 0; w < NT / 64; ++w) big = max(big, part[w]);
         const float amax = a.type == DT_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)big) : __builtin_bit_cast(float, big << 16);
         const float before = fresh ? 0.f : old;
         float after = __builtin_nanf("");
@@ -481,7 +517,7 @@ __global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk
         const float ratio = after > 0.f ? before / after : 0.f;
         const bool rescale = fresh || (number && ratio != 1.f), clear = rescale && ratio == 0.f;
         uint8_t* codes = (isV ? c.v : c.k) + ((int64_t)block * H + h) * (int64_t)bs * D;
-        for (int i = tid; i < (live ? pieces : 0); i += NT) {
+        for (int i = tid; i < pieces; i += NT) {
             int q, o;
             piece(i, q, o);
             const int4 t = *(const int4*)&token[4 * q];
@@ -525,7 +561,7 @@ __global__ __launch_bounds__(NT * SG) void cache_add_kernel(AddArgs a, int chunk
                 }
             }
         }
-        if (live && tid == 0) *sp = after;
+        if (tid == 0) *sp = after;
     }
 }
 
@@ -1084,19 +1120,24 @@ void launch_plan_blocks(const PlanArgs& a, hipStream_t stream) {
 
 template <int CODE>
 static void launch_add(const AddArgs& a, bool vec, hipStream_t stream) {
-    // a workgroup per token while there are few (each is a block of its own in a decoding step), 16 tokens of a prompt's runs
-    const int chunk = a.tokens <= 1024 ? 1 : 32;
-    const unsigned gx = (unsigned)div_up(a.tokens, chunk), units = 2 * a.cache.numHeads;
-    // one wavefront per unit where a block is small work; the scan over many slots is shared by four units
-    const bool small = chunk == 1 && a.cache.blockSize * a.cache.headDim <= 8192;
+    const bool listed = a.tokens > kAddScan;
+    const int units = 2 * a.cache.numHeads;
+    // a workgroup per token of few; of many, four times as many workgroups of 256 threads as the chip holds, so that blocks even out
+    const dim3 grid((unsigned)(listed ? std::min(a.tokens, std::max(8192 / units, 1)) : a.tokens), units);
+    if (listed) {
+        const unsigned n = (unsigned)div_up(a.tokens, 256);
+        add_blocks_kernel<true><<<n, 256, 0, stream>>>(a);
+        add_blocks_kernel<false><<<n, 256, 0, stream>>>(a);
+    }
+    // a wavefront per workgroup where a block has a piece for each lane (64 x 128, a token: 6 us with four wavefronts, 11 with one)
+    const bool small = a.cache.blockSize * a.cache.headDim / 32 <= 64;
+    auto launch = [&](auto kernel, int nt) { kernel<<<grid, nt, 0, stream>>>(a); };
     if (!vec)
-        cache_add_kernel<CODE, false, 256, 1><<<dim3(gx, units), 256, 0, stream>>>(a, chunk);
+        listed ? launch(cache_add_kernel<CODE, false, 256, true>, 256) : launch(cache_add_kernel<CODE, false, 256, false>, 256);
     else if (small)
-        cache_add_kernel<CODE, true, 64, 1><<<dim3(gx, units), 64, 0, stream>>>(a, chunk);
-    else if (chunk == 1)
-        cache_add_kernel<CODE, true, 256, 1><<<dim3(gx, units), 256, 0, stream>>>(a, chunk);
+        listed ? launch(cache_add_kernel<CODE, true, 64, true>, 64) : launch(cache_add_kernel<CODE, true, 64, false>, 64);
     else
-        cache_add_kernel<CODE, true, 256, 4><<<dim3(gx, (unsigned)div_up(units, 4)), 1024, 0, stream>>>(a, chunk);
+        listed ? launch(cache_add_kernel<CODE, true, 256, true>, 256) : launch(cache_add_kernel<CODE, true, 256, false>, 256);
 }
 void launch_cache_add(const AddArgs& a, hipStream_t stream) {
     if (a.tokens == 0) return;

@@ -42,7 +42,8 @@ class _PlanStruct(ctypes.Structure):
 
 class _AddStruct(ctypes.Structure):
     _fields_ = [("keys", _P), ("values", _P), ("keyTokenStride", _I64), ("keyHeadStride", _I64), ("valueTokenStride", _I64),
-                ("valueHeadStride", _I64), ("slots", _P), ("tokens", _I), ("type", _I), ("pointersChecked", _I)]
+                ("valueHeadStride", _I64), ("slots", _P), ("tokens", _I), ("type", _I), ("pointersChecked", _I),
+                ("workspace", _P)]
 
 
 class _AttendStruct(ctypes.Structure):
@@ -230,7 +231,10 @@ class PagedCache:
         _same_length(v, n, "v")
         _same_length(_tensor(res, slots, "slots", torch.int32, 1), n, "slots")
         a = _AddStruct(k.data_ptr() or None, v.data_ptr() or None, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                       slots.data_ptr() or None, n, _HALF[k.dtype], 1)
+                       slots.data_ptr() or None, n, _HALF[k.dtype], 1, None)
+        if n > 512:  # (its blocks are listed)
+            ws = torch.empty(3 * self.num_blocks + 1, dtype=torch.int32, device=k.device)
+            a.workspace = ws.data_ptr()
         _check(self._lib.faiss_amd_PagedCache_add(res._h, self._ref, _byref(a), _stream(res)))
 
     def reconstruct(self, blocks, dtype=torch.float32):

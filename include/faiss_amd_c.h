@@ -524,12 +524,13 @@ int faiss_amd_plan_blocks(FaissAmdGpuResources* res, const FaissAmdPlanBlocksPar
  * (block, head)'s scale is the smallest power of two with which its elements stay within 448 (e4m3) or 127 (int8) and never
  * shrinks; when it grows, the block's other codes are re-expressed.  A token at offset 0 begins its block anew: the old scale
  * is forgotten and every offset that the call does not write becomes zero.  An element that is no finite number makes its
- * block's scale for that head NaN until the block is begun anew. */
+ * block's scale for that head NaN until the block is begun anew.  workspace: 3 * numBlocks + 1 ints for more than 512 tokens. */
 typedef struct FaissAmdCacheAddParams {
     const void *keys, *values;
     int64_t keyTokenStride, keyHeadStride, valueTokenStride, valueHeadStride;
     const int* slots;
     int tokens, type, pointersChecked;
+    int* workspace;
 } FaissAmdCacheAddParams;
 int faiss_amd_PagedCache_add(FaissAmdGpuResources* res, const FaissAmdPagedCache* cache, const FaissAmdCacheAddParams* args, void* stream);
 

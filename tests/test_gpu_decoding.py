@@ -474,6 +474,51 @@ def test_add_long_calls_and_odd_addresses(res, bs, d, n):
         add_both(res, c, k, v, slots)
 
 
+@pytest.mark.parametrize("bs, h, d", [(16, 2, 64), (64, 1, 128), (256, 2, 96)])
+@pytest.mark.parametrize("n", [512, 513, 2500])
+def test_add_listed_blocks(res, bs, h, d, n):
+    """around the number of tokens from which a call's blocks are listed: requests that take turns, skipped slots, the same slot
+    again at the call's other end, a second call that comes back to the blocks"""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n + bs)
+    blocks = -(-n // bs) + 4
+    c = decoding.PagedCache(res, blocks, bs, h, d, "e4m3")
+    k, v = (torch.randn((n, h, d), generator=g, device="cuda").bfloat16() for _ in range(2))
+    half = n // 2
+    slots = [(i // 2 if i % 2 else half + i // 2) for i in range(n)]
+    slots[5], slots[n // 3], slots[n - 2], slots[n - 1] = -1, blocks * bs, 2**31 - 1, slots[0]
+    add_both(res, c, k, v, slots)
+    o = torch.Generator()
+    o.manual_seed(n)
+    again = torch.randperm(blocks * bs, generator=o)[:n].tolist()
+    add_both(res, c, 2 * v, k, again + again[:max(0, n - len(again))])
+
+
+@pytest.mark.parametrize("n", [300, 1000])
+def test_add_captured(res, n):
+    c = decoding.PagedCache(res, 80, 16, 2, 64, "int8")
+    want = decoding.PagedCache(res, 80, 16, 2, 64, "int8")
+    slots = ints(list(range(40, 40 + n)))
+    k, v = torch.zeros((n, 2, 64), device="cuda").half(), torch.zeros((n, 2, 64), device="cuda").half()
+    c.add(k, v, slots)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.add(k, v, slots)
+    want.add(k, v, slots)
+    for i in range(4):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(i)
+        k.copy_(torch.randn((n, 2, 64), generator=g, device="cuda") * 2**i)
+        v.copy_(torch.randn((n, 2, 64), generator=g, device="cuda") * 2**i)
+        slots.copy_(ints(torch.randperm(1280, generator=torch.Generator().manual_seed(i))[:n].tolist()))
+        graph.replay()
+        torch.cuda.synchronize()
+        want.add(k, v, slots)
+        for a, b in ((c.k_codes, want.k_codes), (c.v_codes, want.v_codes), (c.k_scales, want.k_scales), (c.v_scales, want.v_scales)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
 @pytest.mark.parametrize("code", ["e4m3", "int8"])
 def test_reconstruct(res, code):
     for bs, h, d in ((16, 3, 64), (64, 2, 96), (256, 1, 256)):
@@ -876,3 +921,11 @@ def test_refusals_on_the_device(res):
     assert b"device memory" in lib.faiss_amd_get_last_error() or b"resources' device" in lib.faiss_amd_get_last_error()
     a = decoding._BeamStruct(q.data_ptr(), 8, 8, t.data_ptr(), None, q.data_ptr(), q.data_ptr(), q.data_ptr(), 8, 1, 1, 1, 0, 2, 0, q.data_ptr(), 1)
     assert lib.faiss_amd_beam_select(res._h, ctypes.byref(a), None) == -2 and b"workspace" in lib.faiss_amd_get_last_error()
+
+
+def test_add_without_workspace_is_refused(res):
+    c = decoding.PagedCache(res, 40, 16, 1, 64)
+    x, slots = torch.zeros((513, 1, 64), device="cuda").half(), ints(list(range(513)))
+    a = decoding._AddStruct(x.data_ptr(), x.data_ptr(), 64, 64, 64, 64, slots.data_ptr(), 513, decoding._HALF[torch.float16], 0, None)
+    with pytest.raises(RuntimeError, match="workspace must be provided"):
+        decoding._check(c._lib.faiss_amd_PagedCache_add(res._h, c._ref, decoding._byref(a), None))
