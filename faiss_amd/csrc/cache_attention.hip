@@ -88,6 +88,9 @@ __device__ __forceinline__ float groups_max(float x) {
     auto b = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
     return fmaxf(__builtin_bit_cast(float, (unsigned)b[0]), __builtin_bit_cast(float, (unsigned)b[1]));
 }
+// the larger, NaN if either is: one instruction, where fmaxf first quiets the operands that come from a matrix instruction (a row of
+// which a score is NaN becomes NaN whatever its reference)
+__device__ __forceinline__ float highest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ __forceinline__ float groups_sum(float x) {
     auto a = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, x), __builtin_bit_cast(unsigned, x), false, false);
     x = __builtin_bit_cast(float, (unsigned)a[0]) + __builtin_bit_cast(float, (unsigned)a[1]);
@@ -309,12 +312,12 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
     bool change = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        float mx = fmaxf(sc[t][0][0], sc[t][0][1]);
+        float mx = highest(sc[t][0][0], sc[t][0][1]);
 #pragma unroll
-        for (int i = 2; i < 16; ++i) mx = fmaxf(mx, sc[t][i >> 2][i & 3]);
+        for (int i = 2; i < 16; ++i) mx = highest(mx, sc[t][i >> 2][i & 3]);
         mx *= f[t];
         // (2^-22: not below the exact products and sums of the fma below, however large they are)
-        mx = groups_max(__builtin_fmaf(fabsf(mx), 0x1p-22f, mx) + lv);
+        mx = groups_max(__builtin_fmaf(fabsf(mx), 0x1p-22f, mx) + lv); // (NaN where a group's scores are all masked: passed over)
         // the reference follows the maximum only when that has grown by more than 2^8.  It is that of probability and scale
         // together: what a probability loses in fp16 is then small beside the row's largest term, whatever the scales
         const float was = w.top[t], now = mx > was + kSlack ? mx : was;
@@ -599,9 +602,10 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 // Many rows (prompts): bound by the arithmetic.  Each of the WAVES wavefronts has rows of its own; a tile's keys and values are loaded
 // and widened to fp16 once for all of them and laid into LDS fragment by fragment, in the order in which the matrix instructions'
 // lanes read them (no bank conflicts on either side).  Two such buffers: the next tile is loaded while one is worked on.
-// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 597 us, 810 TFLOP/s.  The matrix
-// pipe is busy 33 % of the time: beside 64 matrix instructions a wavefront issues 318 other vector instructions per tile (37 of them
-// transcendental), and 245 registers leave two wavefronts per SIMD.  Ragged prompts: 364 - 370 us; straight from memory, as above, 745.
+// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 574 us, 840 TFLOP/s.  The matrix
+// pipe is busy 35 % of the time: beside 64 matrix instructions a wavefront issues 277 other vector instructions per tile (37 of them
+// transcendental), and 246 registers leave two wavefronts per SIMD.  Half of the wavefronts half a tile behind the others: 620 us;
+// the next tile's products between the softmax's instructions: it spills.  Ragged prompts: the call 365 us; the kernel straight from memory, as above, 745.
 template <int D, int CODE, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16;
@@ -655,7 +659,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
         for (int j = 0; j < VW; ++j) {
             const int i = wave + j * WAVES;
             if (i < MD) {
-                u32x4 c = tail ? cut_tokens(vr[j], valid) : vr[j];
+                u32x4 c = vr[j];
+                if (tail) { // (a branch: as a selection it costs 39 instructions in every tile)
+                    asm volatile("");
+                    c = cut_tokens(c, valid);
+                }
                 if (CODE == CACHE_E4M3 && visMinAll < it.len && (t + 1) * kTile > visMinAll) { // some rows mask tokens that others see
                     const unsigned nan = take_nan<CODE>(c);
                     if (nan) atomicOr(&nanL[t % 3][grp], nan);
