@@ -32,8 +32,8 @@ __device__ __forceinline__ int wgs_lane() {
 // enough for a no-return flat_atomic_add that lands in LDS: under the right timing the wavefront that scans the 256 bins reads
 // them before every increment has been performed, picks a later bucket, returns a key ABOVE the k-th smallest, and the
 // compaction keeps more than k keys -- a partial result of n > k keys then overruns its slot of part_keys and the merge launch
-// faults (tools/wgs_fault_repro.sh reproduces it: 100 % with the out-of-line build whose zeroing is written as a loop, 0 % with an
-// extra `s_waitcnt vmcnt(0)` in front of the barriers, 0 % inlined).  Inlined, the pointers keep their LDS address space and the
+// faults (it did in every run of the out-of-line build whose zeroing is written as a loop, in none with an extra
+// `s_waitcnt vmcnt(0)` in front of the barriers, in none inlined).  Inlined, the pointers keep their LDS address space and the
 // accesses are DS instructions, which lgkmcnt does cover.  tests/test_isa_lint_cpu.py asserts that no kernel file contains a
 // call or a FLAT access at all where LDS is meant.
 #ifdef FAISS_AMD_WGS_OUTOFLINE_REPRO

@@ -256,7 +256,8 @@ class PagedCache:
         block_table [batch, columns], lengths [batch] (int32): each request's blocks and tokens, its new ones included; request
         b's queries are the rows query_offsets[b] ... query_offsets[b + 1] - 1 (int32 [batch + 1]; None: row b) and stand at
         its end.  scale: 1 / sqrt(head_dim) by default.  max_queries: an upper bound of a request's queries, which saves
-        work that only longer ones need.  Rows of no request are left as they are in `out` (zero if it is None)."""
+        work that only longer ones need.  Rows of no request are left as they are in `out` (zero if it is None);
+        out may be q."""
         res = self.res
         _tensor(res, q, "q", None, 3, dense=False)
         if q.dtype not in _HALF:

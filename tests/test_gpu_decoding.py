@@ -207,6 +207,18 @@ def test_attend_sees_nothing_behind_the_last_token(res):
         assert torch.equal(c.attend(q, table, ints(lens)), want)
 
 
+@pytest.mark.parametrize("lens, nq", [([5000, 3, 700], None), ([700, 40, 3000], [300, 1, 17])])
+def test_attend_in_place(res, lens, nq):
+    """the results may take the queries' place: a workgroup reads no rows but its own"""
+    c, table = paged(res, lens, 32, 2, 64, "int8", 9)
+    offs = None if nq is None else [0, nq[0], nq[0] + nq[1], sum(nq)]
+    q = torch.randn((len(lens) if nq is None else sum(nq), 8, 64), device="cuda").half()
+    offsets = None if offs is None else ints(offs)
+    want = c.attend(q, table, ints(lens), query_offsets=offsets)
+    got = c.attend(q, table, ints(lens), query_offsets=offsets, out=q)
+    assert got is q and torch.equal(got, want)
+
+
 def test_attend_masked_scales(res):
     """a block whose scales are no numbers touches the rows that see it, and no others"""
     lens = [40]
