@@ -605,7 +605,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 // Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 574 us, 840 TFLOP/s.  The matrix
 // pipe is busy 35 % of the time: beside 64 matrix instructions a wavefront issues 277 other vector instructions per tile (37 of them
 // transcendental), and 246 registers leave two wavefronts per SIMD.  Half of the wavefronts half a tile behind the others: 620 us;
-// the next tile's products between the softmax's instructions: it spills.  Ragged prompts: the call 365 us; the kernel straight from memory, as above, 745.
+// the next tile's products between the softmax's instructions: it spills.  Ragged prompts: 354 us, straight from memory, as above, 745.
 template <int D, int CODE, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16;
