@@ -279,7 +279,7 @@ __device__ __forceinline__ void load_queries(const AttendArgs& a, const Item& it
 // tok0: the lane group's first token; edge: some row does not see all 64; ks, lvs: the key scale and log2 of the value scale of the
 // lane group's block.  A value's scale goes into its probability's exponent, so the sum of the probabilities themselves is the
 // lane's sum times the inverse of its scale.  All row tiles are worked on between the same branches: they are independent chains.
-// nan: which of the lane group's 16 tokens have a value of code NaN that was taken out (edge steps only): rows that see one are NaN.
+// nan: which of the lane group's 16 tokens have a value of code NaN that was taken out (with edge only): rows that see one are NaN.
 template <int NT, int MD>
 __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float lvs, int tok0, bool edge, unsigned nan, Rows<NT, MD>& w, half8_t (&pr)[NT][2]) {
     float f[NT];
@@ -720,7 +720,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
                     __builtin_amdgcn_sched_group_barrier(0x8, 4 * NT, 0);
                 }
                 half8_t pr[NT][2];
-                softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, CODE == CACHE_E4M3 ? nanL[tile % 3][grp] : 0u, w, pr);
+                // (lay took the codes out wherever some row of the workgroup masks part of the tile: the wavefronts that see all of
+                // it get them back too)
+                unsigned nan = 0;
+                if (CODE == CACHE_E4M3 && visMinAll < it.len && t0 + kTile > visMinAll) nan = nanL[tile % 3][grp];
+                softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin || __ballot(nan != 0), nan, w, pr);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) fr[0][j] = vf[buf][j][lane];
                 __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
