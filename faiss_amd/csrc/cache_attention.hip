@@ -35,6 +35,7 @@ constexpr int kTile = 64;        // tokens per step of a wavefront
 constexpr float kNoScale = -1000.f;
 constexpr int kSeg = 64;         // tiles whose blocks and scales are held in LDS
 constexpr float kBias = 6.f, kSlack = 8.f; // see above; both in units of log 2
+constexpr float kRoom = 40.f;    // what the sums of probabilities are kept below their reference, see softmax_step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // what a launch works on, beside AttendArgs
@@ -49,8 +50,8 @@ struct Sched {
     int merge;        // 0: no request is split
     int sort;         // of 64 requests, the longest first
     int mergeRows;    // workgroups that join a row tile's rows
-    float* partO;     // [maxSlots][rows][dim]
-    float2* partML;   // [maxSlots][rows]
+    float* partO;     // [maxSlots][rows][dim]: results of chunks
+    float2* partML;   // [maxSlots][rows]: references and sums of their probabilities
 };
 
 struct Item {
@@ -198,11 +199,11 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
 }
 
 // four adjacent elements of a result (any alignment)
-__device__ __forceinline__ void store4(unsigned short* p, f32x4 x, float f, int type) {
+__device__ __forceinline__ void store4(unsigned short* p, f32x4 x, int type) {
     unsigned short r[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-        r[e] = type == DT_F16 ? __builtin_bit_cast(unsigned short, (_Float16)(x[e] * f)) : __builtin_bit_cast(unsigned short, (__bf16)(x[e] * f));
+        r[e] = type == DT_F16 ? __builtin_bit_cast(unsigned short, (_Float16)x[e]) : __builtin_bit_cast(unsigned short, (__bf16)x[e]);
     __builtin_memcpy(p, r, 8);
 }
 
@@ -213,14 +214,15 @@ struct Rows {
     float qs[NT];    // what a score is multiplied by beside the block's scale, in units of log 2; not negative
     int limit[NT];   // tokens the row sees
     float top[NT];   // reference of the exponents, log2 of a probability times its value's scale
-    float l[NT];     // sum of the probabilities, in units of 2^(top - vref - kBias)
+    float lref[NT];  // reference of the sum of the probabilities: never more than the largest score met so far
+    float l[NT];     // sum of the probabilities, in units of 2^(lref - kBias + kRoom)
     float vref;      // log2 of the largest value scale met so far
     f32x4 o[NT][MD]; // sums of probability times value, in units of 2^(top - kBias)
     __device__ __forceinline__ void reset() {
         vref = kNoScale;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            top[t] = -INFINITY;
+            top[t] = lref[t] = -INFINITY;
             l[t] = 0.f;
 #pragma unroll
             for (int i = 0; i < MD; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -278,7 +280,10 @@ __device__ __forceinline__ void load_queries(const AttendArgs& a, const Item& it
 // The scores of 64 tokens become probabilities, fp16 operands of the second product; maxima, sums and accumulators follow.
 // tok0: the lane group's first token; edge: some row does not see all 64; ks, lvs: the key scale and log2 of the value scale of the
 // lane group's block.  A value's scale goes into its probability's exponent, so the sum of the probabilities themselves is the
-// lane's sum times the inverse of its scale.  All row tiles are worked on between the same branches: they are independent chains.
+// lane's sum times the inverse of its scale.  That sum has a reference of its own, the largest top - vref so far: a larger scale
+// that comes later takes the row's reference along, and the scores' largest may then lie any distance above top - vref.  No score
+// is more than 100 above it (a scale counts as no less than 2^-100 of vref) and the largest is not below it: a step adds no more
+// than 2^(14 + 100 - kRoom) per token, and the sum is no less than 2^(kBias - kRoom).  All row tiles are worked on between the same branches: they are independent chains.
 // nan: which of the lane group's 16 tokens have a value of code NaN that was taken out (with edge only): rows that see one are NaN.
 template <int NT, int MD>
 __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float lvs, int tok0, bool edge, unsigned nan, Rows<NT, MD>& w, half8_t (&pr)[NT][2]) {
@@ -303,11 +308,11 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
             f[t] = 1.f;
         }
     }
-    const float vnew = fmaxf(w.vref, groups_max(lvs)), vold = w.vref;
+    const float vnew = fmaxf(w.vref, groups_max(lvs));
     w.vref = vnew;
     // the exponent of the lane's value scale: where there is none the probability is needed for the sum alone, and 2^-100 of the
     // largest is as good as less
-    const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f), iv = __builtin_amdgcn_exp2f(vnew - lv);
+    const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f);
     float od[NT];
     bool change = false;
 #pragma unroll
@@ -334,7 +339,9 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
                 sum += p;
                 pr[t][i >> 1][4 * (i & 1) + e] = (_Float16)p;
             }
-        w.l[t] = __builtin_fmaf(sum, iv, w.l[t] * __builtin_amdgcn_exp2f((was - vold) - (top - vnew)));
+        const float ref = fmaxf(w.lref[t], now - vnew), base = now == -INFINITY ? 2000.f : ref; // (nothing seen: sum is 0, or NaN)
+        w.l[t] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f((top - base) - (lv + kRoom)), w.l[t] * __builtin_amdgcn_exp2f(w.lref[t] - base));
+        w.lref[t] = ref;
         change |= od[t] != 1.f;
     }
     if (__ballot(change)) {
@@ -408,35 +415,52 @@ __device__ __forceinline__ unsigned take_nan(u32x4& w) {
     }
     return m;
 }
-__device__ __forceinline__ float log_sum(float m, float l) {
-    return l == 0.f ? -INFINITY : (m - kBias + __builtin_amdgcn_logf(l)) * kLn2;
+__device__ __forceinline__ float log_sum(float ref, float l) {
+    const float up = l < 1.f ? kRoom - kBias : 0.f; // (the two would cancel)
+    return l == 0.f ? -INFINITY : (ref + (kRoom - kBias - up) + __builtin_amdgcn_logf(__builtin_ldexpf(l, (int)up))) * kLn2;
+}
+// What a row's accumulators are multiplied by to become its result, as a factor and a power of two: the scales of the values go up
+// to the largest fp32 numbers and the sums beyond them, the results do not
+struct Norm {
+    float f;
+    int e;
+    __device__ __forceinline__ Norm(float top, float lref, float l) {
+        const float x = top - lref - kRoom, whole = floorf(x);
+        f = l == 0.f ? 0.f : __builtin_amdgcn_exp2f(x - whole) / l;
+        e = l == 0.f ? 0 : (int)whole;
+    }
+    __device__ __forceinline__ f32x4 operator()(f32x4 x) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = __builtin_ldexpf(x[i] * f, e);
+        return x;
+    }
+};
+// Partial results (of a wavefront, of a chunk) are results of their own tokens, with the reference and the sum of their
+// probabilities: they are joined with weights that add up to one.  Where a part saw nothing its reference is -inf, its sum and
+// result are zero.
+__device__ __forceinline__ float weight(float ref, float l, float largest) {
+    return l * __builtin_amdgcn_exp2f(ref - (largest == -INFINITY ? 0.f : largest));
 }
 // a row of a wavefront's own: the result, or a chunk's partial sums
 template <int D, int NT, int MD>
 __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, const Item& it, int G, int row0, int rowsAll, Rows<NT, MD>& w) {
     const int lane = threadIdx.x & 63, n16 = lane & 15, grp = lane >> 4;
-    const float unit = __builtin_amdgcn_exp2f(w.vref);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int r = row0 + 16 * t + n16;
         if (r >= rowsAll) continue;
+        const Norm norm(w.top[t], w.lref[t], w.l[t]);
         if (it.slot >= 0) {
             const int64_t pr = (int64_t)(it.slot + it.c) * s.rows + (r - it.rt * s.rows);
 #pragma unroll
-            for (int i = 0; i < MD; ++i) {
-                f32x4 x = w.o[t][i];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[e] *= unit;
-                *(f32x4*)(s.partO + pr * D + 16 * i + 4 * grp) = x;
-            }
-            if (grp == 0) s.partML[pr] = make_float2(w.top[t] - w.vref, w.l[t]);
+            for (int i = 0; i < MD; ++i) *(f32x4*)(s.partO + pr * D + 16 * i + 4 * grp) = norm(w.o[t][i]);
+            if (grp == 0) s.partML[pr] = make_float2(w.lref[t], w.l[t]);
         } else {
             const int qi = r / G, g = r - qi * G;
-            const float inv = w.l[t] == 0.f ? 0.f : unit / w.l[t];
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + 4 * grp;
 #pragma unroll
-            for (int i = 0; i < MD; ++i) store4(op + 16 * i, w.o[t][i], inv, a.type);
-            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.top[t] - w.vref, w.l[t]);
+            for (int i = 0; i < MD; ++i) store4(op + 16 * i, norm(w.o[t][i]), a.type);
+            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.lref[t], w.l[t]);
         }
     }
 }
@@ -552,20 +576,15 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
     constexpr int PITCH = D + 4;
     __shared__ __align__(16) float sm[kWaves][16 * NT][PITCH];
     __shared__ float sml[kWaves][16 * NT][2];
-    const float unit = __builtin_amdgcn_exp2f(w.vref);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         if (grp == 0) {
-            sml[wave][16 * t + n16][0] = w.top[t] - w.vref;
+            sml[wave][16 * t + n16][0] = w.lref[t];
             sml[wave][16 * t + n16][1] = w.l[t];
         }
+        const Norm norm(w.top[t], w.lref[t], w.l[t]);
 #pragma unroll
-        for (int i = 0; i < MD; ++i) {
-            f32x4 x = w.o[t][i];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] *= unit;
-            *(f32x4*)&sm[wave][16 * t + n16][16 * i + 4 * grp] = x;
-        }
+        for (int i = 0; i < MD; ++i) *(f32x4*)&sm[wave][16 * t + n16][16 * i + 4 * grp] = norm(w.o[t][i]);
     }
     __syncthreads();
     // a thread joins 4 dimensions of a row
@@ -575,13 +594,14 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
         float M = -INFINITY;
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) M = fmaxf(M, sml[v][r][0]);
-        float L = 0.f;
+        float L = 0.f, wt[kWaves];
+#pragma unroll
+        for (int v = 0; v < kWaves; ++v) L += wt[v] = weight(sml[v][r][0], sml[v][r][1], M);
+        const float inv = L == 0.f ? 0.f : 1.f / L;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) {
-            const float mw = sml[v][r][0];
-            const float f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - M);
-            L += f * sml[v][r][1];
+            const float f = wt[v] * inv;
             const f32x4 ow = *(const f32x4*)&sm[v][r][d];
 #pragma unroll
             for (int e = 0; e < 4; ++e) O[e] = __builtin_fmaf(f, ow[e], O[e]);
@@ -593,7 +613,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
         } else {
             const int qi = (row0 + r) / G, g = (row0 + r) - qi * G;
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
-            store4(op, O, L == 0.f ? 0.f : 1.f / L, a.type);
+            store4(op, O, a.type);
             if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
         }
     }
@@ -780,87 +800,94 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
             float M = -INFINITY, L = 0.f;
 #pragma unroll
             for (int c = 0; c < 8; ++c) M = c < it.n ? fmaxf(M, x[c].x) : M;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) L += x[c].y = c < it.n ? weight(x[c].x, x[c].y, M) : 0.f;
+            const float inv = L == 0.f ? 0.f : 1.f / L;
             f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const float f = c >= it.n ? 0.f : x[c].x == -INFINITY ? (x[c].y == x[c].y ? 0.f : x[c].y) : __builtin_amdgcn_exp2f(x[c].x - M);
-                L += f == 0.f ? 0.f : f * x[c].y;
+            for (int c = 0; c < 8; ++c)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) O[j] = f == 0.f ? O[j] : __builtin_fmaf(f, v[c][j], O[j]);
-            }
+                for (int j = 0; j < 4; ++j) O[j] = __builtin_fmaf(x[c].y * inv, v[c][j], O[j]);
             const int qi = row / G, g = row - qi * G;
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
-            store4(op, O, L == 0.f ? 0.f : 1.f / L, a.type);
+            store4(op, O, a.type);
             if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
         }
         return;
     }
-    for (int r = blockIdx.x % s.mergeRows; r < s.rows; r += s.mergeRows) {
-    const int row = it.rt * s.rows + r;
-    if (row >= it.nq * G) return;
-    __syncthreads();
-    const float2* ml = s.partML + (int64_t)it.slot * s.rows + r;
-    const float* po = s.partO + ((int64_t)it.slot * s.rows + r) * D;
     __shared__ __align__(16) float so[256 * 4];
     __shared__ float wt[kMergeChunks];
     __shared__ float red[2][4];
-    float M = -INFINITY;
-    for (int c = threadIdx.x; c < it.n; c += 256) M = fmaxf(M, ml[(int64_t)c * s.rows].x);
+    for (int r = blockIdx.x % s.mergeRows; r < s.rows; r += s.mergeRows) {
+        const int row = it.rt * s.rows + r;
+        if (row >= it.nq * G) return;
+        __syncthreads(); // (the row before has been joined)
+        const float2* ml = s.partML + (int64_t)it.slot * s.rows + r;
+        const float* po = s.partO + ((int64_t)it.slot * s.rows + r) * D;
+        const float2 mine = ml[(int64_t)min((int)threadIdx.x, it.n - 1) * s.rows]; // (one chunk a thread is what there mostly is)
+        float M = mine.x;
+        for (int c = threadIdx.x + 256; c < it.n; c += 256) M = fmaxf(M, ml[(int64_t)c * s.rows].x);
 #pragma unroll
-    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    float L = 0.f;
-    f32x4 O = {0.f, 0.f, 0.f, 0.f};
-    for (int c0 = 0; c0 < it.n; c0 += kMergeChunks) {
-        const int n = min(it.n - c0, kMergeChunks);
+        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+        if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
         __syncthreads();
-        for (int c = threadIdx.x; c < n; c += 256) {
-            const float2 x = ml[(int64_t)(c0 + c) * s.rows];
-            // a chunk that saw nothing has weight zero and no sums; one of which every score was NaN has a NaN sum
-            const float f = x.x == -INFINITY ? (x.y == x.y ? 0.f : x.y) : __builtin_amdgcn_exp2f(x.x - M);
-            wt[c] = f;
-            L += f == 0.f ? 0.f : f * x.y;
+        M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        float L = 0.f;
+        for (int c = threadIdx.x; c < it.n; c += 256) {
+            const float2 x = c == (int)threadIdx.x ? mine : ml[(int64_t)c * s.rows];
+            const float f = weight(x.x, x.y, M);
+            if (c < kMergeChunks) wt[c] = f;
+            L += f;
         }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, 64);
+        if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
         __syncthreads();
-        if (part < parts) {
-            const float* p = po + (int64_t)c0 * s.rows * D + d;
-            int c = part;
-            for (; c + 7 * parts < n; c += 8 * parts) {
-                f32x4 v[8];
+        L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        f32x4 O = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = 0; c0 < it.n; c0 += kMergeChunks) {
+            const int n = min(it.n - c0, kMergeChunks);
+            if (c0) {
+                __syncthreads();
+                for (int c = threadIdx.x; c < n; c += 256) {
+                    const float2 x = ml[(int64_t)(c0 + c) * s.rows];
+                    wt[c] = weight(x.x, x.y, M);
+                }
+                __syncthreads();
+            }
+            if (part < parts) {
+                const float* p = po + (int64_t)c0 * s.rows * D + d;
+                int c = part;
+                for (; c + 7 * parts < n; c += 8 * parts) {
+                    f32x4 v[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] = *(const f32x4*)(p + (int64_t)(c + e * parts) * s.rows * D);
+                    for (int e = 0; e < 8; ++e) v[e] = *(const f32x4*)(p + (int64_t)(c + e * parts) * s.rows * D);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float f = wt[c + e * parts];
+                    for (int e = 0; e < 8; ++e) {
+                        const float f = wt[c + e * parts] * inv;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) O[j] = f == 0.f ? O[j] : __builtin_fmaf(f, v[e][j], O[j]);
+                        for (int j = 0; j < 4; ++j) O[j] = __builtin_fmaf(f, v[e][j], O[j]);
+                    }
+                }
+                for (; c < n; c += parts) {
+                    const f32x4 v = *(const f32x4*)(p + (int64_t)c * s.rows * D);
+                    const float f = wt[c] * inv;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) O[j] = __builtin_fmaf(f, v[j], O[j]);
                 }
             }
-            for (; c < n; c += parts) {
-                const f32x4 v = *(const f32x4*)(p + (int64_t)c * s.rows * D);
-                const float f = wt[c];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) O[j] = f == 0.f ? O[j] : __builtin_fmaf(f, v[j], O[j]);
-            }
         }
-    }
+        *(f32x4*)&so[4 * threadIdx.x] = O;
+        __syncthreads();
+        if (threadIdx.x >= quads) continue;
+        for (int p = 1; p < parts; ++p)
 #pragma unroll
-    for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, 64);
-    if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
-    *(f32x4*)&so[4 * threadIdx.x] = O;
-    __syncthreads();
-    if (threadIdx.x >= quads) continue;
-    L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-    for (int p = 1; p < parts; ++p)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) O[e] += so[4 * (p * quads + threadIdx.x) + e];
-    const int qi = row / G, g = row - qi * G;
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
-    store4(op, O, inv, a.type);
-    if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
+            for (int e = 0; e < 4; ++e) O[e] += so[4 * (p * quads + threadIdx.x) + e];
+        const int qi = row / G, g = row - qi * G;
+        unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
+        store4(op, O, a.type);
+        if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
     }
 }
 

@@ -34,3 +34,65 @@ def test_attend_nan_value_codes_anywhere(res, d, hq, length, nq, at):
         got, lse = c.attend(q, table, ints([length]), query_offsets=offs, return_lse=True)
         assert bool(got[sees][:, :, 50].isnan().all())
         check(got[~sees], lse[~sees], want[~sees], wl[~sees], tol[~sees])
+
+
+# ------------------------------------------------------------------------------------------------ scores and scales far apart
+def stepped(res, code, tiles, seed=0, extra=2, sign=False):
+    """a context of 64 tokens per entry (score in units of log 2 of a query whose first element is 1, scale of the values)"""
+    n, bs, d = 64 * len(tiles), 16, 64
+    c, table = paged(res, [n], bs, 1, d, code, seed)
+    wide = torch.full((1, table.shape[1] + extra), -1, dtype=I32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    c.k_codes.zero_()
+    c.k_scales.fill_(1.0)
+    if sign:  # values that add up
+        c.v_codes.copy_(c.v_codes.float().abs().to(c.v_codes.dtype))
+    for t, (score, scale) in enumerate(tiles):
+        pages = table[0, 4 * t:4 * t + 4].long()
+        c.k_codes[pages, 0, :, 0] = torch.tensor(float(score), device="cuda").to(c.k_codes.dtype)
+        c.v_scales[pages] = scale
+    return c, wide, n
+
+
+STEPS = {
+    # tiles of zero values with large scores, then small scores, then what nearly all of the probability goes to
+    "zero first": [(96, 0.0)] * 4 + [(-32, 0.125)] * 4 + [(120, 0.125)] * 4,
+    "zero first, small": [(96, 0.0)] * 4 + [(-32, 2.0 ** -125)] * 4 + [(120, 2.0 ** -120)] * 4,
+    "zero first, nothing more": [(96, 0.0)] * 4 + [(-120, 0.125)] * 8,
+    "zero last": [(-32, 0.125)] * 4 + [(112, 0.0)] * 8,
+    # scales that grow by far more than the scores fall
+    "small first": [(80, 2.0 ** -85)] * 4 + [(-80, 2.0 ** 90)] * 4,
+    "small first, then between": [(64, 2.0 ** -60)] * 4 + [(-64, 2.0 ** 70)] * 4 + [(0, 1.0)] * 4,
+    "growing": [(120 - 30 * (i // 4), 2.0 ** (-100 + 50 * (i // 4))) for i in range(16)],
+    "large first": [(-80, 2.0 ** 90)] * 4 + [(80, 1.0)] * 4,
+    "up and down": [(96, 2.0 ** -40)] * 4 + [(-96, 2.0 ** 40)] * 4 + [(104, 2.0 ** -40)] * 4 + [(-24, 2.0 ** 40)] * 4,
+}
+
+
+@pytest.mark.parametrize("name", list(STEPS))
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attend_scores_and_scales_far_apart(res, name, code):
+    """what a value's scale is has no say in the sum of the probabilities, in whichever order the scales come; both kernels, whole
+    and split contexts (a wider table), several requests' worth of rows"""
+    for nq in (1, 2, 40, 150):
+        for extra in (2, 90):
+            c, table, n = stepped(res, code, STEPS[name], extra=extra)
+            q = torch.randn((nq, 2, 64), device="cuda").bfloat16()
+            q[:, :, 0] = 1.0
+            q[:, 1, 0] = 0.75
+            got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
+            want, wl, tol = reference(c, q, table, [n], [0, nq], math.log(2), False)
+            check(got, lse, want, wl, tol, (name, code, nq, extra))
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attend_large_values(res, code):
+    """values near the top of the type's range: what is joined are results, which fit it"""
+    for nq in (1, 40):
+        for extra, tiles in ((2, 12), (90, 12), (2, 700)):
+            c, table, n = stepped(res, code, [(3, 2.0 ** 118)] * tiles, extra=extra, sign=True)
+            q = torch.ones((nq, 2, 64), device="cuda").bfloat16()
+            got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), return_lse=True)
+            want, wl, tol = reference(c, q, table, [n], [0, nq], math.log(2), True)
+            assert bool(torch.isfinite(got).all())
+            check(got, lse, want, wl, tol, (code, nq, extra, tiles))
