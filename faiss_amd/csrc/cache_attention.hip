@@ -415,6 +415,18 @@ __device__ __forceinline__ unsigned take_nan(u32x4& w) {
     }
     return m;
 }
+// The sums of the lane groups together.  A NaN code of a value has reached the accumulators of its dimension, or the scores where some
+// rows mask it: either way the row is NaN as a whole, its sum too, and so is what it is joined with
+template <int NT, int MD>
+__device__ __forceinline__ void close_rows(Rows<NT, MD>& w) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float m = w.o[t][0][0];
+#pragma unroll
+        for (int i = 1; i < 4 * MD; ++i) m = highest(m, w.o[t][i >> 2][i & 3]);
+        w.l[t] = groups_sum(w.l[t] + (m - m)); // (sums are finite or NaN)
+    }
+}
 __device__ __forceinline__ float log_sum(float ref, float l) {
     const float up = l < 1.f ? kRoom - kBias : 0.f; // (the two would cancel)
     return l == 0.f ? -INFINITY : (ref + (kRoom - kBias - up) + __builtin_amdgcn_logf(__builtin_ldexpf(l, (int)up))) * kLn2;
@@ -553,6 +565,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
                 for (int i = 0; i < MD; ++i) nan |= take_nan<CODE>(vr[i]);
 #pragma unroll
                 for (int o = 8; o; o >>= 1) nan |= (unsigned)__shfl_xor((int)nan, o, 64);
+                if (lvs == kNoScale) nan = 0; // (cut below: zero whatever the codes)
             }
             softmax_step(sc, ks, lvs, t0 + 16 * grp, t0 + kTile > visMin, nan, w, pr);
             if (t0 + kTile > it.len || __ballot(lvs == kNoScale)) {
@@ -570,8 +583,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
             }
         }
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) w.l[t] = groups_sum(w.l[t]);
+    close_rows(w);
 
     constexpr int PITCH = D + 4;
     __shared__ __align__(16) float sm[kWaves][16 * NT][PITCH];
@@ -769,8 +781,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
             __syncthreads();
         }
     }
-#pragma unroll
-    for (int t = 0; t < NT; ++t) w.l[t] = groups_sum(w.l[t]);
+    close_rows(w);
     write_rows<D>(a, s, it, G, row0, rowsAll, w);
 }
 

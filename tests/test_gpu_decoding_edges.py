@@ -36,6 +36,46 @@ def test_attend_nan_value_codes_anywhere(res, d, hq, length, nq, at):
         check(got[~sees], lse[~sees], want[~sees], wl[~sees], tol[~sees])
 
 
+@pytest.mark.parametrize("d, hq, length, nq", [(64, 2, 300, 1), (64, 1, 300, 200), (128, 4, 2000, 3), (192, 1, 700, 90), (96, 2, 3000, 150)])
+def test_attend_nan_codes_make_the_whole_row_nan(res, d, hq, length, nq):
+    """every dimension and the log-sum, for keys and values, whether some rows mask the code's tile or all see it"""
+    c, table = paged(res, [length], 16, 1, d, "e4m3", 3)
+    q = torch.randn((nq, hq, d), device="cuda").bfloat16()
+    want, wl, tol = reference(c, q, table, [length], [0, nq], 1 / math.sqrt(d), True)
+    for at in (0, 63, length // 2, length - nq - 1, length - nq, length - nq // 2 - 1, length - 1):
+        if at < 0:
+            continue
+        sees = torch.arange(nq) + length - nq + 1 > at
+        for codes, where in ((c.k_codes, (0, at % 16, 7)), (c.v_codes, (0, d - 1, at % 16))):
+            raw = codes.view(torch.uint8)[int(table[0, at // 16])]
+            old = int(raw[where])
+            raw[where] = 0xff
+            got, lse = c.attend(q, table, ints([length]), query_offsets=ints([0, nq]), return_lse=True)
+            raw[where] = old
+            assert bool(got[sees].isnan().all()) and bool(lse[sees].isnan().all()), (at, where)
+            check(got[~sees], lse[~sees], want[~sees], wl[~sees], tol[~sees], at)
+
+
+@pytest.mark.parametrize("nq", [1, 7, 20, 150])
+def test_attend_nan_codes_of_values_that_are_zero(res, nq):
+    """values of a zero scale are zero whatever their codes, wherever the rows' limits are"""
+    length = 200
+    c, table = paged(res, [length], 16, 1, 64, "e4m3", 3)
+    q = torch.randn((nq, 2, 64), device="cuda").bfloat16()
+    for col in (0, 5, 10, 12):
+        page = int(table[0, col])
+        old = c.v_scales[page].clone()
+        c.v_scales[page] = 0.0
+        want, wl, tol = reference(c, q, table, [length], [0, nq], 1 / 8, True)
+        raw = c.v_codes.view(torch.uint8)[page]
+        was = raw.clone()
+        raw[:, ::3] = 0x7f
+        got, lse = c.attend(q, table, ints([length]), query_offsets=ints([0, nq]), return_lse=True)
+        raw.copy_(was)
+        c.v_scales[page] = old
+        check(got, lse, want, wl, tol, col)
+
+
 # ------------------------------------------------------------------------------------------------ scores and scales far apart
 def stepped(res, code, tiles, seed=0, extra=2, sign=False):
     """a context of 64 tokens per entry (score in units of log 2 of a query whose first element is 1, scale of the values)"""
@@ -96,3 +136,14 @@ def test_attend_large_values(res, code):
             want, wl, tol = reference(c, q, table, [n], [0, nq], math.log(2), True)
             assert bool(torch.isfinite(got).all())
             check(got, lse, want, wl, tol, (code, nq, extra, tiles))
+
+
+@pytest.mark.parametrize("extra", [2, 60])
+@pytest.mark.parametrize("nq", [1, 40])
+def test_attend_nan_codes_of_no_weight(res, nq, extra):
+    """tokens whose probability is zero in fp32 are seen all the same"""
+    c, table, n = stepped(res, "e4m3", [(120, 0.1)] * 12 + [(-120, 0.1)] * 12, extra=extra)
+    c.v_codes.view(torch.uint8)[int(table[0, 20 * 4]), 0, 5, 3] = 0x7f
+    q = torch.ones((nq, 2, 64), device="cuda").bfloat16()
+    got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
+    assert bool(got.isnan().all()) and bool(lse.isnan().all())
