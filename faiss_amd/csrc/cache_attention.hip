@@ -383,7 +383,8 @@ __device__ __forceinline__ void look_up(const AttendArgs& a, const Item& it, int
         }
         z.at[i] = (unsigned)((((int64_t)max(p, 0) * a.cache.numHeads + it.h) * (bs * a.cache.headDim)) >> 9);
         z.ks[i] = ks;
-        z.lvs[i] = vs >= FLT_MIN && vs < INFINITY ? __builtin_amdgcn_logf(vs) : kNoScale;
+        const bool tiny = vs < FLT_MIN; // (the instruction takes subnormal numbers for zero)
+        z.lvs[i] = vs > 0.f && vs < INFINITY ? __builtin_amdgcn_logf(tiny ? vs * 0x1p32f : vs) - (tiny ? 32.f : 0.f) : kNoScale;
     }
 }
 

@@ -147,3 +147,20 @@ def test_attend_nan_codes_of_no_weight(res, nq, extra):
     q = torch.ones((nq, 2, 64), device="cuda").bfloat16()
     got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
     assert bool(got.isnan().all()) and bool(lse.isnan().all())
+
+
+@pytest.mark.parametrize("code", ["int8", "e4m3"])
+def test_attend_subnormal_scales(res, code):
+    """value scales below fp32's normal numbers, alone and beside larger ones; key scales too (their scores vanish)"""
+    for nq in (1, 40):
+        for extra in (2, 60):
+            for tiles in ([(3, 2.0 ** -130)] * 12, [(60, 2.0 ** -128)] * 4 + [(0, 2.0 ** -60)] * 8, [(3, 2.0 ** -149)] * 4 + [(3, 2.0 ** -127)] * 4):
+                c, table, n = stepped(res, code, tiles, extra=extra, sign=True)
+                q = torch.ones((nq, 2, 64), device="cuda").bfloat16()
+                got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
+                want, wl, tol = reference(c, q, table, [n], [0, nq], math.log(2), False)
+                check(got, lse, want, wl, tol, (code, nq, extra, tiles[0]))
+                c.k_scales[table[0, 1].long()] = 2.0 ** -135
+                got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
+                want, wl, tol = reference(c, q, table, [n], [0, nq], math.log(2), False)
+                check(got, lse, want, wl, tol, (code, nq, extra, tiles[0]))
