@@ -101,11 +101,7 @@ __device__ __forceinline__ float groups_sum(float x) {
 
 // the request's queries and tokens, clamped to what the arrays hold whatever the device arrays say
 __device__ __forceinline__ void request(const AttendArgs& a, int b, int& len, int& q0, int& nq) {
-    const long long cap = (long long)a.cols * a.cache.blockSize;
-    len = a.lengths[b];
-    len = len < 0 ? 0 : len;
-    // tokens behind the table's last column count as bad blocks: one of them is enough to make a row NaN
-    len = len > cap ? (int)cap + 1 : len;
+    len = max(a.lengths[b], 0);
     if (a.queryOffsets) {
         q0 = min(max(a.queryOffsets[b], 0), a.tokens);
         nq = min(max(a.queryOffsets[b + 1], q0), a.tokens) - q0;
@@ -116,6 +112,9 @@ __device__ __forceinline__ void request(const AttendArgs& a, int b, int& len, in
 }
 
 __device__ __forceinline__ int tiles_of(int len) { return (int)(((unsigned)len + kTile - 1) / kTile); }
+// tiles that are worked on.  Tokens behind the table's last column count as bad blocks: the first of them makes every row NaN that
+// sees any (the rows' limits go by the length as it is)
+__device__ __forceinline__ int tiles_within(const AttendArgs& a, int len) { return tiles_of(min(len, a.cols * a.cache.blockSize + 1)); }
 __device__ __forceinline__ int chunks(int lt, int tiles, int slack) {
     return (unsigned)lt > (unsigned)tiles * slack ? (lt + tiles - 1) / tiles : 1;
 }
@@ -139,7 +138,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
         if (b < a.batch) {
             int len, q0, nq;
             request(a, b, len, q0, nq);
-            const long long work = (long long)row_tiles(nq) * tiles_of(len);
+            const long long work = (long long)row_tiles(nq) * tiles_within(a, len);
             w = (int)((work + (1ll << s.wshift) - 1) >> s.wshift);
         }
         sum += __builtin_amdgcn_readlane((int)wave_incl_scan((unsigned)w), 63);
@@ -166,7 +165,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
         if (b < a.batch) {
             request(a, b, len, q0, nq);
             rts = row_tiles(nq);
-            n = chunks(tiles_of(len), tiles, s.slack);
+            n = chunks(tiles_within(a, len), tiles, s.slack);
             w = rts * n * a.cache.numHeads;
             sl = n > 1 ? w : 0;
             if (MERGE) w = n > 1 ? rts * a.cache.numHeads : 0;
@@ -183,7 +182,7 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
             it.nq = __builtin_amdgcn_readlane(nq, src);
             rts = __builtin_amdgcn_readlane(rts, src);
             const int s0 = __builtin_amdgcn_readlane(sincl - sl, src);
-            it.tiles = it.n > 1 ? (tiles_of(it.len) + it.n - 1) / it.n : tiles_of(it.len); // chunks of the same length
+            it.tiles = (tiles_within(a, it.len) + it.n - 1) / it.n; // chunks of the same length
             const int H = a.cache.numHeads, m = MERGE ? 1 : it.n;
             it.c = k % m;
             it.h = (k / m) % H;
@@ -367,7 +366,7 @@ __device__ __forceinline__ void look_up(const AttendArgs& a, const Item& it, int
         const int u = 4 * seg0 + i; // 16 tokens
         int p = -1;
         float ks = 0.f, vs = 0.f;
-        if (u < (it.len + 15) >> 4) { // there should be a block
+        if (u < (int)(((unsigned)it.len + 15) >> 4)) { // there should be a block
             const int col = (u << 4) >> shift;
             p = col < a.cols ? tb[col] : -1;
             if ((unsigned)p < (unsigned)a.cache.numBlocks) {
@@ -497,7 +496,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
     const int H = a.cache.numHeads, G = a.heads / H, bs = a.cache.blockSize;
     const int rowsAll = it.nq * G, row0 = it.rt * ROWS;
     const int vis = visible(a, it, G, min(rowsAll, row0 + ROWS) - 1), visMin = visible(a, it, G, row0); // what the last / the first row sees
-    const int tile0 = it.c * it.tiles, end = min(tile0 + it.tiles, (vis + kTile - 1) / kTile);
+    const int tile0 = it.c * it.tiles, end = min(tile0 + it.tiles, tiles_of(vis));
     int tile = tile0 + wave;
     __shared__ Stretch z;
 
@@ -654,8 +653,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(Attend
     const int lastRow = min(rowsAll, row0 + 16 * NT) - 1;
     const int vis = lastRow >= row0 ? visible(a, it, G, lastRow) : 0, visMin = lastRow >= row0 ? visible(a, it, G, row0) : 0;
     const int tile0 = it.c * it.tiles;
-    const int end = min(tile0 + it.tiles, (vis + kTile - 1) / kTile);
-    const int endAll = min(tile0 + it.tiles, (visible(a, it, G, min(rowsAll, it.rt * ROWS + ROWS) - 1) + kTile - 1) / kTile);
+    const int end = min(tile0 + it.tiles, tiles_of(vis));
+    const int endAll = min(tile0 + it.tiles, tiles_of(visible(a, it, G, min(rowsAll, it.rt * ROWS + ROWS) - 1)));
     __shared__ Stretch z;
     __shared__ __align__(16) half8_t kf[2][4 * KS][64]; // fragment (i, k): tokens 16 g + 4 i + e in row 4 g + e, dimensions 32 k ...
     __shared__ __align__(16) half8_t vf[2][MD * 2][64]; // fragment (i, h): dimensions 16 i ..., tokens 16 grp + 8 h ...

@@ -164,3 +164,46 @@ def test_attend_subnormal_scales(res, code):
                 got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
                 want, wl, tol = reference(c, q, table, [n], [0, nq], math.log(2), False)
                 check(got, lse, want, wl, tol, (code, nq, extra, tiles[0]))
+
+
+# ------------------------------------------------------------------------------------------------ lengths and batches
+@pytest.mark.parametrize("code, bs, hq, length, nq, cols", [
+    ("e4m3", 16, 2, 1000, 10, 62), ("int8", 16, 2, 1000, 300, 53), ("e4m3", 16, 1, 1000, 300, 52), ("int8", 64, 2, 5000, 200, 77),
+    ("e4m3", 64, 4, 5000, 6, 78), ("int8", 128, 1, 700, 700, 3), ("e4m3", 16, 2, 100, 90, 0), ("e4m3", 256, 2, 300, 20, 1)])
+def test_attend_lengths_past_the_table(res, code, bs, hq, length, nq, cols):
+    """rows that see tokens behind the table's last column are NaN; those that do not are what they are with a wider table"""
+    c, table = paged(res, [length, 50], bs, 1, 64, code, 3)
+    q = torch.randn((nq + 3, hq, 64), device="cuda").half()
+    offs = [0, nq, nq + 3]
+    want, wl, tol = reference(c, q, table, [length, 50], offs, 1 / 8, True)
+    narrow = table[:, :cols].contiguous()
+    got, lse = c.attend(q, narrow, ints([length, 50]), query_offsets=ints(offs), return_lse=True)
+    fine = torch.cat([length - nq + 1 + torch.arange(nq), 50 - 3 + 1 + torch.arange(3)]) <= cols * bs
+    check(got[fine], lse[fine], want[fine], wl[fine], tol[fine])
+    assert bool(got[~fine].isnan().all()) and bool(lse[~fine].isnan().all())
+    got = c.attend(q, narrow, ints([length, 50]), query_offsets=ints(offs), causal=False)
+    assert bool(got[:nq].isnan().all())
+    # the largest length there is, and the rows that mask all of what is not there
+    most = 2 ** 31 - 1
+    got, lse = c.attend(q, narrow, ints([most, 50]), query_offsets=ints(offs), return_lse=True)
+    assert bool(got[:nq].isnan().all()) and bool(lse[:nq].isnan().all())
+
+
+@pytest.mark.parametrize("queries", [None, 2, 40])
+@pytest.mark.parametrize("split", [False, True])
+def test_attend_many_requests(res, queries, split):
+    """more requests than a wavefront has lanes, three groups of 64 and a rest; short ones, and contexts that are split"""
+    n = 130 if queries != 40 else 67
+    g = torch.Generator()
+    g.manual_seed(n)
+    lens = torch.randint(0, 150, (n,), generator=g).tolist()
+    if split:
+        for i in (0, 5, 63, 64, 66, n - 1):
+            lens[i] = 2000 + 900 * (i % 4)
+    nq = None if queries is None else torch.randint(0, queries + 1, (n,), generator=g).tolist()
+    offs = None if nq is None else [0] + torch.tensor(nq).cumsum(0).tolist()
+    c, table = paged(res, lens, 16, 2, 64, "e4m3", 7)
+    q = torch.randn((n if nq is None else offs[-1], 4, 64), device="cuda").bfloat16()
+    got, lse = c.attend(q, table, ints(lens), query_offsets=None if offs is None else ints(offs), return_lse=True)
+    want, wl, tol = reference(c, q, table, lens, offs, 1 / 8, True)
+    check(got, lse, want, wl, tol)
