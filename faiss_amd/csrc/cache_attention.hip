@@ -188,7 +188,8 @@ __device__ __forceinline__ bool find_item(const AttendArgs& a, const Sched& s, i
             it.h = (k / m) % H;
             it.rt = rts - 1 - k / (m * H);
             it.slot = it.n > 1 ? s0 + (k / m) * it.n : -1;
-            if (it.slot >= 0 && it.slot + it.n > s.maxSlots) return false; // offsets that overlap: nothing to work in
+            // offsets that decrease: requests share rows, there may be nothing to work in, and the sum may have passed 2^31
+            if (it.n > 1 && (it.slot < 0 || it.slot > s.maxSlots - it.n)) return false;
             return true;
         }
         base = __builtin_amdgcn_readlane(incl, 63);

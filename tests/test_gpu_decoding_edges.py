@@ -207,3 +207,20 @@ def test_attend_many_requests(res, queries, split):
     got, lse = c.attend(q, table, ints(lens), query_offsets=None if offs is None else ints(offs), return_lse=True)
     want, wl, tol = reference(c, q, table, lens, offs, 1 / 8, True)
     check(got, lse, want, wl, tol)
+
+
+@pytest.mark.parametrize("length, most", [(300, None), (40000, None), (40000, 1)])
+def test_attend_offsets_that_decrease(res, length, most):
+    """requests that claim each other's rows, many times the work and the partial results that the call has room for: what lies
+    around the call's own memory is left alone, and rows of no request too"""
+    n, t = 70, 64
+    c, table = paged(res, [length], 16, 1, 64, "int8", 3)
+    table = table.repeat(n, 1)
+    q = torch.randn((t + 2, 2, 64), device="cuda").half()
+    out = torch.full((t + 4, 2, 64), 3.0, device="cuda").half()
+    offs = [0, t] * (n // 2) + [0]
+    c.attend(q[:t], table, ints([length] * n), query_offsets=ints(offs), max_queries=most, out=out[2:t + 2])
+    torch.cuda.synchronize()
+    assert bool((out[:2] == 3).all()) and bool((out[t + 2:] == 3).all())
+    want, _, tol = reference(c, q[:1], table[:1], [length], [0, 1], 1 / 8, True)
+    check(c.attend(q[:1], table[:1], ints([length])), None, want, None, tol)
