@@ -297,8 +297,7 @@ void reorder_beams(const GpuResources* r, int n, const FaissAmdBeamState* states
         const uintptr_t o0 = (uintptr_t)s.out, o1 = o0 + (uintptr_t)((int64_t)batch * keep * s.rowBytes);
         FA_THROW_IF_NOT_MSG(o1 <= i0 || i1 <= o0, "reorder_beams: a state's output overlaps its input");
     }
-    for (int i = 0; i < n; i += kMaxReorderStates)
-        launch_beam_reorder(st.data() + i, std::min(kMaxReorderStates, n - i), parents, batch, beams, keep, stream);
+    launch_beam_reorder(st.data(), n, parents, batch, beams, keep, stream);
 }
 
 void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* p, hipStream_t stream) {

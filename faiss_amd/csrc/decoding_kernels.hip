@@ -1006,10 +1006,15 @@ __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSc
 }
 
 // ================================================================================================ reordering by parent
+struct ReorderPiece { // `bytes` of a state's rows, from in and out on
+    const uint8_t* in;
+    uint8_t* out;
+    int64_t inBatchBytes, inBeamBytes, rowBytes, bytes;
+};
 template <int CAP>
 struct ReorderTable { // (a kernel's argument: a launch of few states carries few)
-    ReorderState st[CAP];
-    int first[CAP + 1]; // workgroups of a row before state i
+    ReorderPiece st[CAP];
+    int first[CAP + 1]; // workgroups of a row before piece i
 };
 constexpr int kReorderBytes = 16384; // of a row per workgroup
 
@@ -1019,14 +1024,14 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(ReorderTable<CAP> tab
     const int chunk = blockIdx.y;
     int lo = 0;
     while (lo + 1 < n && tab.first[lo + 1] <= chunk) ++lo;
-    const ReorderState& s = tab.st[lo];
+    const ReorderPiece& s = tab.st[lo];
     const int64_t row = blockIdx.x;
     const int b = (int)(row / keep);
     const int parent = parents[row];
-    const int64_t at = (int64_t)(chunk - tab.first[lo]) * kReorderBytes, len = min((int64_t)kReorderBytes, s.rowBytes - at);
-    uint8_t* out = (uint8_t*)s.out + row * s.rowBytes + at;
+    const int64_t at = (int64_t)(chunk - tab.first[lo]) * kReorderBytes, len = min((int64_t)kReorderBytes, s.bytes - at);
+    uint8_t* out = s.out + row * s.rowBytes + at;
     const bool none = parent < 0 || parent >= beams; // such a row becomes zero
-    const uint8_t* in = (const uint8_t*)s.in + (int64_t)b * s.inBatchBytes + (int64_t)(none ? 0 : parent) * s.inBeamBytes + at;
+    const uint8_t* in = s.in + (int64_t)b * s.inBatchBytes + (int64_t)(none ? 0 : parent) * s.inBeamBytes + at;
     // rows of any length lie anywhere: 16 bytes at a time where the output is aligned (the loads need not be), single ones around
     const int head = (int)min(len, (int64_t)((16 - ((uintptr_t)out & 15)) & 15)), mid = (int)(len - head) / 16, done = head + 16 * mid;
     u32x4 v[4];
@@ -1205,31 +1210,43 @@ void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream) {
     HIP_CHECK(hipGetLastError());
 }
 
-template <int CAP>
-static void launch_reorder(const ReorderState* states, int n, const int* parents, int64_t rows, int beams, int keep, hipStream_t stream) {
-    ReorderTable<CAP> tab;
-    int64_t first = 0;
-    for (int i = 0; i < n; ++i) {
-        tab.st[i] = states[i];
-        tab.first[i] = (int)first;
-        first += (states[i].rowBytes + kReorderBytes - 1) / kReorderBytes;
-        FA_THROW_IF_NOT_MSG(first <= 65535, "reorder: rows too long for one call");
-    }
-    tab.first[n] = (int)first;
-    beam_reorder_kernel<CAP><<<dim3((unsigned)rows, (unsigned)first), 256, 0, stream>>>(tab, n, parents, beams, keep);
-    HIP_CHECK(hipGetLastError());
-}
+// Pieces of up to 65535 chunks go into a launch (a grid has no more in y), and long rows into several
 void launch_beam_reorder(const ReorderState* states, int n, const int* parents, int batch, int beams, int keep, hipStream_t stream) {
     const int64_t rows = (int64_t)batch * keep;
-    ReorderState some[kMaxReorderStates];
-    int k = 0;
+    if (rows == 0) return;
+    constexpr int FEW = 8, ROOM = 65535;
+    ReorderTable<kMaxReorderStates> tab;
+    int k = 0, chunks = 0;
+    auto launch = [&]() {
+        if (k == 0) return;
+        tab.first[k] = chunks;
+        const dim3 grid((unsigned)rows, (unsigned)chunks);
+        if (k <= FEW) {
+            ReorderTable<FEW> few;
+            std::copy(tab.st, tab.st + k, few.st);
+            std::copy(tab.first, tab.first + k + 1, few.first);
+            beam_reorder_kernel<FEW><<<grid, 256, 0, stream>>>(few, k, parents, beams, keep);
+        } else {
+            beam_reorder_kernel<kMaxReorderStates><<<grid, 256, 0, stream>>>(tab, k, parents, beams, keep);
+        }
+        HIP_CHECK(hipGetLastError());
+        k = chunks = 0;
+    };
     for (int i = 0; i < n; ++i)
-        if (states[i].rowBytes > 0) some[k++] = states[i];
-    if (rows == 0 || k == 0) return;
-    if (k <= 8)
-        launch_reorder<8>(some, k, parents, rows, beams, keep, stream);
-    else
-        launch_reorder<kMaxReorderStates>(some, k, parents, rows, beams, keep, stream);
+        for (int64_t at = 0; at < states[i].rowBytes;) {
+            if (k == kMaxReorderStates || chunks == ROOM) launch();
+            ReorderPiece& p = tab.st[k];
+            p.in = (const uint8_t*)states[i].in + at;
+            p.out = (uint8_t*)states[i].out + at;
+            p.inBatchBytes = states[i].inBatchBytes;
+            p.inBeamBytes = states[i].inBeamBytes;
+            p.rowBytes = states[i].rowBytes;
+            p.bytes = std::min(states[i].rowBytes - at, (int64_t)(ROOM - chunks) * kReorderBytes);
+            tab.first[k++] = chunks;
+            chunks += (int)((p.bytes + kReorderBytes - 1) / kReorderBytes);
+            at += p.bytes;
+        }
+    launch();
 }
 
 void launch_fork_blocks(const ForkArgs& a, const CacheView* caches, int n, hipStream_t stream) {

@@ -224,3 +224,17 @@ def test_attend_offsets_that_decrease(res, length, most):
     assert bool((out[:2] == 3).all()) and bool((out[t + 2:] == 3).all())
     want, _, tol = reference(c, q[:1], table[:1], [length], [0, 1], 1 / 8, True)
     check(c.attend(q[:1], table[:1], ints([length])), None, want, None, tol)
+
+
+# ------------------------------------------------------------------------------------------------ long rows, other layouts
+def test_reorder_long_rows(res):
+    """rows, and states together, of more than 65535 pieces of 16384 bytes (a launch's), between short ones; more than 64 states"""
+    edge = 65535 * 16384
+    p = ints([[1, 0]])
+    for sizes in ([edge + 16384 + 7], [100, edge // 2, 5, edge // 2 + 3, 40000], [3] * 63 + [edge - 200, 16385, 9]):
+        states = [torch.randint(0, 255, (1, 2, (n + 7) // 8), device="cuda").view(torch.uint8)[:, :, :n] if n > 1000 else
+                  torch.randint(0, 255, (1, 2, n), device="cuda", dtype=torch.uint8) for n in sizes]
+        got = decoding.reorder_beams(res, states, p)
+        for x, y in zip(got, states):
+            assert torch.equal(x[0, 0], y[0, 1]) and torch.equal(x[0, 1], y[0, 0]), y.shape
+        del states, got
