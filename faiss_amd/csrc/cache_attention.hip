@@ -996,6 +996,14 @@ size_t cache_attend_workspace(const AttendArgs& a, int num_cus) {
     return bytes;
 }
 
+int64_t cache_attend_threads(const AttendArgs& a) {
+    Launch L[2];
+    const int n = plan_launches(a, 256, L); // (fewer CUs make fewer)
+    int64_t most = 0;
+    for (int i = 0; i < n; ++i) most = std::max({most, L[i].grid * (L[i].waves ? 64 * L[i].waves : 256), L[i].mergeGrid * 256});
+    return most;
+}
+
 void launch_cache_attend(const AttendArgs& a, int num_cus, hipStream_t stream) {
     Launch L[2];
     const int n = plan_launches(a, num_cus, L);
@@ -1007,7 +1015,6 @@ void launch_cache_attend(const AttendArgs& a, int num_cus, hipStream_t stream) {
             s.partML = (float2*)(ws + round_up((size_t)s.maxSlots * s.rows * a.cache.headDim * 4, 256));
             ws += L[i].bytes;
         }
-        FA_THROW_IF_NOT_MSG(L[i].grid < ((int64_t)1 << 31) && L[i].mergeGrid < ((int64_t)1 << 31), "attend: too many rows for one call");
         switch (a.cache.headDim) {
             case 64: launch_code<64>(a, L[i], stream); break;
             case 96: launch_code<96>(a, L[i], stream); break;

@@ -24,6 +24,11 @@ void aligned(const void* p, size_t n, const char* what) {
     if ((uintptr_t)p % n) FA_THROW_MSG(std::string(what) + " is not aligned to " + std::to_string(n) + " bytes");
 }
 
+// A launch holds less than 2^32 threads.  All of a call's launches are checked before the first one: it is refused as a whole
+void launchable(int64_t workgroups, int threads, const char* call) {
+    if (workgroups * threads >= (int64_t)1 << 32) FA_THROW_MSG(std::string(call) + ": too many rows for one call");
+}
+
 // the calling thread's device is the resources' one while a call checks its memory and launches its work
 struct DeviceScope {
     int before = -1;
@@ -86,6 +91,7 @@ void plan_blocks(const GpuResources* r, const FaissAmdPlanBlocksParams* p, hipSt
                         "plan_blocks: number of blocks out of range");
     FA_THROW_IF_NOT_MSG((int64_t)p->numColumns * p->blockSize < ((int64_t)1 << 31), "plan_blocks: table too wide");
     FA_THROW_IF_NOT_MSG(p->tableStride >= p->numColumns && (!p->ownedTable || p->ownedStride >= p->numColumns), "plan_blocks: rows of the table overlap");
+    launchable((int64_t)p->batch + (int64_t)div_up(p->maxTokens, kPlanSlots), 256, "plan_blocks");
     const int checked = p->pointersChecked;
     DeviceScope scope(r);
     if (p->batch > 0) {
@@ -159,6 +165,7 @@ void cache_reconstruct(const GpuResources* r, const FaissAmdPagedCache* c, int n
     a.cache = view(c);
     FA_THROW_IF_NOT_MSG(type == DT_F32 || half_type(type), "reconstruct: type must be float32, float16 or bfloat16");
     FA_THROW_IF_NOT_MSG(n >= 0, "reconstruct: negative number of blocks");
+    launchable((int64_t)n * c->numHeads, 256, "reconstruct");
     DeviceScope scope(r);
     if (n == 0) return;
     check_memory(*r, a.cache, checked);
@@ -208,6 +215,7 @@ void cache_attend(const GpuResources* r, const FaissAmdPagedCache* c, const Fais
     a.scale = p->scale;
     a.workspace = p->workspace;
     a.workspaceBytes = p->workspaceBytes;
+    launchable(cache_attend_threads(a), 1, "attend");
     const int checked = p->pointersChecked;
     DeviceScope scope(r);
     const size_t need = cache_attend_workspace(a, r->num_cus);
@@ -238,6 +246,8 @@ void beam_select(const GpuResources* r, const FaissAmdBeamSelectParams* p, hipSt
     FA_THROW_IF_NOT_MSG(p->type == DT_F32 || half_type(p->type), "beam_select: logits must be float32, float16 or bfloat16");
     FA_THROW_IF_NOT_MSG(p->batch >= 0, "beam_select: negative batch");
     FA_THROW_IF_NOT_MSG(p->beams >= 1 && p->beams <= kMaxBeams && p->keep >= 1 && p->keep <= kMaxBeams, "beam_select: beams and beams kept must be in [1, 64]");
+    launchable((int64_t)p->batch * p->beams, 256, "beam_select"); // (rows are split while there are few)
+    launchable(p->batch, kBeamJoin, "beam_select");
     FA_THROW_IF_NOT_MSG(p->vocab >= 1 && p->vocab < ((int64_t)1 << 31), "beam_select: vocabulary out of range");
     FA_THROW_IF_NOT_MSG(p->padToken >= 0 && p->padToken < p->vocab, "beam_select: padToken is no token");
     BeamArgs a;
@@ -281,6 +291,7 @@ void beam_select(const GpuResources* r, const FaissAmdBeamSelectParams* p, hipSt
 void reorder_beams(const GpuResources* r, int n, const FaissAmdBeamState* states, const int* parents, int batch, int beams, int keep, int checked, hipStream_t stream) {
     FA_THROW_IF_NOT_MSG(n >= 0 && batch >= 0 && beams >= 1 && keep >= 0, "reorder_beams: negative size");
     FA_THROW_IF_NOT_MSG((int64_t)batch * keep < ((int64_t)1 << 31) && (int64_t)batch * beams < ((int64_t)1 << 31), "reorder_beams: too many rows");
+    launchable((int64_t)batch * keep, 256, "reorder_beams");
     DeviceScope scope(r);
     if (n == 0 || batch == 0 || keep == 0) return;
     FA_THROW_IF_NOT_MSG(states, "reorder_beams: null states");
@@ -305,6 +316,7 @@ void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches,
     FA_THROW_IF_NOT_MSG(n >= 1 && caches, "fork_blocks: at least one cache");
     FA_THROW_IF_NOT_MSG(p->batch >= 0 && p->beams >= 1 && p->numColumns >= 0, "fork_blocks: negative size");
     FA_THROW_IF_NOT_MSG((int64_t)p->batch * p->beams < ((int64_t)1 << 31), "fork_blocks: too many rows");
+    launchable((int64_t)p->batch * p->beams, 256, "fork_blocks");
     FA_THROW_IF_NOT_MSG(p->tableStride >= p->numColumns, "fork_blocks: rows of the table overlap");
     std::vector<CacheView> v((size_t)n);
     for (int i = 0; i < n; ++i) {

@@ -39,6 +39,7 @@ struct PlanArgs {
     int batch = 0, cols = 0, numBlocks = 0, blockSize = 0, maxTokens = 0;
 };
 size_t plan_scratch_ints(int batch);
+constexpr int kPlanSlots = 1024; // per workgroup
 void launch_plan_blocks(const PlanArgs& a, hipStream_t stream);
 
 struct AddArgs {
@@ -80,6 +81,7 @@ struct AttendArgs {
     size_t workspaceBytes = 0;
 };
 size_t cache_attend_workspace(const AttendArgs& a, int num_cus);
+int64_t cache_attend_threads(const AttendArgs& a); // of the largest launch, on a whole chip
 void launch_cache_attend(const AttendArgs& a, int num_cus, hipStream_t stream);
 
 struct BeamArgs {
@@ -96,6 +98,7 @@ struct BeamArgs {
     size_t workspaceBytes = 0;
 };
 constexpr int kMaxBeams = 64; // beams and beams kept
+constexpr int kBeamJoin = 1024; // threads that join a batch item's rows
 size_t beam_select_workspace(const BeamArgs& a, int num_cus);
 void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream);
 

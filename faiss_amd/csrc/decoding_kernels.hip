@@ -292,7 +292,6 @@ __global__ __launch_bounds__(kPlanThreads) void plan_scan_kernel(PlanArgs a) {
     }
 }
 
-constexpr int kPlanSlots = 1024; // per workgroup
 __global__ __launch_bounds__(256) void plan_fill_kernel(PlanArgs a) {
     const PlanScratch s = plan_scratch(a.scratch, a.batch);
     if ((int)blockIdx.x < a.batch) {
@@ -888,7 +887,6 @@ __device__ __forceinline__ u64 double_flip(double x) { // larger is smaller
 }
 
 // a workgroup of 16 wavefronts per batch item
-constexpr int kBeamJoin = 1024;
 __global__ __launch_bounds__(kBeamJoin) void beam_join_kernel(BeamArgs a, BeamSched s) {
     __shared__ u64 val[kMaxBeams * kMaxBeams]; // double_flip of a candidate's value
     __shared__ unsigned tok[kMaxBeams * kMaxBeams];
@@ -1168,7 +1166,6 @@ static void launch_reconstruct(const ReconstructArgs& a, hipStream_t stream) {
 }
 void launch_cache_reconstruct(const ReconstructArgs& a, hipStream_t stream) {
     if (a.n == 0) return;
-    FA_THROW_IF_NOT_MSG((int64_t)a.n * a.cache.numHeads < ((int64_t)1 << 31), "reconstruct: too many blocks for one call");
     if (a.cache.code == CACHE_E4M3)
         launch_reconstruct<CACHE_E4M3>(a, stream);
     else
@@ -1198,7 +1195,6 @@ void launch_beam_select(const BeamArgs& a, int num_cus, hipStream_t stream) {
     size_t bytes;
     beam_sched(a, num_cus, s, bytes);
     const int64_t grid = (int64_t)a.batch * a.beams * s.parts;
-    FA_THROW_IF_NOT_MSG(grid < ((int64_t)1 << 31), "beam_select: too many rows for one call");
     if (a.type == DT_F32)
         launch_beam_scan<float>(a, s, (unsigned)grid, stream);
     else if (a.type == DT_F16)

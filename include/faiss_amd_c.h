@@ -488,7 +488,10 @@ int faiss_amd_GpuIndexIVF_list_major_rule(const FaissAmdIndex* index, int64_t n,
  *      code: 0 = int8, 1 = e4m3; blockSize: 16, 32, 64, 128, 256; headDim: 64, 96, 128, 192, 256; numBlocks * blockSize < 2^31.
  *      Types of other operands: 1 = F32, 2 = F16, 3 = BF16 (DistanceDataType).
  *      pointersChecked: 0 = every pointer is looked up (0.4 us each) and refused if it is no memory of res's device; otherwise the
- *      caller has done so, as the Python mirror has, and only null pointers are refused. */
+ *      caller has done so, as the Python mirror has, and only null pointers are refused.
+ *      A launch holds less than 2^32 threads.  Calls that would need a larger one are refused before anything is launched:
+ *      plan_blocks from batch + maxTokens / 1024 = 2^24 on, reconstruct n * numHeads = 2^24, beam_select batch * beams = 2^24 or batch =
+ *      2^22, reorder_beams batch * keep = 2^24, fork_blocks batch * beams = 2^24, attend about 2^23 pairs of a request and a key-value head. */
 typedef struct FaissAmdPagedCache {
     void *keys, *values;
     float *keyScales, *valueScales;
