@@ -317,7 +317,7 @@ void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches,
     FA_THROW_IF_NOT_MSG(p->batch >= 0 && p->beams >= 1 && p->numColumns >= 0, "fork_blocks: negative size");
     FA_THROW_IF_NOT_MSG((int64_t)p->batch * p->beams < ((int64_t)1 << 31), "fork_blocks: too many rows");
     launchable((int64_t)p->batch * p->beams, 256, "fork_blocks");
-    FA_THROW_IF_NOT_MSG(p->tableStride >= p->numColumns, "fork_blocks: rows of the table overlap");
+    FA_THROW_IF_NOT_MSG(p->tableStride >= p->numColumns && (!p->ownedTable || p->ownedStride >= p->numColumns), "fork_blocks: rows of the table overlap");
     std::vector<CacheView> v((size_t)n);
     for (int i = 0; i < n; ++i) {
         v[i] = view(&caches[i]);
@@ -331,7 +331,9 @@ void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches,
     if (p->numColumns > 0) {
         on_device(*r, p->blockTable, "blockTable", checked);
         on_device(*r, p->tableOut, "tableOut", checked);
-        FA_THROW_IF_NOT_MSG(p->tableOut != p->blockTable, "fork_blocks: outputs overlap inputs");
+        FA_THROW_IF_NOT_MSG(p->tableOut != p->blockTable && p->ownedTable != p->blockTable && (!p->ownedTable || p->ownedTable != p->tableOut),
+                            "fork_blocks: outputs overlap inputs");
+        if (p->ownedTable) on_device(*r, p->ownedTable, "ownedTable", checked);
     }
     on_device(*r, p->lengths, "lengths", checked);
     on_device(*r, p->spare, "spare", checked);
@@ -348,6 +350,8 @@ void fork_blocks(const GpuResources* r, int n, const FaissAmdPagedCache* caches,
     a.tableOut = p->tableOut;
     a.lengthsOut = p->lengthsOut;
     a.spareOut = p->spareOut;
+    a.owned = p->ownedTable;
+    a.ownedStride = p->ownedStride;
     a.batch = p->batch;
     a.beams = p->beams;
     a.cols = p->numColumns;

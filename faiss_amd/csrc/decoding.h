@@ -120,6 +120,8 @@ struct ForkArgs {
     int* tableOut = nullptr;      // [batch * beams][cols]
     int* lengthsOut = nullptr;
     int* spareOut = nullptr;
+    int* owned = nullptr; // nullable: plan_blocks' second table, kept in step
+    int64_t ownedStride = 0;
     int batch = 0, beams = 0, cols = 0;
 };
 constexpr int kMaxForkCaches = 32; // per launch

@@ -1067,7 +1067,16 @@ __global__ __launch_bounds__(256) void fork_blocks_kernel(ForkArgs a, ForkTable 
             a.tableOut[(int64_t)row * a.cols + j] = j == tail ? (ok ? dst : -1) : a.table[(int64_t)parent * a.tableStride + j];
         if (threadIdx.x == 0) {
             a.lengthsOut[row] = a.lengths[parent];
-            a.spareOut[row] = tail < 0 ? dst : mine % blockSize ? a.table[(int64_t)row * a.tableStride + mine / blockSize] : -1;
+            int spare = tail < 0 ? dst : mine % blockSize ? a.table[(int64_t)row * a.tableStride + mine / blockSize] : -1;
+            if (a.owned) { // the row's blocks and its spare one change places: each block stays in one of the two
+                spare = dst;
+                if (ok) {
+                    int* own = a.owned + (int64_t)row * a.ownedStride + tail;
+                    spare = *own;
+                    *own = dst;
+                }
+            }
+            a.spareOut[row] = spare;
         }
         return;
     }

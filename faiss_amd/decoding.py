@@ -1,12 +1,12 @@
 """faiss_amd/decoding.py -- operators of a program that decodes with a model next to its searches, over torch tensors.
 
     cache = PagedCache(res, num_blocks, block_size, num_heads, head_dim, code="e4m3")   # one per layer
-    plan = plan_blocks(res, table, lengths, new_lengths, ring, state, block_size, max_tokens)
+    plan = plan_blocks(res, table, lengths, new_lengths, ring, state, block_size, max_tokens, owned_table=owned)
     cache.add(k, v, plan.slots)
     out = cache.attend(q, table, plan.lengths, query_offsets=plan.query_offsets)
     scores, parents, tokens = beam_select(res, logits, scores, num_beams)
     states = reorder_beams(res, states, parents)
-    table, lengths, spare = fork_blocks(res, caches, table, lengths, spare, parents)
+    table, lengths, spare = fork_blocks(res, caches, table, lengths, spare, parents, owned_table=owned)
 
 The work of a call is ordered on torch's current stream of the resources' device and nothing is synchronised, so calls can be
 captured into a graph; results and scratch come from torch's allocator.  What the calls compute, and what they do with lengths,
@@ -65,7 +65,8 @@ class _StateStruct(ctypes.Structure):
 
 class _ForkStruct(ctypes.Structure):
     _fields_ = [("blockTable", _P), ("tableStride", _I64), ("lengths", _P), ("spare", _P), ("parents", _P), ("tableOut", _P),
-                ("lengthsOut", _P), ("spareOut", _P), ("batch", _I), ("beams", _I), ("numColumns", _I), ("pointersChecked", _I)]
+                ("lengthsOut", _P), ("spareOut", _P), ("batch", _I), ("beams", _I), ("numColumns", _I), ("pointersChecked", _I),
+                ("ownedTable", _P), ("ownedStride", _I64)]
 
 
 _byref = ctypes.byref
@@ -390,11 +391,14 @@ def reorder_beams(res, states, parents):
     return outs
 
 
-def fork_blocks(res, caches, block_table, lengths, spare, parents):
+def fork_blocks(res, caches, block_table, lengths, spare, parents, owned_table=None):
     """Reorders beams over paged caches (all the layers that block_table leads to): row b * beams + j takes over the blocks of row
     b * beams + parents[b, j]; full blocks are shared, a partly filled last one is copied into the row's spare block.  ->
     new (block_table, lengths, spare).  block_table [batch * beams, columns], lengths, spare [batch * beams], parents [batch,
-    beams], all int32 (faiss_amd_fork_blocks)."""
+    beams], all int32 (faiss_amd_fork_blocks).  owned_table (the shape of block_table, updated in place): the one given to
+    plan_blocks for these rows; with it every block stays in one of owned_table, spare and the free blocks.  Without it the new
+    spare blocks are still noted there: once the rows are released, take the spare blocks first given again.  The beams of an item
+    shrink together, in one call of plan_blocks, to zero or to whole blocks."""
     _rows(res, block_table, "block_table")
     _tensor(res, parents, "parents", torch.int32, 2)
     n, w = parents.shape
@@ -403,6 +407,10 @@ def fork_blocks(res, caches, block_table, lengths, spare, parents):
         raise ValueError("block_table must have batch * beams = %d rows" % (n * w))
     for t, name in ((lengths, "lengths"), (spare, "spare")):
         _same_length(_tensor(res, t, name, torch.int32, 1), rows, name)
+    if owned_table is not None:
+        _rows(res, owned_table, "owned_table")
+        if owned_table.shape != block_table.shape:
+            raise ValueError("owned_table must have the shape of block_table")
     if not caches:
         raise ValueError("at least one cache")
     for c in caches:
@@ -413,7 +421,8 @@ def fork_blocks(res, caches, block_table, lengths, spare, parents):
                        torch.empty(rows, dtype=torch.int32, device=dev))
     arr = (_CacheStruct * len(caches))(*[c._s for c in caches])
     a = _ForkStruct(block_table.data_ptr() or None, _row_stride(block_table), lengths.data_ptr() or None, spare.data_ptr() or None,
-                    parents.data_ptr() or None, table.data_ptr() or None, lens.data_ptr() or None, sp.data_ptr() or None, n, w, cols, 1)
+                    parents.data_ptr() or None, table.data_ptr() or None, lens.data_ptr() or None, sp.data_ptr() or None, n, w, cols, 1,
+                    owned_table.data_ptr() or None if owned_table is not None else None, _row_stride(owned_table) if owned_table is not None else 0)
     if rows:
         _check(res._lib.faiss_amd_fork_blocks(res._h, len(caches), arr, _byref(a), _stream(res)))
     return table, lens, sp

@@ -604,13 +604,21 @@ int faiss_amd_reorder_beams(FaissAmdGpuResources* res, int n, const FaissAmdBeam
  * block is copied into spare[row], which takes its place in the row's table, and the row's own last block becomes its spare
  * one.  spare [batch * beams]: one block per row that no table names; the beams of a batch item have the same length.
  * Outputs [batch * beams][numColumns], [batch * beams], [batch * beams] overlap no input.  A spare block out of range where
- * one is needed: the row's table gets -1 there. */
+ * one is needed: the row's table gets -1 there.
+ * ownedTable (nullable, [batch * beams][ownedStride], updated in place): the one that plan_blocks is given for these rows.  A row's
+ * entry for the partly filled block and its spare one change places, so that every block is in exactly one of ownedTable, spare
+ * and the ring of free blocks, whoever's tables name it, and rows and spares can be used on when the requests are done (where the
+ * spare block is out of range both stay as they are).  Without it the blocks in spareOut are still noted in ownedTable: after the rows
+ * have been released they are free, and the spares first given have to be taken again.  Shared blocks keep their column: the beams of a
+ * batch item are to shrink together, in one call of plan_blocks, to zero or to whole blocks. */
 typedef struct FaissAmdForkBlocksParams {
     const int* blockTable;
     int64_t tableStride;
     const int *lengths, *spare, *parents;
     int *tableOut, *lengthsOut, *spareOut;
     int batch, beams, numColumns, pointersChecked;
+    int* ownedTable;
+    int64_t ownedStride;
 } FaissAmdForkBlocksParams;
 int faiss_amd_fork_blocks(FaissAmdGpuResources* res, int n, const FaissAmdPagedCache* caches, const FaissAmdForkBlocksParams* args, void* stream);
 

@@ -238,3 +238,90 @@ def test_reorder_long_rows(res):
         for x, y in zip(got, states):
             assert torch.equal(x[0, 0], y[0, 1]) and torch.equal(x[0, 1], y[0, 0]), y.shape
         del states, got
+
+
+# ------------------------------------------------------------------------------------------------ blocks that come back
+@pytest.mark.parametrize("n, w, bs, prompt, steps", [(2, 3, 16, 21, 30), (3, 4, 32, 64, 40), (1, 2, 16, 0, 20)])
+def test_fork_and_plan_keep_every_block_once(res, n, w, bs, prompt, steps):
+    """three rounds of requests over the same rows, without giving anything by hand: plan, add, fork, whole blocks taken back,
+    release.  Every block is in one of the owned table, the spare ones and the free ones at all times, and each beam's context
+    is what its history says"""
+    import random
+    rng = random.Random(n * w)
+    h, d, cols = 1, 64, 6
+    rows = n * w
+    emb = torch.randn((50, 2, h, d), device="cuda").bfloat16()
+    total = rows * (cols + 1)
+    c = decoding.PagedCache(res, total, bs, h, d, "e4m3")
+    pages = torch.randperm(total, generator=torch.Generator().manual_seed(n)).to(I32).cuda()
+    spare, ring = pages[:rows].clone(), torch.cat([pages[rows:], torch.full((rows,), -1, dtype=I32, device="cuda")])
+    state = torch.tensor([0, total - rows], dtype=torch.int64, device="cuda")
+    view = torch.full((rows, cols), -1, dtype=I32, device="cuda")
+    owned, lengths = view.clone(), torch.zeros(rows, dtype=I32, device="cuda")
+
+    def plan(want, room):
+        p = decoding.plan_blocks(res, view, lengths, ints(want), ring, state, bs, room, owned_table=owned, free_state_out=state)
+        assert p.granted.tolist() == [1] * rows
+        return p
+
+    def once():
+        free = [int(ring[(int(state[0]) + i) % total]) for i in range(int(state[1]))]
+        held = [x for r in range(rows) for x in owned[r, :-(-int(lengths[r]) // bs)].tolist()]
+        assert sorted(free + held + spare.tolist()) == list(range(total))
+        # no two beams write to the same block, and none into a spare or free one
+        tails = [int(view[r, int(lengths[r]) // bs]) for r in range(rows) if int(lengths[r]) % bs]
+        assert len(set(tails)) == len(tails) and not set(tails) & set(spare.tolist() + free)
+
+    for trial in range(3):
+        history = [[rng.randrange(50) for _ in range(prompt + trial)] for _ in range(n) for _ in range(w)]
+        history = [list(history[(r // w) * w]) for r in range(rows)]
+        new = [list(x) for x in history]
+        for step in range(steps):
+            p = plan([len(x) for x in history], sum(map(len, new)) + 1)
+            lengths = p.lengths
+            tok = torch.tensor([t for x in new for t in x] + [0], device="cuda")
+            c.add(emb[tok, 0], emb[tok, 1], p.slots)
+            once()
+            for r in range(rows):
+                m = len(history[r])
+                if m == 0:
+                    continue
+                for got, i in zip(c.reconstruct(view[r, :-(-m // bs)]), (0, 1)):
+                    e = emb[torch.tensor(history[r], device="cuda"), i].float()
+                    got = got.transpose(1, 2).reshape(-1, h, d)[:m]
+                    # a code is off by half a step, 2^-4 of the value; a block's scale that grows may round it again: twice that
+                    assert bool(((got - e).abs() <= 2 ** -3 * e.abs() + 0.02).all()), (trial, step, r)
+            parents = [[rng.randrange(w) for _ in range(w)] for _ in range(n)]
+            view, lengths, spare = decoding.fork_blocks(res, [c], view, lengths, spare, ints(parents), owned_table=owned)
+            once()
+            history = [list(history[(r // w) * w + parents[r // w][r % w]]) for r in range(rows)]
+            if step == steps // 2:  # back by whole blocks, all beams together
+                keep = [len(x) // bs * bs - bs if len(x) >= bs else 0 for x in history]
+                lengths = plan(keep, 1).lengths
+                history = [x[:k] for x, k in zip(history, keep)]
+                once()
+            new = [[rng.randrange(50)] for _ in range(rows)]
+            history = [x + y for x, y in zip(history, new)]
+        lengths = plan([0] * rows, 1).lengths
+        assert int(state[1]) == total - rows
+        once()
+
+
+def test_fork_blocks_owned_table_on_its_own(res):
+    """the owned table and the spare blocks: changed where a block is copied, left where there is nothing to copy or no block for it"""
+    bs, w = 16, 3
+    c = filled(res, 40, 1, bs, 64, "int8", 1)
+    table = ints([[i, 10 + i, -1] for i in range(2 * w)])
+    owned = torch.full((2 * w, 5), -7, dtype=I32, device="cuda")[:, :3]  # rows of a wider table
+    owned.copy_(ints([[i, 20 + i, -1] for i in range(2 * w)]))
+    lengths, spare = ints([20] * w + [32] * w), ints([30, -1, 40, 33, 34, 35])
+    parents = ints([[2, 0, 1], [1, 1, 5]])
+    t, l, s = decoding.fork_blocks(res, [c], table, lengths, spare, parents, owned_table=owned)
+    assert t.tolist() == [[2, 30, -1], [0, -1, -1], [1, -1, -1], [4, 14, -1], [4, 14, -1], [5, 15, -1]]
+    assert owned.tolist() == [[0, 30, -1], [1, 21, -1], [2, 22, -1], [3, 23, -1], [4, 24, -1], [5, 25, -1]]
+    assert s.tolist() == [20, -1, 40, 33, 34, 35] and l.tolist() == lengths.tolist()
+    assert owned._base[:, 3:].eq(-7).all()
+    with pytest.raises(ValueError):
+        decoding.fork_blocks(res, [c], table, lengths, spare, parents, owned_table=owned[:, :2])
+    with pytest.raises(TypeError):
+        decoding.fork_blocks(res, [c], table, lengths, spare, parents, owned_table=owned.long())
