@@ -59,9 +59,12 @@ __device__ __forceinline__ void wg_scan2(u64& x, u64& y, u64 (*part)[2]) {
     }
 }
 
-__device__ __forceinline__ int ring_at(int head, u64 i, int n) { // (head + i) mod n, i < 2 n
+__device__ __forceinline__ int ring_at(int head, u64 i, int n) { // (head + i) mod n, head < n
     u64 p = (u64)head + i;
-    while (p >= (u64)n) p -= n;
+    if (p >= (u64)n) {
+        p -= n;
+        if (p >= (u64)n) p %= (u64)n; // (i >= n only where lengths claim more blocks than there are)
+    }
     return (int)p;
 }
 

@@ -325,3 +325,33 @@ def test_fork_blocks_owned_table_on_its_own(res):
         decoding.fork_blocks(res, [c], table, lengths, spare, parents, owned_table=owned[:, :2])
     with pytest.raises(TypeError):
         decoding.fork_blocks(res, [c], table, lengths, spare, parents, owned_table=owned.long())
+
+
+@pytest.mark.parametrize("n, total, cols", [(1, 1, 1 << 20), (3, 7, 300000), (1500, 5, 4000)])
+def test_plan_blocks_given_back_more_than_there_are(res, n, total, cols):
+    """lengths that claim many times the ring's blocks: what is returned goes round, the count stays within the ring, and what
+    lies around it is left alone"""
+    table = torch.arange(cols, dtype=I32, device="cuda").repeat(n, 1)
+    ring = torch.full((total + 2,), -9, dtype=I32, device="cuda")
+    state = torch.tensor([total - 1, total], dtype=torch.int64, device="cuda")
+    p = decoding.plan_blocks(res, table, ints([cols] * n), ints([0] * n), ring[1:-1], state, 1, 3)
+    assert p.free_state.tolist() == [total - 1, total] and p.lengths.tolist() == [0] * n and p.granted.tolist() == [1] * n
+    assert ring[0] == -9 and ring[-1] == -9 and bool(((ring[1:-1] >= 0) & (ring[1:-1] < cols)).all())
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 1025])
+@pytest.mark.parametrize("tokens", [1, 40])
+def test_plan_blocks_around_a_thread_per_request(res, n, tokens):
+    """where the plan goes from one workgroup to the general kernels, with few and many slots"""
+    import random
+    from test_gpu_decoding import plan_both
+    rng = random.Random(n + tokens)
+    cols, bs = 5, 16
+    total = 3 * n
+    ring = list(range(total))
+    rng.shuffle(ring)
+    table = [[-1] * cols for _ in range(n)]
+    lens, state = [0] * n, [total - 5, total]
+    for step in range(3):
+        new = [rng.choice([x + tokens if x + tokens <= cols * bs else 0, max(x - 20, 0), x]) for x in lens]
+        lens, state = plan_both(res, table, None, lens, new, ring, state, bs, n * tokens)
