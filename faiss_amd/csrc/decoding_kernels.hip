@@ -515,7 +515,8 @@ __global__ __launch_bounds__(NT) void cache_add_kernel(AddArgs a) {
         // anything that is no number makes the block's scale, and with it all its values, no number until the block is begun anew
         if (amax < INFINITY && before >= 0.f && before < INFINITY) after = fmaxf(before, pow2_scale<CODE>(__builtin_bit_cast(unsigned, amax)));
         const bool number = after == after;
-        const float inv = number && after > 0.f ? 1.f / after : 0.f;
+        // (a subnormal scale is one that the caller has brought, and all that is added is zero: its inverse may be infinite)
+        const float inv = number && after >= FLT_MIN ? 1.f / after : 0.f;
         const float ratio = after > 0.f ? before / after : 0.f;
         const bool rescale = fresh || (number && ratio != 1.f), clear = rescale && ratio == 0.f;
         uint8_t* codes = (isV ? c.v : c.k) + ((int64_t)block * H + h) * (int64_t)bs * D;

@@ -355,3 +355,34 @@ def test_plan_blocks_around_a_thread_per_request(res, n, tokens):
     for step in range(3):
         new = [rng.choice([x + tokens if x + tokens <= cols * bs else 0, max(x - 20, 0), x]) for x in lens]
         lens, state = plan_both(res, table, None, lens, new, ring, state, bs, n * tokens)
+
+
+# ------------------------------------------------------------------------------------------------ adding
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("scale", [1e-40, 2.0 ** -149, 2.0 ** -126, 3e-20, 2.0 ** 127, 3e38])
+def test_add_over_any_scale(res, code, scale):
+    """zeros, then numbers, added behind tokens whose scale is subnormal, no power of two or the largest there is"""
+    for bs, d in ((16, 64), (64, 128)):
+        c = filled(res, 3, 2, bs, d, code, 1)
+        if scale > 1e30:  # (the old values stay within fp32)
+            c.k_codes.zero_()
+            c.v_codes.zero_()
+        c.k_scales.fill_(scale)
+        c.v_scales.fill_(scale)
+        old = [c.k_codes.double().clone(), c.v_codes.double().clone()]
+        x = torch.zeros((2, 2, d), device="cuda").bfloat16()
+        c.add(x, x, ints([bs + 3, bs + 9]))
+        k, v = c.k_codes.double(), c.v_codes.double()
+        assert bool((k[1, :, [3, 9]] == 0).all()) and bool((v[1, :, :, [3, 9]] == 0).all())
+        assert bool((c.k_scales == scale).all()) and bool((c.v_scales == scale).all())
+        old[0][1, :, [3, 9]], old[1][1, :, :, [3, 9]] = 0.0, 0.0
+        assert torch.equal(k, old[0]) and torch.equal(v, old[1])
+        # numbers: the scale is the larger of the old one and their power of two; a code is off by half a step of it
+        x = torch.randn((2, 2, d), device="cuda").bfloat16()
+        c.add(x, x, ints([bs + 4, 2 * bs + 1]))
+        got, _ = c.reconstruct(ints([1, 2]))
+        e = torch.stack([got[0, :, 4], got[1, :, 1]]).double() - x.double()
+        s = torch.stack([c.k_scales[1], c.k_scales[2]]).double()[:, :, None]
+        # (1 / scale and the product are rounded first: 2^-23 of the code)
+        room = (s * 2 ** -10 + x.double().abs() * 2 ** -4 if code == "e4m3" else s * 0.5) + x.double().abs() * 2 ** -22
+        assert bool((e.abs() <= room).all())
