@@ -11,7 +11,8 @@
 The work of a call is ordered on torch's current stream of the resources' device and nothing is synchronised, so calls can be
 captured into a graph; results and scratch come from torch's allocator.  What the calls compute, and what they do with lengths,
 slots, block ids and parents that are out of range, is stated in include/faiss_amd_c.h.  Tensors must be on the resources'
-device; arguments of the wrong shape, type or device raise ValueError / TypeError before anything is launched.
+device; arguments of the wrong shape, type or device raise ValueError / TypeError before anything is launched.  Nothing here has a
+backward pass: a tensor that requires a gradient is refused while gradients are recorded (torch.no_grad() says that none is meant).
 """
 import collections
 import ctypes
@@ -80,6 +81,8 @@ def _tensor(res, t, name, dtype=None, dim=None, dense=True):
         raise TypeError("%s must be %s, not %s" % (name, dtype, t.dtype))
     if dim is not None and t.dim() != dim:
         raise ValueError("%s must have %d dimensions, not %d" % (name, dim, t.dim()))
+    if dtype is not torch.int32 and t.requires_grad and torch.is_grad_enabled():
+        raise ValueError("%s requires a gradient, which this call does not give" % name)
     if not t.is_cuda or t.device.index != res.device:
         raise ValueError("%s must be on the resources' device cuda:%d, not %s" % (name, res.device, t.device))
     if dense and not t.is_contiguous():

@@ -60,3 +60,36 @@ def test_attend_past_a_launch(batch, heads, kv, fits):
     a = decoding._AttendStruct(tableStride=40, batch=batch, tokens=batch, heads=heads, numColumns=40, maxQueries=1, type=3, causal=1, scale=0.125)
     say = _error("faiss_amd_PagedCache_attend", None, ctypes.byref(_cache(numHeads=kv)), ctypes.byref(a), None)
     assert ("null resources" if fits else "too many rows") in say
+
+
+class _Res:  # what the wrappers look at before the library sees the call
+    device = 0
+    _h = None
+    _lib = None
+
+
+def _cache_on_the_host():
+    c = decoding.PagedCache.__new__(decoding.PagedCache)
+    c.res, c.num_heads, c.head_dim = _Res, 2, 64
+    return c
+
+
+def test_gradients_are_not_dropped():
+    """no operator has a backward pass: a tensor that requires a gradient is refused, unless none is recorded"""
+    i32 = torch.int32
+    c, x, n = _cache_on_the_host(), torch.zeros((3, 2, 64), dtype=torch.float16), torch.zeros(3, dtype=i32)
+    g = x.clone().requires_grad_()
+    table, parents = torch.zeros((3, 4), dtype=i32), torch.zeros((1, 2), dtype=i32)
+    logits, scores = torch.zeros((1, 2, 5)), torch.zeros((1, 2))
+    calls = [(lambda: c.attend(g, table, n), True), (lambda: c.attend(x, table, n), False), (lambda: c.add(g, x, n), True),
+             (lambda: decoding.beam_select(_Res, logits.clone().requires_grad_(), scores, 2), True),
+             (lambda: decoding.beam_select(_Res, logits, scores, 2), False)]
+    for call, refused in calls:
+        with pytest.raises(ValueError, match="gradient" if refused else "device"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="device"):
+            call()
+        with torch.inference_mode(), pytest.raises(ValueError, match="device"):
+            call()
+    with pytest.raises(ValueError, match="device"):  # (looked at first)
+        decoding.reorder_beams(_Res, [g], parents)

@@ -386,3 +386,25 @@ def test_add_over_any_scale(res, code, scale):
         # (1 / scale and the product are rounded first: 2^-23 of the code)
         room = (s * 2 ** -10 + x.double().abs() * 2 ** -4 if code == "e4m3" else s * 0.5) + x.double().abs() * 2 ** -22
         assert bool((e.abs() <= room).all())
+
+
+# ------------------------------------------------------------------------------------------------ refusals
+def test_gradients_are_not_dropped_on_the_device(res):
+    c = filled(res, 4, 2, 16, 64, "e4m3", 0)
+    x = torch.randn((1, 2, 64), device="cuda").half()
+    g = x.clone().requires_grad_()
+    table, n, parents = ints([[0, 1]]), ints([3]), ints([[1, 0]])
+    logits, scores = torch.randn((1, 2, 5), device="cuda"), torch.zeros((1, 2), device="cuda")
+    state = torch.randn((1, 2, 7), device="cuda")
+    calls = [lambda f: c.attend(f(x), table, n), lambda f: c.attend(x, table, n, out=f(x.clone())), lambda f: c.add(f(x), x, n),
+             lambda f: c.add(x, f(x), n), lambda f: decoding.beam_select(res, f(logits), scores, 2),
+             lambda f: decoding.beam_select(res, logits, f(scores), 2), lambda f: decoding.reorder_beams(res, [state, f(state)], parents)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call(lambda t: t.clone().requires_grad_())
+        want = call(lambda t: t)
+        with torch.no_grad():
+            got = call(lambda t: t.clone().requires_grad_())
+        for a, b in zip(got if isinstance(got, (list, tuple)) else [got], want if isinstance(want, (list, tuple)) else [want]):
+            assert a is None or torch.equal(a, b)
+    assert g.grad is None
