@@ -81,8 +81,11 @@ def _tensor(res, t, name, dtype=None, dim=None, dense=True):
         raise TypeError("%s must be %s, not %s" % (name, dtype, t.dtype))
     if dim is not None and t.dim() != dim:
         raise ValueError("%s must have %d dimensions, not %d" % (name, dim, t.dim()))
-    if dtype is not torch.int32 and t.requires_grad and torch.is_grad_enabled():
-        raise ValueError("%s requires a gradient, which this call does not give" % name)
+    if dtype is not torch.int32:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError("%s requires a gradient, which this call does not give" % name)
+        if t.is_neg() or t.is_conj():  # (the memory holds other numbers than the tensor)
+            raise ValueError("%s is negated or conjugated lazily: resolve_neg() or resolve_conj() first" % name)
     if not t.is_cuda or t.device.index != res.device:
         raise ValueError("%s must be on the resources' device cuda:%d, not %s" % (name, res.device, t.device))
     if dense and not t.is_contiguous():

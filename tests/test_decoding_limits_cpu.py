@@ -93,3 +93,20 @@ def test_gradients_are_not_dropped():
             call()
     with pytest.raises(ValueError, match="device"):  # (looked at first)
         decoding.reorder_beams(_Res, [g], parents)
+
+
+def test_lazily_negated_and_conjugated_tensors_are_refused():
+    """their memory holds other numbers than the tensor does"""
+    i32 = torch.int32
+    c, n, table, parents = _cache_on_the_host(), torch.zeros(3, dtype=i32), torch.zeros((3, 4), dtype=i32), torch.zeros((1, 2), dtype=i32)
+    z = torch.randn((1, 2, 5), dtype=torch.complex64)
+    neg = z.conj().imag
+    assert neg.is_neg()
+    scores = torch.zeros((1, 2))
+    for call in (lambda: decoding.beam_select(_Res, neg, scores, 2), lambda: decoding.beam_select(_Res, torch._neg_view(neg.clone()), scores, 2)):
+        with pytest.raises(ValueError, match="lazily"):
+            call()
+    half = torch._neg_view(torch.zeros((3, 2, 64), dtype=torch.float16))
+    for call in (lambda: c.attend(half, table, n), lambda: c.add(half, half, n)):
+        with pytest.raises(ValueError, match="lazily"):
+            call()

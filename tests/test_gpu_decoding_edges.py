@@ -408,3 +408,14 @@ def test_gradients_are_not_dropped_on_the_device(res):
         for a, b in zip(got if isinstance(got, (list, tuple)) else [got], want if isinstance(want, (list, tuple)) else [want]):
             assert a is None or torch.equal(a, b)
     assert g.grad is None
+
+
+def test_reorder_complex_states(res):
+    """complex rows are reordered as bytes; a lazy conjugate, whose memory holds other numbers, is refused"""
+    z = torch.randn((2, 3, 5), dtype=torch.complex64, device="cuda")
+    p = ints([[2, 0, 1], [1, 1, 2]])
+    for t in (z, z.conj().resolve_conj(), z.conj().imag.resolve_neg()):
+        assert torch.equal(decoding.reorder_beams(res, [t], p)[0], t[torch.arange(2, device="cuda")[:, None], p.long()])
+    for t in (z.conj(), z.conj().imag):
+        with pytest.raises(ValueError, match="lazily"):
+            decoding.reorder_beams(res, [t], p)
