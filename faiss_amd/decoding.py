@@ -118,6 +118,15 @@ def _dense_last(t, name):
         raise ValueError("the last dimension of %s must be dense" % name)
 
 
+def _rows_apart(t, name):
+    """no two rows of t [n, m, dense] share memory (or are interleaved): one of two results would stand there"""
+    reach = t.shape[2]
+    for stride, n in sorted((t.stride(i), t.shape[i]) for i in (0, 1)):
+        if n > 1 and stride < reach:
+            raise ValueError("the rows of %s must not overlap" % name)
+        reach += stride * (n - 1) if n > 1 else 0
+
+
 try:  # the same number without a Stream object around it (a microsecond of every call)
     _raw_stream = torch._C._cuda_getCurrentRawStream
 except AttributeError:  # a torch without CUDA / HIP
@@ -264,7 +273,7 @@ class PagedCache:
         b's queries are the rows query_offsets[b] ... query_offsets[b + 1] - 1 (int32 [batch + 1]; None: row b) and stand at
         its end.  scale: 1 / sqrt(head_dim) by default.  max_queries: an upper bound of a request's queries, which saves
         work that only longer ones need.  Rows of no request are left as they are in `out` (zero if it is None);
-        out may be q."""
+        out may be q itself, and shares no other memory with it."""
         res = self.res
         _tensor(res, q, "q", None, 3, dense=False)
         if q.dtype not in _HALF:
@@ -291,6 +300,7 @@ class PagedCache:
             if out.shape != q.shape:
                 raise ValueError("out must have the shape of q")
             _dense_last(out, "out")
+            _rows_apart(out, "out")
         lse = None
         if return_lse:
             lse = torch.full((t, h), -math.inf, device=q.device)

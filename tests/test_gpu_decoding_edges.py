@@ -419,3 +419,25 @@ def test_reorder_complex_states(res):
     for t in (z.conj(), z.conj().imag):
         with pytest.raises(ValueError, match="lazily"):
             decoding.reorder_beams(res, [t], p)
+
+
+def test_attend_out_that_overlaps_is_refused(res):
+    c, table = paged(res, [20, 20, 20], 16, 1, 64, "e4m3", 0)
+    q, lens = torch.randn((3, 4, 64), device="cuda").half(), ints([20, 20, 20])
+    base = torch.zeros(4096, device="cuda").half()
+    want = c.attend(q, table, lens)
+    for stride in ((0, 64, 1), (256, 0, 1), (256, 63, 1), (255, 64, 1), (64, 64, 1), (63, 192, 1), (64, 191, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            c.attend(q, table, lens, out=base.as_strided((3, 4, 64), stride))
+    for stride in ((256, 64, 1), (300, 67, 1), (64, 192, 1), (70, 400, 1)):
+        out = base.as_strided((3, 4, 64), stride)
+        assert c.attend(q, table, lens, out=out) is out and torch.equal(out, want)
+    # one row or one head: the other stride does not matter
+    for shape, stride in (((1, 4, 64), (0, 64, 1)), ((3, 1, 64), (64, 0, 1)), ((1, 1, 64), (0, 0, 1))):
+        out = base.as_strided(shape, stride)
+        x = q[:shape[0], :shape[1]]
+        assert torch.equal(c.attend(x, table[:shape[0]], lens[:shape[0]], out=out), want[:shape[0], :shape[1]])
+    with pytest.raises(ValueError, match="overlap"):
+        c.attend(q[:, :1], table, lens, out=base.as_strided((3, 1, 64), (32, 0, 1)))
+    with pytest.raises(ValueError, match="overlap"):
+        c.attend(q[:1], table[:1], lens[:1], out=base.as_strided((1, 4, 64), (0, 32, 1)))
