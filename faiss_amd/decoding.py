@@ -209,6 +209,8 @@ class PagedCache:
         return self
 
     def _set(self, res, k, v, ks, vs):
+        if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
+            raise TypeError("codes must be torch tensors")
         if k.dtype not in _CODE_OF or v.dtype != k.dtype:
             raise TypeError("codes must be torch.int8 or torch.float8_e4m3fn, keys and values alike")
         _tensor(res, k, "k_codes", None, 4)
@@ -340,10 +342,10 @@ def beam_select(res, logits, scores, num_beams, finished=None, pad_token=0):
     if tuple(_tensor(res, scores, "scores", torch.float32, 2).shape) != (n, w):
         raise ValueError("scores must have the shape %s" % ((n, w),))
     if finished is not None:
-        if finished.dtype not in (torch.bool, torch.uint8):
-            raise TypeError("finished must be bool or uint8")
         if tuple(_tensor(res, finished, "finished", None, 2).shape) != (n, w):
             raise ValueError("finished must have the shape %s" % ((n, w),))
+        if finished.dtype not in (torch.bool, torch.uint8):
+            raise TypeError("finished must be bool or uint8")
     k = int(num_beams)
     dev = logits.device
     if k < 1:
@@ -427,9 +429,12 @@ def fork_blocks(res, caches, block_table, lengths, spare, parents, owned_table=N
         _rows(res, owned_table, "owned_table")
         if owned_table.shape != block_table.shape:
             raise ValueError("owned_table must have the shape of block_table")
+    caches = list(caches)
     if not caches:
         raise ValueError("at least one cache")
     for c in caches:
+        if not isinstance(c, PagedCache):
+            raise TypeError("caches must be PagedCache objects")
         if c.res.device != res.device:
             raise ValueError("the caches must be on the resources' device")
     dev = block_table.device

@@ -110,3 +110,13 @@ def test_lazily_negated_and_conjugated_tensors_are_refused():
     for call in (lambda: c.attend(half, table, n), lambda: c.add(half, half, n)):
         with pytest.raises(ValueError, match="lazily"):
             call()
+
+
+def test_what_is_no_tensor_is_a_type_error():
+    t = torch.zeros((1, 1, 16, 64), dtype=torch.int8)
+    s = torch.zeros((1, 1))
+    for k, v in (([0], t), (t, [0]), (None, None)):
+        with pytest.raises(TypeError):
+            decoding.PagedCache.wrap(_Res, k, v, s, s)
+    with pytest.raises(ValueError, match="device"):
+        decoding.PagedCache.wrap(_Res, t, t, s, s)

@@ -441,3 +441,19 @@ def test_attend_out_that_overlaps_is_refused(res):
         c.attend(q[:, :1], table, lens, out=base.as_strided((3, 1, 64), (32, 0, 1)))
     with pytest.raises(ValueError, match="overlap"):
         c.attend(q[:1], table[:1], lens[:1], out=base.as_strided((1, 4, 64), (0, 32, 1)))
+
+
+def test_wrong_kinds_are_type_errors(res):
+    """what is no tensor, or no cache, is a TypeError like a wrong dtype"""
+    logits, scores = torch.zeros((1, 2, 5), device="cuda"), torch.zeros((1, 2), device="cuda")
+    for bad in ([[True, False]], scores, 1):
+        with pytest.raises(TypeError):
+            decoding.beam_select(res, logits, scores, 2, finished=bad)
+    c = filled(res, 4, 1, 16, 64, "int8", 0)
+    args = (ints([[0], [1]]), ints([3, 3]), ints([2, 3]), ints([[0, 1]]))
+    for bad in ([c, None], [c.k_codes], 3):
+        with pytest.raises(TypeError):
+            decoding.fork_blocks(res, bad, *args)
+    with pytest.raises(ValueError):
+        decoding.fork_blocks(res, [], *args)
+    decoding.fork_blocks(res, (x for x in [c]), *args)  # any iterable
