@@ -628,8 +628,11 @@ __global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs 
 // ================================================================================================ beam selection
 // value(w, v) = score_w + x_wv - log sum_v exp x_wv.  Inside a beam candidates rank as their logits do, so one pass over the logits
 // keeps the `keep` best (logit, lowest v) of every piece of a row beside its maximum and sum of exponentials; a second launch
-// joins the pieces of a row, then the rows of a batch item.  The exponentials' sum is accumulated in 64 bits and candidates of
-// different beams are compared as 64-bit values: they come in the order of the exact values unless those agree to ~1e-8.
+// joins the pieces of a row, then the rows of a batch item.  An exponential is an fp32 one: its argument is off by (2^-23 + 2^-26)
+// |x - max|, the instruction by 2^-23; four are added in fp32, everything beyond that in 64 bits, and candidates of different beams are
+// compared as 64-bit values.  Measured, a log-sum is off by 1e-8 where logits are spread (128001 of them, 3e-8 at 1000) and by up
+// to 8e-8 where one dominates (all sixteen of a lane added in fp32, and lanes joined by fp32 exponentials: 6e-8 and 9e-7, in the
+// same time); beams whose values are closer than that may change places.
 // 512 rows of 128001 bf16 logits, 16 kept: 43 us (131 MB, 3.0 TB/s) and 9 us for the join; 4 rows of 32000:
 // 7.9 + 5.1 us.  13 vector instructions per logit keep the SIMDs busy for half of the time; neither they nor the memory are full.
 constexpr int kBeamVpt = 16;                                   // logits per lane and step
@@ -783,16 +786,21 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s)
                 best[j] = mx;
                 // running maximum and sum of the lane; a NaN or an infinity makes the sum NaN
                 const float mn = fmaxf(m, mx);
-                float p = 0.f;
+                double p = 0.0;
 #pragma unroll
-                for (int i = 0; i < kBeamVpt; ++i) p += __builtin_amdgcn_exp2f((v[i] - mn) * 1.4426950408889634f);
+                for (int i = 0; i < kBeamVpt; i += 4) {
+                    float e[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = __builtin_amdgcn_exp2f((v[i + j] - mn) * 1.4426950408889634f);
+                    p += (double)((e[0] + e[1]) + (e[2] + e[3])); // (one that dominates leaves the others 24 bits, not 20)
+                }
                 if (mn == -INFINITY) { // (nothing but -inf so far, or a NaN among it)
-                    p = 0.f;
+                    float q = 0.f;
 #pragma unroll
-                    for (int i = 0; i < kBeamVpt; ++i) p = v[i] == v[i] ? p : v[i];
-                    sum += (double)p;
+                    for (int i = 0; i < kBeamVpt; ++i) q = v[i] == v[i] ? q : v[i];
+                    sum += (double)q;
                 } else {
-                    sum = sum * (double)__builtin_amdgcn_exp2f((m - mn) * 1.4426950408889634f) + (double)p;
+                    sum = sum * (double)__builtin_amdgcn_exp2f((m - mn) * 1.4426950408889634f) + p;
                 }
                 m = mn;
             }
@@ -855,7 +863,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamArgs a, BeamSched s)
     float M = m;
 #pragma unroll
     for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-    double S = (m == -INFINITY && sum == sum) ? 0.0 : sum * (double)__builtin_amdgcn_exp2f((m - M) * 1.4426950408889634f);
+    double S = (m == -INFINITY && sum == sum) ? 0.0 : sum * exp((double)m - (double)M);
 #pragma unroll
     for (int o = 32; o; o >>= 1) S += __shfl_xor(S, o, 64);
     if (lane == 0) {

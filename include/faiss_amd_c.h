@@ -573,7 +573,9 @@ int faiss_amd_PagedCache_attend_workspace(FaissAmdGpuResources* res, const Faiss
  * logits[b][w][u], the `keep` largest in order, ties to the lowest w, then the lowest v.  logits F32 / F16 / BF16 with strides in
  * elements, the last dimension dense; finished (nullable, bytes [batch][beams]): such a beam's only candidate is (w, padToken)
  * with the value scores[b][w].  Candidates of probability zero or without a number (a row with NaN or +inf) are none; where
- * fewer than `keep` remain, score -inf, parent -1, token -1.  beams, keep <= 64.  Outputs [batch][keep]. */
+ * fewer than `keep` remain, score -inf, parent -1, token -1.  beams, keep <= 64.  Outputs [batch][keep].
+ * Within a beam the order is that of the logits, exactly.  Between beams it is that of the values as computed: exponentials are
+ * fp32, their sum fp64, which leaves a log-sum off by 1e-8 ... 1e-7 (2^-17 if all roundings went the same way). */
 typedef struct FaissAmdBeamSelectParams {
     const void* logits;
     int64_t batchStride, beamStride;

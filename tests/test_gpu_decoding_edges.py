@@ -457,3 +457,66 @@ def test_wrong_kinds_are_type_errors(res):
     with pytest.raises(ValueError):
         decoding.fork_blocks(res, [], *args)
     decoding.fork_blocks(res, (x for x in [c]), *args)  # any iterable
+
+
+# ------------------------------------------------------------------------------------------------ beams
+def _log_sums_less(rows):
+    """rows [n, v]: fp32 scores that take nearly all of each row's best value away, so that the fp32 results keep the digits of
+    the log-sum's error; the exact values that they leave"""
+    top = rows.double().amax(-1)
+    lse = torch.logsumexp(rows.double(), -1)
+    s = (lse - top).float()
+    return s, s.double() + top - lse
+
+
+@pytest.mark.parametrize("far", [-0.5, -3.0, -7.7, -10.0, -11.3, -12.9, -14.2, -16.0])
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+def test_beam_select_one_token_dominates(res, far, dt):
+    """One token at 0, the others at `far`, 1000 of them: 16 of a lane at most, one step.  Lanes without the token have exact terms
+    (2^0).  In its lane a term is off by |far| (2^-23 + 2^-26) and 2^-23; four terms are added in fp32, two roundings of 2^-24 of
+    at most 1 + 3 e^far; sums beyond that are in 64 bits."""
+    for pos in (0, 5, 500, 999):
+        x = torch.full((1, 1, 1000), far, device="cuda").to(dt)
+        x[0, 0, pos] = 0
+        e = math.exp(float(x[0, 0, pos - 1]))
+        s, want = _log_sums_less(x[0])
+        got, _, tok = decoding.beam_select(res, x, s[None], 1)
+        tol = (2 ** -23 * (1 + 3 * e) + 15 * e * (abs(far) * (2 ** -23 + 2 ** -26) + 2 ** -23)) / (1 + 999 * e) + 2 ** -45
+        assert int(tok) == pos and abs(float(got.double() - want)) <= tol, (pos, float(got.double() - want), tol)
+
+
+@pytest.mark.parametrize("v", [1000, 32000, 128001])
+@pytest.mark.parametrize("dt", [torch.float32, torch.float16, torch.bfloat16])
+def test_beam_select_log_sums(res, v, dt):
+    """Rows of all kinds.  A term is off by |x - max| (2^-23 + 2^-26) (its own exponential's argument and those that rescale the
+    sums it is in: their differences add up) and by 2^-23 for each of them, at most one a step: 2^-23 (3 + steps) with the sums of four"""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(v)
+    n = torch.randn((12, v), generator=g, device="cuda")
+    up = torch.linspace(-20, 0, v, device="cuda")
+    rows = torch.stack([n[0], n[1] * 3, n[2] * 10, n[3] * 0.1, n[4].exp(), -(n[5].abs()) * 4, up, up.flip(0), up * 3, n[6] * 3 + 100,
+                        n[7] * 30 - 1000, torch.zeros_like(up)]).to(dt)
+    for row in rows:
+        s, want = _log_sums_less(row[None])
+        got, _, _ = decoding.beam_select(res, row[None, None], s[None], 1)
+        d = row.double() - row.double().max()
+        p = d.exp()
+        steps = min(v // 1024 + 1, 8 + v // 4096)
+        tol = float((p * -d).sum() / p.sum()) * (2 ** -23 + 2 ** -26) + 2 ** -23 * (3 + steps) + 2 ** -45
+        assert abs(float(got.double() - want)) <= tol
+
+
+def test_beam_select_beams_that_are_close(res):
+    """beams whose values differ by less than an fp32 sum of 16 tells, in both orders"""
+    x = torch.full((1, 2, 1000), -math.inf, device="cuda")
+    x[0, 0, :2] = 0.0                  # log-sum log 2
+    for far, pos in ((-10.0, 700), (-11.3, 5), (-11.3, 700), (-12.9, 999), (-7.7, 0)):
+        x[0, 1] = far
+        x[0, 1, pos] = 0.0
+        lse = torch.logsumexp(x[0].double(), -1)
+        for gap in (-3e-7, 3e-7):
+            s = (lse + torch.tensor([0.0, gap], device="cuda").double()).float()
+            exact = s.double() - lse
+            assert 2.4e-7 < abs(float(exact[0] - exact[1])) < 3.6e-7
+            _, parents, _ = decoding.beam_select(res, x, s[None], 1)
+            assert int(parents) == int(exact.argmax()), (far, pos, gap)
