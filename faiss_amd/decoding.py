@@ -170,18 +170,20 @@ def plan_blocks(res, block_table, lengths, new_lengths, free_ring, free_state, b
         free_state_out = torch.empty(2, dtype=torch.int64, device=dev)
     else:
         _same_length(_tensor(res, free_state_out, "free_state_out", torch.int64, 1), 2, "free_state_out")
-    max_tokens = int(max_tokens)
+    max_tokens, block_size = int(max_tokens), int(block_size)
+    if not (0 <= max_tokens < 1 << 31 and 1 <= block_size < 1 << 31):
+        raise ValueError("block_size or max_tokens out of range")
     # everything that is made here in one allocation
     made = 0 if lengths_out is not None else n
-    offsets, granted, scratch, slots, own = torch.empty(6 * n + 3 + max(max_tokens, 0) + made, dtype=torch.int32, device=dev).split(
-        [n + 1, n, 4 * n + 2, max(max_tokens, 0), made])
+    offsets, granted, scratch, slots, own = torch.empty(6 * n + 3 + max_tokens + made, dtype=torch.int32, device=dev).split(
+        [n + 1, n, 4 * n + 2, max_tokens, made])
     if lengths_out is None:
         lengths_out = own
     a = _PlanStruct(block_table.data_ptr() or None, owned_table.data_ptr() if owned_table is not None else None,
                     _row_stride(block_table), _row_stride(owned_table) if owned_table is not None else 0, lengths.data_ptr() or None,
                     new_lengths.data_ptr() or None, free_ring.data_ptr() or None, free_state.data_ptr(), lengths_out.data_ptr() or None,
                     free_state_out.data_ptr(), offsets.data_ptr(), slots.data_ptr() or None, granted.data_ptr(), scratch.data_ptr(),
-                    n, cols, free_ring.shape[0], int(block_size), max_tokens, 1)
+                    n, cols, free_ring.shape[0], block_size, max_tokens, 1)
     _check(res._lib.faiss_amd_plan_blocks(res._h, _byref(a), _stream(res)))
     return BlockPlan(lengths_out, free_state_out, offsets, slots, granted)
 
@@ -293,7 +295,7 @@ class PagedCache:
             most = 1
         else:
             _same_length(_tensor(res, query_offsets, "query_offsets", torch.int32, 1), n + 1, "query_offsets")
-            most = t if max_queries is None else int(max_queries)
+            most = t if max_queries is None else min(int(max_queries), t)
         if out is None:
             out = torch.empty((t, h, d), dtype=q.dtype, device=q.device) if query_offsets is None else torch.zeros(
                 (t, h, d), dtype=q.dtype, device=q.device)
@@ -348,8 +350,10 @@ def beam_select(res, logits, scores, num_beams, finished=None, pad_token=0):
             raise TypeError("finished must be bool or uint8")
     k = int(num_beams)
     dev = logits.device
-    if k < 1:
+    if not 1 <= k <= 64:
         raise ValueError("num_beams must be in [1, 64]")
+    if not 0 <= int(pad_token) < max(v, 1):
+        raise ValueError("pad_token is no token of the vocabulary")
     out = torch.empty((n, k), device=dev)
     which = torch.empty((2, n, k), dtype=torch.int32, device=dev)
     parents, tokens = which[0], which[1]

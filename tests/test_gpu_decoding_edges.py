@@ -520,3 +520,22 @@ def test_beam_select_beams_that_are_close(res):
             assert 2.4e-7 < abs(float(exact[0] - exact[1])) < 3.6e-7
             _, parents, _ = decoding.beam_select(res, x, s[None], 1)
             assert int(parents) == int(exact.argmax()), (far, pos, gap)
+
+
+def test_numbers_past_32_bits_are_refused(res):
+    """they would reach the library without their upper halves"""
+    logits, scores = torch.randn((1, 2, 50), device="cuda"), torch.zeros((1, 2), device="cuda")
+    done = torch.tensor([[True, False]], device="cuda")
+    for kw in (dict(pad_token=2 ** 32 + 3), dict(pad_token=50), dict(pad_token=-1), dict(num_beams=2 ** 32 + 2), dict(num_beams=65), dict(num_beams=0)):
+        with pytest.raises(ValueError):
+            decoding.beam_select(res, **{**dict(logits=logits, scores=scores, num_beams=2, finished=done), **kw})
+    table, n, ring, state = ints([[-1] * 4]), ints([0]), ints([0, 1, 2]), torch.tensor([0, 3], device="cuda")
+    for bs, room in ((2 ** 32 + 16, 4), (0, 4), (-16, 4), (16, -1), (16, 2 ** 32 + 4)):
+        with pytest.raises(ValueError):
+            decoding.plan_blocks(res, table, n, ints([3]), ring, state, bs, room)
+    # a bound on the queries may be any number
+    c, table = paged(res, [40], 16, 1, 64, "e4m3", 0)
+    q = torch.randn((40, 2, 64), device="cuda").half()
+    want = c.attend(q, table, ints([40]), query_offsets=ints([0, 40]))
+    for most in (2 ** 32 + 1, 2 ** 40, 41):
+        assert torch.equal(c.attend(q, table, ints([40]), query_offsets=ints([0, 40]), max_queries=most), want)
