@@ -673,7 +673,7 @@ __global__ void __launch_bounds__(FB_MAX) ivfflat_fused_kernel(IvfFusedParams p)
 // both read from LDS as wave-wide broadcasts (every row of a block belongs to the same list):
 //   L2: tt = fmaf(-code, s_i, a_i), a_i = (q_i [- centroid_i]) - b_i   (fp16: tt = a_i - half)   acc = fmaf(tt, tt, acc)
 //   IP: acc = fmaf(w_i, code, acc), w_i = q_i * s_i                     (fp16: w_i = q_i);  + <q, b> (+ coarse term)
-// as two sequential chains, one over the even and one over the odd dimensions (packed fp32 math), added at the end:
+// as two sequential chains, one over the even and one over the odd dimensions, added at the end:
 // the distance to the reconstruction b_i + s_i * code_i of
 // faiss::ScalarQuantizer (quantizers.h:92-150: vmin + (code + 0.5) / 255 * vdiff) without materialising it.  With
 // residual encoding the L2 row a changes with the list: one row per probe of the workgroup (built once per query,
@@ -705,8 +705,8 @@ __device__ __forceinline__ float sq_comp(const unsigned (&w)[SqChunk<CT>::WORDS]
         return (float)__builtin_bit_cast(_Float16, hw);
     }
 }
-// components E, E + 1 of a chunk folded into the (even, odd) pair of chains with packed fp32 math (v_pk_fma_f32: two
-// IEEE fmas per instruction): acc[0] runs over the even dimensions, acc[1] over the odd ones
+// components E, E + 1 of a chunk folded into the (even, odd) pair of chains, two IEEE fmas (packed fp32 instructions are off for
+// every file): acc[0] runs over the even dimensions, acc[1] over the odd ones
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <int METRIC, int CT, int E>
 __device__ __forceinline__ void sq_fold(const unsigned (&w)[SqChunk<CT>::WORDS], const float* sv, const float* av, f32x2& acc) {

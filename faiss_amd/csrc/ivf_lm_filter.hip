@@ -490,8 +490,8 @@ __device__ __forceinline__ void lmf_scores(f32x16& a, const f32x4 (&rn)[4], bool
         // ONE v_fma_f32 per accumulator.  Rounds 4 / 5 asked for v_pk_fma_f32 here (two accumulators per instruction); round 6's
         // ablation (tools/pq_sweep_ablation.py, profiles/r6_pq_sweep_ablation.txt) put the always-on part of the epilogue at 0.6 of
         // the 3.2 ms of sweep 2 at nb = 100M -- ~ 520 cycles per 32-row block for 24 packed fma + 24 v_max3 --, and the guide's
-        // timing table prices a packed f32 instruction beside MFMAs at + 22 cycles against two plain ones (the file is compiled
-        // with -fno-slp-vectorize for the same reason: hipcc packs adjacent scalar f32 operations by itself).
+        // timing table prices a packed f32 instruction beside MFMAs at + 22 cycles against two plain ones (they are off for every
+        // file: hipcc packs adjacent scalar f32 operations by itself).
 #ifdef FAISS_AMD_LMF_PK_SCORES
         const f32x2 mh = f32x2{-0.5f, -0.5f};
 #pragma unroll
@@ -517,7 +517,7 @@ __device__ __forceinline__ void lmf_scores(f32x16& a, const f32x4 (&rn)[4], bool
         // interlock a VALU read of a register an MFMA is still writing (19 wait states behind a 16-pass XDL write).  Found in
         // round 5: with ONE query block per item the v_max3 sat right behind the last MFMA and read stale maxima -- rows of
         // the answer were not collected, a few queries per thousand, depending on the instruction schedule.  (L2: the
-        // compiler-visible v_pk_fma above reads the accumulators first and gets its wait states from the compiler.)
+        // compiler-visible fma above reads the accumulators first and gets its wait states from the compiler.)
         asm volatile("s_nop 15\n\ts_nop 3" ::"v"(a));
     }
     // L2: rows behind the end of the chunk arrive with |y'|^2 = +inf (rn_fetch of the sweeps), so they are -inf already --
