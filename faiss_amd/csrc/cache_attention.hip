@@ -33,6 +33,7 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kWaves = 4;
 constexpr int kTile = 64;        // tokens per step of a wavefront
 constexpr float kNoScale = -1000.f;
+constexpr float kNothing = -FLT_MAX; // reference of a row that has seen nothing (finite: its differences are no NaN)
 constexpr int kSeg = 64;         // tiles whose blocks and scales are held in LDS
 constexpr float kBias = 6.f, kSlack = 8.f; // see above; both in units of log 2
 constexpr float kRoom = 40.f;    // what the sums of probabilities are kept below their reference, see softmax_step
@@ -216,14 +217,15 @@ struct Rows {
     float top[NT];   // reference of the exponents, log2 of a probability times its value's scale
     float lref[NT];  // reference of the sum of the probabilities: never more than the largest score met so far
     float l[NT];     // sum of the probabilities, in units of 2^(lref - kBias + kRoom)
+    float unit[NT];  // one of 2^(top - vref - kBias) in these units
     float vref;      // log2 of the largest value scale met so far
     f32x4 o[NT][MD]; // sums of probability times value, in units of 2^(top - kBias)
     __device__ __forceinline__ void reset() {
         vref = kNoScale;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            top[t] = lref[t] = -INFINITY;
-            l[t] = 0.f;
+            top[t] = lref[t] = kNothing;
+            l[t] = unit[t] = 0.f;
 #pragma unroll
             for (int i = 0; i < MD; ++i) o[t][i] = f32x4{0.f, 0.f, 0.f, 0.f};
         }
@@ -309,12 +311,11 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
         }
     }
     const float vnew = fmaxf(w.vref, groups_max(lvs));
-    w.vref = vnew;
     // the exponent of the lane's value scale: where there is none the probability is needed for the sum alone, and 2^-100 of the
     // largest is as good as less
-    const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f);
-    float od[NT];
-    bool change = false;
+    const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f), iv = __builtin_amdgcn_exp2f(vnew - lv);
+    float now[NT];
+    bool change = vnew != w.vref;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         float mx = highest(sc[t][0][0], sc[t][0][1]);
@@ -325,11 +326,27 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
         mx = groups_max(__builtin_fmaf(fabsf(mx), 0x1p-22f, mx) + lv); // (NaN where a group's scores are all masked: passed over)
         // the reference follows the maximum only when that has grown by more than 2^8.  It is that of probability and scale
         // together: what a probability loses in fp16 is then small beside the row's largest term, whatever the scales
-        const float was = w.top[t], now = mx > was + kSlack ? mx : was;
-        const float top = now == -INFINITY ? 0.f : now;
-        w.top[t] = now;
-        od[t] = __builtin_amdgcn_exp2f(was - top);
-        const float sub = lv - (top - kBias);
+        now[t] = mx > w.top[t] + kSlack ? mx : w.top[t];
+        change |= now[t] != w.top[t];
+    }
+    if (__ballot(change)) {
+        w.vref = vnew;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const float od = __builtin_amdgcn_exp2f(w.top[t] - now[t]), ref = fmaxf(w.lref[t], now[t] - vnew);
+            w.l[t] *= __builtin_amdgcn_exp2f(w.lref[t] - ref);
+            w.unit[t] = __builtin_amdgcn_exp2f((now[t] - vnew) - ref - kRoom);
+            w.lref[t] = ref;
+            w.top[t] = now[t];
+#pragma unroll
+            for (int i = 0; i < MD; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w.o[t][i][e] *= od;
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const float sub = lv - (w.top[t] - kBias);
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -339,18 +356,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
                 sum += p;
                 pr[t][i >> 1][4 * (i & 1) + e] = (_Float16)p;
             }
-        const float ref = fmaxf(w.lref[t], now - vnew), base = now == -INFINITY ? 2000.f : ref; // (nothing seen: sum is 0, or NaN)
-        w.l[t] = __builtin_fmaf(sum, __builtin_amdgcn_exp2f((top - base) - (lv + kRoom)), w.l[t] * __builtin_amdgcn_exp2f(w.lref[t] - base));
-        w.lref[t] = ref;
-        change |= od[t] != 1.f;
-    }
-    if (__ballot(change)) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < MD; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) w.o[t][i][e] *= od[t];
+        w.l[t] = __builtin_fmaf(sum, iv * w.unit[t], w.l[t]);
     }
 }
 
@@ -449,11 +455,8 @@ struct Norm {
     }
 };
 // Partial results (of a wavefront, of a chunk) are results of their own tokens, with the reference and the sum of their
-// probabilities: they are joined with weights that add up to one.  Where a part saw nothing its reference is -inf, its sum and
-// result are zero.
-__device__ __forceinline__ float weight(float ref, float l, float largest) {
-    return l * __builtin_amdgcn_exp2f(ref - (largest == -INFINITY ? 0.f : largest));
-}
+// probabilities: they are joined with weights that add up to one.  Where a part saw nothing its sum and result are zero.
+__device__ __forceinline__ float weight(float ref, float l, float largest) { return l * __builtin_amdgcn_exp2f(ref - largest); }
 // a row of a wavefront's own: the result, or a chunk's partial sums
 template <int D, int NT, int MD>
 __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, const Item& it, int G, int row0, int rowsAll, Rows<NT, MD>& w) {
