@@ -37,6 +37,7 @@ constexpr float kNothing = -FLT_MAX; // reference of a row that has seen nothing
 constexpr int kSeg = 64;         // tiles whose blocks and scales are held in LDS
 constexpr float kBias = 6.f, kSlack = 8.f; // see above; both in units of log 2
 constexpr float kRoom = 40.f;    // what the sums of probabilities are kept below their reference, see softmax_step
+constexpr float kFar = 4096.f;   // references beyond this are taken from a base of their own, see softmax_step
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // what a launch works on, beside AttendArgs
@@ -52,7 +53,7 @@ struct Sched {
     int sort;         // of 64 requests, the longest first
     int mergeRows;    // workgroups that join a row tile's rows
     float* partO;     // [maxSlots][rows][dim]: results of chunks
-    float2* partML;   // [maxSlots][rows]: references and sums of their probabilities
+    float4* partML;   // [maxSlots][rows]: {base, reference, sum} of their probabilities
 };
 
 struct Item {
@@ -219,11 +220,15 @@ struct Rows {
     float l[NT];     // sum of the probabilities, in units of 2^(lref - kBias + kRoom)
     float unit[NT];  // one of 2^(top - vref - kBias) in these units
     float vref;      // log2 of the largest value scale met so far
+    float base[NT];  // what scores and references are counted from: 0 but where the scores are far from it
+    bool far;        // some row's base is not 0
     f32x4 o[NT][MD]; // sums of probability times value, in units of 2^(top - kBias)
     __device__ __forceinline__ void reset() {
         vref = kNoScale;
+        far = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
+            base[t] = 0.f;
             top[t] = lref[t] = kNothing;
             l[t] = unit[t] = 0.f;
 #pragma unroll
@@ -310,26 +315,67 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
             f[t] = 1.f;
         }
     }
+    if (w.far) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sc[t][i][e] = __builtin_fmaf(sc[t][i][e], f[t], -w.base[t]);
+            f[t] = 1.f;
+        }
+    }
     const float vnew = fmaxf(w.vref, groups_max(lvs));
     // the exponent of the lane's value scale: where there is none the probability is needed for the sum alone, and 2^-100 of the
     // largest is as good as less
     const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f), iv = __builtin_amdgcn_exp2f(vnew - lv);
+    auto lane_max = [&](int t) {
+        float mx = highest(sc[t][0][0], sc[t][0][1]);
+#pragma unroll
+        for (int i = 2; i < 16; ++i) mx = highest(mx, sc[t][i >> 2][i & 3]);
+        return mx * f[t];
+    };
+    auto reference = [&](int t) {
+        const float mx = lane_max(t);
+        // (2^-22: not below the exact products and sums of the fma below)
+        const float all = groups_max(__builtin_fmaf(fabsf(mx), 0x1p-22f, mx) + lv); // (NaN where a group's scores are all masked: passed over)
+        // the reference follows the maximum only when that has grown by more than 2^8.  It is that of probability and scale
+        // together: what a probability loses in fp16 is then small beside the row's largest term, whatever the scales
+        return all > w.top[t] + kSlack ? all : w.top[t];
+    };
     float now[NT];
     bool change = vnew != w.vref;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        float mx = highest(sc[t][0][0], sc[t][0][1]);
-#pragma unroll
-        for (int i = 2; i < 16; ++i) mx = highest(mx, sc[t][i >> 2][i & 3]);
-        mx *= f[t];
-        // (2^-22: not below the exact products and sums of the fma below, however large they are)
-        mx = groups_max(__builtin_fmaf(fabsf(mx), 0x1p-22f, mx) + lv); // (NaN where a group's scores are all masked: passed over)
-        // the reference follows the maximum only when that has grown by more than 2^8.  It is that of probability and scale
-        // together: what a probability loses in fp16 is then small beside the row's largest term, whatever the scales
-        now[t] = mx > w.top[t] + kSlack ? mx : w.top[t];
+        now[t] = reference(t);
         change |= now[t] != w.top[t];
     }
     if (__ballot(change)) {
+        // A reference is off by 2^-23 of itself, which from 2^13 on is felt in the probabilities and from 2^30 on takes them out of
+        // fp32.  Such a row's scores are counted from their largest so far instead: a difference of scores is one rounding
+        bool far = false;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) far |= now[t] != w.top[t] && fabsf(now[t]) > kFar && fabsf(now[t]) < INFINITY;
+        if (__ballot(far)) {
+            w.far = true;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const float most = groups_max(lane_max(t));
+                const bool moves = now[t] != w.top[t] && fabsf(now[t]) > kFar && fabsf(most) < INFINITY;
+                const float by = moves ? most : 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) sc[t][i][e] = __builtin_fmaf(sc[t][i][e], f[t], -by);
+                f[t] = 1.f;
+                w.base[t] += by;
+                if (w.top[t] != kNothing) {
+                    w.top[t] -= by;
+                    w.lref[t] -= by;
+                }
+                now[t] = reference(t);
+            }
+        }
         w.vref = vnew;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -434,9 +480,9 @@ __device__ __forceinline__ void close_rows(Rows<NT, MD>& w) {
         w.l[t] = groups_sum(w.l[t] + (m - m)); // (sums are finite or NaN)
     }
 }
-__device__ __forceinline__ float log_sum(float ref, float l) {
+__device__ __forceinline__ float log_sum(float base, float ref, float l) {
     const float up = l < 1.f ? kRoom - kBias : 0.f; // (the two would cancel)
-    return l == 0.f ? -INFINITY : (ref + (kRoom - kBias - up) + __builtin_amdgcn_logf(__builtin_ldexpf(l, (int)up))) * kLn2;
+    return l == 0.f ? -INFINITY : (base + (ref + (kRoom - kBias - up) + __builtin_amdgcn_logf(__builtin_ldexpf(l, (int)up)))) * kLn2;
 }
 // What a row's accumulators are multiplied by to become its result, as a factor and a power of two: the scales of the values go up
 // to the largest fp32 numbers and the sums beyond them, the results do not
@@ -456,7 +502,16 @@ struct Norm {
 };
 // Partial results (of a wavefront, of a chunk) are results of their own tokens, with the reference and the sum of their
 // probabilities: they are joined with weights that add up to one.  Where a part saw nothing its sum and result are zero.
-__device__ __forceinline__ float weight(float ref, float l, float largest) { return l * __builtin_amdgcn_exp2f(ref - largest); }
+struct Part {
+    float base, ref, l;
+    __device__ __forceinline__ float above(const Part& o) const { return (base - o.base) + (ref - o.ref); } // of references
+    __device__ __forceinline__ void raise(const Part& o) { // to the larger reference
+        const bool up = o.above(*this) > 0.f;
+        base = up ? o.base : base;
+        ref = up ? o.ref : ref;
+    }
+    __device__ __forceinline__ float weight(const Part& most) const { return l * __builtin_amdgcn_exp2f(above(most)); }
+};
 // a row of a wavefront's own: the result, or a chunk's partial sums
 template <int D, int NT, int MD>
 __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, const Item& it, int G, int row0, int rowsAll, Rows<NT, MD>& w) {
@@ -470,13 +525,13 @@ __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, 
             const int64_t pr = (int64_t)(it.slot + it.c) * s.rows + (r - it.rt * s.rows);
 #pragma unroll
             for (int i = 0; i < MD; ++i) *(f32x4*)(s.partO + pr * D + 16 * i + 4 * grp) = norm(w.o[t][i]);
-            if (grp == 0) s.partML[pr] = make_float2(w.lref[t], w.l[t]);
+            if (grp == 0) s.partML[pr] = make_float4(w.base[t], w.lref[t], w.l[t], 0.f);
         } else {
             const int qi = r / G, g = r - qi * G;
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + 4 * grp;
 #pragma unroll
             for (int i = 0; i < MD; ++i) store4(op + 16 * i, norm(w.o[t][i]), a.type);
-            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.lref[t], w.l[t]);
+            if (grp == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(w.base[t], w.lref[t], w.l[t]);
         }
     }
 }
@@ -591,13 +646,10 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 
     constexpr int PITCH = D + 4;
     __shared__ __align__(16) float sm[kWaves][16 * NT][PITCH];
-    __shared__ float sml[kWaves][16 * NT][2];
+    __shared__ Part sml[kWaves][16 * NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        if (grp == 0) {
-            sml[wave][16 * t + n16][0] = w.lref[t];
-            sml[wave][16 * t + n16][1] = w.l[t];
-        }
+        if (grp == 0) sml[wave][16 * t + n16] = {w.base[t], w.lref[t], w.l[t]};
         const Norm norm(w.top[t], w.lref[t], w.l[t]);
 #pragma unroll
         for (int i = 0; i < MD; ++i) *(f32x4*)&sm[wave][16 * t + n16][16 * i + 4 * grp] = norm(w.o[t][i]);
@@ -607,12 +659,12 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
     for (int x = threadIdx.x; x < 16 * NT * (D / 4); x += 256) {
         const int r = x / (D / 4), d = 4 * (x - r * (D / 4));
         if (row0 + r >= rowsAll) break;
-        float M = -INFINITY;
+        Part M = sml[0][r];
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) M = fmaxf(M, sml[v][r][0]);
+        for (int v = 1; v < kWaves; ++v) M.raise(sml[v][r]);
         float L = 0.f, wt[kWaves];
 #pragma unroll
-        for (int v = 0; v < kWaves; ++v) L += wt[v] = weight(sml[v][r][0], sml[v][r][1], M);
+        for (int v = 0; v < kWaves; ++v) L += wt[v] = sml[v][r].weight(M);
         const float inv = L == 0.f ? 0.f : 1.f / L;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -625,12 +677,12 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
         if (it.slot >= 0) {
             const int64_t pr = (int64_t)(it.slot + it.c) * ROWS + r;
             *(f32x4*)(s.partO + pr * D + d) = O;
-            if (d == 0) s.partML[pr] = make_float2(M, L);
+            if (d == 0) s.partML[pr] = make_float4(M.base, M.ref, L, 0.f);
         } else {
             const int qi = (row0 + r) / G, g = (row0 + r) - qi * G;
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
             store4(op, O, a.type);
-            if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
+            if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M.base, M.ref, L);
         }
     }
 }
@@ -804,71 +856,75 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
             const int row = it.rt * s.rows + r;
             if (row >= it.nq * G) return;
             const int64_t at = (int64_t)it.slot * s.rows + r;
-            float2 x[8];
+            Part x[8];
             f32x4 v[8];
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
                 const int64_t p = at + (int64_t)min(c, it.n - 1) * s.rows;
-                x[c] = s.partML[p];
+                const float4 ml = s.partML[p];
+                x[c] = {ml.x, ml.y, ml.z};
                 v[c] = *(const f32x4*)(s.partO + p * D + d);
             }
-            float M = -INFINITY, L = 0.f;
+            Part M = x[0];
 #pragma unroll
-            for (int c = 0; c < 8; ++c) M = c < it.n ? fmaxf(M, x[c].x) : M;
+            for (int c = 1; c < 8; ++c) M.raise(x[c]); // (those behind the last are the last)
+            float L = 0.f;
 #pragma unroll
-            for (int c = 0; c < 8; ++c) L += x[c].y = c < it.n ? weight(x[c].x, x[c].y, M) : 0.f;
+            for (int c = 0; c < 8; ++c) L += x[c].l = c < it.n ? x[c].weight(M) : 0.f;
             const float inv = L == 0.f ? 0.f : 1.f / L;
             f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 8; ++c)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) O[j] = __builtin_fmaf(x[c].y * inv, v[c][j], O[j]);
+                for (int j = 0; j < 4; ++j) O[j] = __builtin_fmaf(x[c].l * inv, v[c][j], O[j]);
             const int qi = row / G, g = row - qi * G;
             unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
             store4(op, O, a.type);
-            if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
+            if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M.base, M.ref, L);
         }
         return;
     }
     __shared__ __align__(16) float so[256 * 4];
     __shared__ float wt[kMergeChunks];
-    __shared__ float red[2][4];
+    __shared__ Part redM[4];
+    __shared__ float red[4];
     for (int r = blockIdx.x % s.mergeRows; r < s.rows; r += s.mergeRows) {
         const int row = it.rt * s.rows + r;
         if (row >= it.nq * G) return;
         __syncthreads(); // (the row before has been joined)
-        const float2* ml = s.partML + (int64_t)it.slot * s.rows + r;
+        const float4* ml = s.partML + (int64_t)it.slot * s.rows + r;
+        auto part_of = [&](int c) {
+            const float4 x = ml[(int64_t)c * s.rows];
+            return Part{x.x, x.y, x.z};
+        };
         const float* po = s.partO + ((int64_t)it.slot * s.rows + r) * D;
-        const float2 mine = ml[(int64_t)min((int)threadIdx.x, it.n - 1) * s.rows]; // (one chunk a thread is what there mostly is)
-        float M = mine.x;
-        for (int c = threadIdx.x + 256; c < it.n; c += 256) M = fmaxf(M, ml[(int64_t)c * s.rows].x);
+        const Part mine = part_of(min((int)threadIdx.x, it.n - 1)); // (one chunk a thread is what there mostly is)
+        Part M = mine;
+        for (int c = threadIdx.x + 256; c < it.n; c += 256) M.raise(part_of(c));
 #pragma unroll
-        for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-        if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = M;
+        for (int o = 32; o; o >>= 1) M.raise({__shfl_xor(M.base, o, 64), __shfl_xor(M.ref, o, 64), 0.f});
+        if ((threadIdx.x & 63) == 0) redM[threadIdx.x >> 6] = M;
         __syncthreads();
-        M = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        M = redM[0];
+        for (int v = 1; v < 4; ++v) M.raise(redM[v]);
         float L = 0.f;
         for (int c = threadIdx.x; c < it.n; c += 256) {
-            const float2 x = c == (int)threadIdx.x ? mine : ml[(int64_t)c * s.rows];
-            const float f = weight(x.x, x.y, M);
+            const float f = (c == (int)threadIdx.x ? mine : part_of(c)).weight(M);
             if (c < kMergeChunks) wt[c] = f;
             L += f;
         }
 #pragma unroll
         for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, 64);
-        if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = L;
+        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = L;
         __syncthreads();
-        L = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+        L = red[0] + red[1] + red[2] + red[3];
         const float inv = L == 0.f ? 0.f : 1.f / L;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
         for (int c0 = 0; c0 < it.n; c0 += kMergeChunks) {
             const int n = min(it.n - c0, kMergeChunks);
             if (c0) {
                 __syncthreads();
-                for (int c = threadIdx.x; c < n; c += 256) {
-                    const float2 x = ml[(int64_t)(c0 + c) * s.rows];
-                    wt[c] = weight(x.x, x.y, M);
-                }
+                for (int c = threadIdx.x; c < n; c += 256) wt[c] = part_of(c0 + c).weight(M);
                 __syncthreads();
             }
             if (part < parts) {
@@ -902,7 +958,7 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
         const int qi = row / G, g = row - qi * G;
         unsigned short* op = (unsigned short*)a.out + (int64_t)(it.q0 + qi) * a.outTokenStride + (int64_t)(it.h * G + g) * a.outHeadStride + d;
         store4(op, O, a.type);
-        if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M, L);
+        if (d == 0 && a.lse) a.lse[(int64_t)(it.q0 + qi) * a.heads + it.h * G + g] = log_sum(M.base, M.ref, L);
     }
 }
 
@@ -948,7 +1004,7 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         const int64_t groups = std::min<int64_t>(rowTiles * a.cache.numHeads, s.maxSlots / 2);
         s.mergeRows = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(s.rows, most), 2048 / std::max<int64_t>(groups, 1)));
         L.mergeGrid = s.merge ? groups * s.mergeRows : 0;
-        L.bytes = s.merge ? round_up((size_t)s.maxSlots * s.rows * D * 4, 256) + round_up((size_t)s.maxSlots * s.rows * 8, 256) : 0;
+        L.bytes = s.merge ? round_up((size_t)s.maxSlots * s.rows * D * 4, 256) + round_up((size_t)s.maxSlots * s.rows * 16, 256) : 0;
         s.partO = nullptr;
         s.partML = nullptr;
     };
@@ -1015,7 +1071,7 @@ void launch_cache_attend(const AttendArgs& a, int num_cus, hipStream_t stream) {
         Sched& s = L[i].s;
         if (s.merge) {
             s.partO = (float*)ws;
-            s.partML = (float2*)(ws + round_up((size_t)s.maxSlots * s.rows * a.cache.headDim * 4, 256));
+            s.partML = (float4*)(ws + round_up((size_t)s.maxSlots * s.rows * a.cache.headDim * 4, 256));
             ws += L[i].bytes;
         }
         switch (a.cache.headDim) {

@@ -166,6 +166,49 @@ def test_attend_subnormal_scales(res, code):
                 check(got, lse, want, wl, tol, (code, nq, extra, tiles[0]))
 
 
+LARGE = {
+    "ties": [(5, 0.01), (3, 0.01), (5, 0.01), (-7, 0.01)],
+    "ties of other scales": [(5, 2.0 ** -9), (5, 2.0 ** 3), (-7, 2.0 ** 20), (5, 2.0 ** -12)] * 3,
+    "growing": [(-100 + 10 * i, 0.01 + 0.002 * i) for i in range(20)],
+    "falling": [(100 - 10 * i, 0.01 + 0.002 * i) for i in range(20)],
+    "all far below": [(-96, 0.01), (-112, 0.5), (-96, 0.25), (-120, 1.0)] * 2,
+    "zero values first": [(-64, 0.0)] * 4 + [(64, 0.5)] * 4 + [(-3, 2.0 ** 30)] * 4,
+    "zero values are largest": [(3, 0.5)] * 4 + [(64, 0.0)] * 8,
+}
+
+
+@pytest.mark.parametrize("name", list(LARGE))
+@pytest.mark.parametrize("k", [0, 4, 8, 11, 12, 13, 16, 20, 24, 27, 30, 48, 90])
+def test_attend_large_scores(res, name, k):
+    """Scores far from zero, up to 2^97: their differences count, not their size.  The scores are small integers times 2^k (times ln 2
+    log2 e, which rounds them all by the same factor): from k = 8 on equal ones share the probability, all others have none"""
+    for nq in (1, 40):
+        for extra in (2, 60):
+            c, table, n = stepped(res, "int8", LARGE[name], extra=extra)
+            q = torch.zeros((nq, 2, 64), device="cuda").bfloat16()
+            q[:, 0, 0] = 2.0 ** k
+            q[:, 1, 0] = -(2.0 ** k)
+            got, lse = c.attend(q, table, ints([n]), query_offsets=ints([0, nq]), scale=math.log(2), causal=False, return_lse=True)
+            pages = table[0, :n // 16].long()
+            v = (c.v_codes.double() * c.v_scales.double()[:, :, None, None]).transpose(2, 3)[pages, 0].reshape(-1, 64)
+            each = c.v_scales.double()[pages, 0].repeat_interleave(16)
+            for head, sign in ((0, 1), (1, -1)):
+                z = c.k_codes.double()[pages, 0, :, 0].reshape(-1) * 2.0 ** k * sign
+                m = z.max()
+                p = torch.exp2(z - m)
+                # fp16 probabilities (and those that vanish), sums in fp32, the result's rounding; the factor that all scores are
+                # rounded by (two roundings, the guard of the reference) where they are not equal
+                gap = (m - z)[(z < m) & (z > m - 200)]
+                f = 2 ** -11 + (n / 16 + 300) * 2 ** -24 + 2 * (float(gap.max()) if gap.numel() else 0.0) * 2 ** -22
+                big, low = p @ v.abs() / p.sum(), 2 ** -31 * (p * each).max() * 127 * n / p.sum()
+                want = p @ v / p.sum()
+                tol = (f * big + low) * 1.01 + 2 ** -8 * want.abs() + 2 ** -120
+                bad = ~((got[:, head].double() - want).abs() <= tol)
+                assert not bad.any(), (nq, extra, head, float((got[:, head].double() - want).abs().max()))
+                wl = float((m + p.sum().log2()) * math.log(2))
+                assert float((lse[:, head].double() - wl).abs().max()) <= 2 ** -11 + abs(wl) * 2 ** -21
+
+
 # ------------------------------------------------------------------------------------------------ lengths and batches
 @pytest.mark.parametrize("code, bs, hq, length, nq, cols", [
     ("e4m3", 16, 2, 1000, 10, 62), ("int8", 16, 2, 1000, 300, 53), ("e4m3", 16, 1, 1000, 300, 52), ("int8", 64, 2, 5000, 200, 77),
