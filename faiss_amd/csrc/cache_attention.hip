@@ -321,7 +321,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sc[t][i][e] = __builtin_fmaf(sc[t][i][e], f[t], -w.base[t]);
+                for (int e = 0; e < 4; ++e) sc[t][i][e] = sc[t][i][e] * f[t] - w.base[t]; // (two roundings: the base is such a product)
             f[t] = 1.f;
         }
     }
@@ -352,7 +352,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
     }
     if (__ballot(change)) {
         // A reference is off by 2^-23 of itself, which from 2^13 on is felt in the probabilities and from 2^30 on takes them out of
-        // fp32.  Such a row's scores are counted from their largest so far instead: a difference of scores is one rounding
+        // fp32.  Such a row's scores are counted from their largest so far instead, as numbers of fp32
         bool far = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) far |= now[t] != w.top[t] && fabsf(now[t]) > kFar && fabsf(now[t]) < INFINITY;
@@ -366,7 +366,7 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) sc[t][i][e] = __builtin_fmaf(sc[t][i][e], f[t], -by);
+                    for (int e = 0; e < 4; ++e) sc[t][i][e] = sc[t][i][e] * f[t] - by;
                 f[t] = 1.f;
                 w.base[t] += by;
                 if (w.top[t] != kNothing) {

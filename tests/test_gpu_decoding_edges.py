@@ -209,6 +209,41 @@ def test_attend_large_scores(res, name, k):
                 assert float((lse[:, head].double() - wl).abs().max()) <= 2 ** -11 + abs(wl) * 2 ** -21
 
 
+@pytest.mark.parametrize("dt, power", [(torch.bfloat16, 8), (torch.bfloat16, 16), (torch.bfloat16, 23), (torch.bfloat16, 30), (torch.bfloat16, 60),
+                                       (torch.bfloat16, 100), (torch.float16, 8), (torch.float16, 13)])
+@pytest.mark.parametrize("code, lengths, nq", [("e4m3", [90, 700], 1), ("int8", [200, 90], 40), ("e4m3", [9000, 33], 1), ("int8", [20000, 9], 70)])
+def test_attend_large_queries(res, code, lengths, nq, dt, power):
+    """queries of any numbers times 2^power: a row takes its values from the token with the largest score wherever the next one's is
+    further below than the products' and sums' error, (d + 8) 2^-24 sum |q_d k_d|, and 40 units of log 2 tell"""
+    c, table = paged(res, lengths, 16, 1, 64, code, 5)
+    if code == "int8" and dt == torch.float16:
+        c.k_scales.mul_(2.0 ** 10)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(power)
+    q = (torch.randn((2 * nq, 2, 64), generator=g, device="cuda") * 2.0 ** power).to(dt)
+    got, lse = c.attend(q, table, ints(lengths), query_offsets=ints([0, nq, 2 * nq]), causal=False, return_lse=True)
+    assert bool(torch.isfinite(got).all()) and bool(torch.isfinite(lse).all())
+    alone = 0
+    for b, n in enumerate(lengths):
+        pages = table[b, :-(-n // 16)].long()
+        k = (c.k_codes.double() * c.k_scales.double()[:, :, None, None])[pages, 0].reshape(-1, 64)[:n]
+        v = (c.v_codes.double() * c.v_scales.double()[:, :, None, None]).transpose(2, 3)[pages, 0].reshape(-1, 64)[:n]
+        x = q[b * nq:(b + 1) * nq].double().reshape(-1, 64)
+        z = x @ k.T / 8
+        error = (x.abs() @ k.abs().T / 8).amax(-1) * 72 * 2 ** -24
+        two, at = z.topk(2, -1)
+        clear = two[:, 0] - two[:, 1] > 2 * error + 40 * math.log(2)
+        alone += int(clear.sum())
+        want = v[at[:, 0]][clear]
+        out = got[b * nq:(b + 1) * nq].reshape(-1, 64).double()[clear]
+        # one probability of one (2^-40 of others), a value, the rounding of its fp16 product and of the result
+        assert bool(((out - want).abs() <= (2 ** -11 + 2 ** -20 + torch.finfo(dt).eps / 2) * want.abs() + 2 ** -20).all())
+        wl = lse[b * nq:(b + 1) * nq].reshape(-1).double()
+        assert bool(((wl - two[:, 0]).abs() <= error + math.log(n) + two[:, 0].abs() * 2 ** -22 + 2 ** -10).all())
+    if power >= 16:
+        assert alone > nq
+
+
 # ------------------------------------------------------------------------------------------------ lengths and batches
 @pytest.mark.parametrize("code, bs, hq, length, nq, cols", [
     ("e4m3", 16, 2, 1000, 10, 62), ("int8", 16, 2, 1000, 300, 53), ("e4m3", 16, 1, 1000, 300, 52), ("int8", 64, 2, 5000, 200, 77),
