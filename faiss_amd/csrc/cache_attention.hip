@@ -512,6 +512,8 @@ struct Part {
     }
     __device__ __forceinline__ float weight(const Part& most) const { return l * __builtin_amdgcn_exp2f(above(most)); }
 };
+// A sum of zero is that of a row that sees nothing, or of one all of whose scores are -inf (an infinite query): that one is NaN
+__device__ __forceinline__ float sum_seen(float l, int sees) { return l == 0.f && sees > 0 ? __builtin_nanf("") : l; }
 // a row of a wavefront's own: the result, or a chunk's partial sums
 template <int D, int NT, int MD>
 __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, const Item& it, int G, int row0, int rowsAll, Rows<NT, MD>& w) {
@@ -520,6 +522,7 @@ __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, 
     for (int t = 0; t < NT; ++t) {
         const int r = row0 + 16 * t + n16;
         if (r >= rowsAll) continue;
+        if (it.slot < 0) w.l[t] = sum_seen(w.l[t], visible(a, it, G, r));
         const Norm norm(w.top[t], w.lref[t], w.l[t]);
         if (it.slot >= 0) {
             const int64_t pr = (int64_t)(it.slot + it.c) * s.rows + (r - it.rt * s.rows);
@@ -665,6 +668,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
         float L = 0.f, wt[kWaves];
 #pragma unroll
         for (int v = 0; v < kWaves; ++v) L += wt[v] = sml[v][r].weight(M);
+        if (it.slot < 0) L = sum_seen(L, visible(a, it, G, row0 + r));
         const float inv = L == 0.f ? 0.f : 1.f / L;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -871,6 +875,7 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
             float L = 0.f;
 #pragma unroll
             for (int c = 0; c < 8; ++c) L += x[c].l = c < it.n ? x[c].weight(M) : 0.f;
+            L = sum_seen(L, visible(a, it, G, row));
             const float inv = L == 0.f ? 0.f : 1.f / L;
             f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -917,7 +922,7 @@ __global__ __launch_bounds__(256) void cache_attend_merge_kernel(AttendArgs a, S
         for (int o = 32; o; o >>= 1) L += __shfl_xor(L, o, 64);
         if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = L;
         __syncthreads();
-        L = red[0] + red[1] + red[2] + red[3];
+        L = sum_seen(red[0] + red[1] + red[2] + red[3], visible(a, it, G, row));
         const float inv = L == 0.f ? 0.f : 1.f / L;
         f32x4 O = {0.f, 0.f, 0.f, 0.f};
         for (int c0 = 0; c0 < it.n; c0 += kMergeChunks) {

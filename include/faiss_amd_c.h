@@ -547,7 +547,8 @@ int faiss_amd_PagedCache_reconstruct(FaissAmdGpuResources* res, const FaissAmdPa
  * causal, all `length` tokens otherwise.  A row that sees nothing is zero (lse -inf); rows of no request are left as they
  * are.  A row that sees a block id out of range (or tokens behind the table's last column), a block
  * whose scale is negative or no number or infinite, or a NaN code is NaN as a whole (its lse too); a row that masks them is not.
- * Values whose scale is zero are zero whatever their codes.
+ * Values whose scale is zero are zero whatever their codes.  Infinite queries make NaN where softmax does: scores that are
+ * all -inf, or one of +inf.
  * Value scales more than 2^100 below a head's largest count as 2^100 below it.  lse (nullable)
  * [tokens][heads]: log sum_j p_j.  q / out: F16 or BF16, strides in elements, the last dimension dense.  maxQueries: an upper
  * bound of a request's queries; a smaller one costs time, not results.  workspace (may be NULL when its size is 0): at least

@@ -244,6 +244,31 @@ def test_attend_large_queries(res, code, lengths, nq, dt, power):
         assert alone > nq
 
 
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("nq, cols", [(3, None), (3, 200), (3, 2000), (50, None), (50, 200)])
+def test_attend_infinite_queries(res, dt, nq, cols):
+    """the softmax of scores that are all -inf, or of which one is +inf, is no number; rows that see nothing are zero"""
+    length = 2 if cols is None else 1500 if cols == 200 else 30000
+    c, table = paged(res, [length], 16, 1, 64, "int8", 1)
+    if cols:
+        wide = torch.full((1, cols), -1, dtype=I32, device="cuda")
+        wide[:, :table.shape[1]] = table
+        table = wide
+    c.k_codes[..., 0] = 5
+    c.k_codes[int(table[0, 0]), 0, 1, 1] = -3
+    c.k_codes[int(table[0, 0]), 0, 0, 1] = 3
+    for value, at in ((-math.inf, 0), (math.inf, 0), (-math.inf, 1)):
+        q = torch.randn((nq, 2, 64), device="cuda").to(dt)
+        clean = q.clone()
+        q[:, 1, at] = value
+        got, lse = c.attend(q, table, ints([length]), query_offsets=ints([0, nq]), return_lse=True)
+        want, wl, tol = reference(c, clean, table, [length], [0, nq], 1 / 8, True)
+        sees = torch.arange(nq) + length - nq + 1 > 0
+        assert bool(got[sees][:, 1].isnan().all()) and bool(lse[sees][:, 1].isnan().all())
+        assert bool((got[~sees] == 0).all()) and bool((lse[~sees] == -math.inf).all())
+        check(got[:, 0], lse[:, 0], want[:, 0], wl[:, 0], tol[:, 0])
+
+
 # ------------------------------------------------------------------------------------------------ lengths and batches
 @pytest.mark.parametrize("code, bs, hq, length, nq, cols", [
     ("e4m3", 16, 2, 1000, 10, 62), ("int8", 16, 2, 1000, 300, 53), ("e4m3", 16, 1, 1000, 300, 52), ("int8", 64, 2, 5000, 200, 77),
