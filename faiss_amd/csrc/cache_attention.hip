@@ -544,8 +544,9 @@ __device__ __forceinline__ void write_rows(const AttendArgs& a, const Sched& s, 
 // LDS.  A tile's values are asked for before its scores are computed and the next tile's keys before its softmax; what a wait would
 // hold up is looked up beforehand (Stretch).
 // 64 ragged contexts of up to 16384 tokens, 8 heads of 128, e4m3 (1.34 GB): 263 us, 5.1 TB/s, as fast as a large copy; 3 of 131071,
-// one head of 256, int8 (0.2 GB): 48 us, 4.2 TB/s (358 registers: one wavefront per SIMD); 1 of 1000: 12 us, a chain of dependent
-// loads (lengths, blocks, scales, keys, values).
+// one head of 256, int8 (0.2 GB): 50 us, 4.0 TB/s (367 registers: one wavefront per SIMD); 1 of 1000: 12 us, a chain of dependent
+// loads (lengths, blocks, scales, keys, values).  Drafts over the ragged contexts, 2 / 4 / 5 / 8 queries each, 4 heads to one: 259 / 268 / 277 /
+// 284 us a call (one: 252).
 template <int D, int CODE, int NT>
 __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16; // steps of the first product, row tiles of the second
@@ -694,10 +695,11 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 // Many rows (prompts): bound by the arithmetic.  Each of the WAVES wavefronts has rows of its own; a tile's keys and values are loaded
 // and widened to fp16 once for all of them and laid into LDS fragment by fragment, in the order in which the matrix instructions'
 // lanes read them (no bank conflicts on either side).  Two such buffers: the next tile is loaded while one is worked on.
-// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 574 us, 840 TFLOP/s.  The matrix
-// pipe is busy 35 % of the time: beside 64 matrix instructions a wavefront issues 277 other vector instructions per tile (37 of them
-// transcendental), and 246 registers leave two wavefronts per SIMD.  Half of the wavefronts half a tile behind the others: 620 us;
-// the next tile's products between the softmax's instructions: it spills.  Ragged prompts: 354 us, straight from memory, as above, 745.
+// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 563 us, 856 TFLOP/s.  The matrix
+// pipe is busy 35 % of the time: beside 64 matrix instructions a wavefront issues 265 other vector instructions per tile (34 of them
+// transcendental), and 250 registers leave two wavefronts per SIMD.  Half of the wavefronts half a tile behind the others (before the last
+// steps, which took 595 to 574) 620; the next tile's products between the softmax's instructions: it spills.  Ragged prompts: 356 us, of which
+// the longest work item alone takes some 330 (256 rows that see 8192 tokens, at what a CU does here); straight from memory, as above, 745.
 template <int D, int CODE, int NT, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, 2) void cache_attend_rows_kernel(AttendArgs a, Sched s) {
     constexpr int KS = D / 32, MD = D / 16;
@@ -997,7 +999,9 @@ int plan_launches(const AttendArgs& a, int num_cus, Launch out[2]) {
         s.sort = waves != 0;
         const int64_t rowTiles = std::min(((int64_t)a.tokens * G + s.rows - 1) / s.rows + a.batch, (int64_t)a.batch * ((s.rowHi + (int64_t)s.rows - 1) / s.rows));
         const int64_t tiles = ((int64_t)a.cols * a.cache.blockSize + kTile) / kTile;
-        // a split costs a launch to join it (4 us), a tile of a wavefront 1 us: contexts of up to 16 tiles are not split
+        // a split costs a launch to join it (4 us), a tile of a wavefront 1 us: where the table holds no more than 16 tiles nothing is
+        // split.  What the host can go by is the table's width, not the lengths: 1000 tokens take 11.9 us through a table of 63 blocks of
+        // 16, 13.3 through one of 512 (split, joined), 50 tokens 7.8 and 9.7 (a join that finds nothing)
         s.minTiles = waves || tiles > 16 ? 8 : 16;
         s.wshift = 0;
         while (((rowTiles * tiles) >> s.wshift) + a.batch > (int64_t)1 << 30) ++s.wshift;

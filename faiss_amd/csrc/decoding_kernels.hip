@@ -26,7 +26,8 @@ __device__ __forceinline__ int lanes_before(unsigned long long mask) {
 // the granted requests that add tokens are a prefix of those that ask, and where a request's blocks and slots begin is an
 // exclusive prefix sum: one pass.  Free blocks wait in a ring: taken from its front, returned behind its end -- the two ranges
 // cannot meet (all blocks together fit the ring), so nothing has to be ordered between requests.  256 requests, a token each: 8 us
-// in one workgroup, a chain of dependent loads; 64 prompts over 384003 slots: 5.6 + 7 us.
+// in one workgroup, a chain of dependent loads, 1000 in 11.5; 64 prompts over 384003 slots: 6 + 7 us.  Through the general kernels
+// 1025 requests take 32 us, 1500 36, 8000 124: a workgroup goes through them 1024 at a time.
 constexpr int kPlanThreads = 1024;
 
 struct PlanScratch { // per request
@@ -410,12 +411,12 @@ __global__ __launch_bounds__(256) void add_blocks_kernel(AddArgs a) {
 // blockIdx.y: the keys or the values of a head.  A workgroup of few tokens (LISTED false) looks at token blockIdx.x: where its block
 // differs from its predecessor's it scans the call's slots for all tokens of that block: if none comes earlier it serves them (a
 // block's tokens may stand anywhere in the call; of several tokens for one slot the last wins), else another workgroup does.  Many
-// tokens would be scanned too often (131072 tokens in blocks of 64: 1078 us): for them the blocks are listed first, and a
+// tokens would be scanned too often (65536 tokens in blocks of 64: 8.6 ms): for them the blocks are listed first, and a
 // workgroup takes every gridDim.x-th, and scans from its first token to its last.
 // Keys are written as 8 dimensions of a token, values as 4 tokens of 8 dimensions: 4 x 4 bytes are transposed in registers, so
-// that both layouts get words.  16384 tokens of 8 x 128, int8, blocks of 64: 32 us with the list (100 MB, 20 us at the rate of a
-// copy), 65536: 109 us; 256 tokens of as many blocks of 16: 8.5 us.  4096 tokens of as many blocks of 64 take 240 us: a value's code
-// is a byte in a line of its own.
+// that both layouts get words.  16384 tokens of 8 x 128, int8, blocks of 64: 33 us with the list (100 MB, 20 us at the rate of a
+// copy), 65536: 109 us; 256 tokens of as many blocks of 16: 8.5 us in a graph (9.7 under a tracer), of 64 18, of 128 26, 4096 tokens of
+// as many blocks of 64 240: a value's code is a byte in a line of its own.
 template <int CODE, bool VEC, int NT, bool LISTED>
 __global__ __launch_bounds__(NT) void cache_add_kernel(AddArgs a) {
     const CacheView& c = a.cache;
@@ -633,8 +634,8 @@ __global__ __launch_bounds__(256) void cache_reconstruct_kernel(ReconstructArgs 
 // compared as 64-bit values.  Measured, a log-sum is off by 1e-8 where logits are spread (128001 of them, 3e-8 at 1000) and by up
 // to 8e-8 where one dominates (all sixteen of a lane added in fp32, and lanes joined by fp32 exponentials: 6e-8 and 9e-7, in the
 // same time); beams whose values are closer than that may change places.
-// 512 rows of 128001 bf16 logits, 16 kept: 43 us (131 MB, 3.0 TB/s) and 9 us for the join; 4 rows of 32000:
-// 7.9 + 5.1 us.  13 vector instructions per logit keep the SIMDs busy for half of the time; neither they nor the memory are full.
+// 512 rows of 128001 bf16 logits, 16 kept: 44 us (131 MB, 3.0 TB/s) and 9 us for the join; 4 rows of 32000:
+// 8 + 5 us.  13.5 vector instructions per logit keep the SIMDs busy for half of the time; neither they nor the memory are full.
 constexpr int kBeamVpt = 16;                                   // logits per lane and step
 constexpr int kBeamPend = 128;                                 // keys a wavefront collects before it cuts them to `keep`
 constexpr int kBeamCap = kBeamPend + 64 * kBeamVpt / 2;        // keys a wavefront may hold at once

@@ -543,14 +543,15 @@ int faiss_amd_PagedCache_reconstruct(FaissAmdGpuResources* res, const FaissAmdPa
 
 /* Attention: out[r][h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q[r][h] . k_j), query head h over key-value head
  * h / (heads / numHeads).  Request b's queries are the rows queryOffsets[b] ... queryOffsets[b + 1] - 1 (NULL: row b; offsets
- * must not decrease and are clamped to `tokens`); they are its last ones: query i of n sees the tokens j <= length - n + i if
+ * are clamped to `tokens`; they must not decrease, or rows hold anything); they are its last ones: query i of n sees the tokens j <= length - n + i if
  * causal, all `length` tokens otherwise.  A row that sees nothing is zero (lse -inf); rows of no request are left as they
  * are.  A row that sees a block id out of range (or tokens behind the table's last column), a block
  * whose scale is negative or no number or infinite, or a NaN code is NaN as a whole (its lse too); a row that masks them is not.
  * Values whose scale is zero are zero whatever their codes.  Infinite queries make NaN where softmax does: scores that are
  * all -inf, or one of +inf.
- * Value scales more than 2^100 below a head's largest count as 2^100 below it.  lse (nullable)
- * [tokens][heads]: log sum_j p_j.  q / out: F16 or BF16, strides in elements, the last dimension dense.  maxQueries: an upper
+ * Value scales more than 2^100 below the largest that a row has met count as 2^100 below it.  lse (nullable)
+ * [tokens][heads]: log sum_j p_j.  q / out: F16 or BF16, strides in elements, the last dimension dense; out may be q with the same
+ * strides, and its rows must not overlap otherwise.  maxQueries: an upper
  * bound of a request's queries; a smaller one costs time, not results.  workspace (may be NULL when its size is 0): at least
  * faiss_amd_PagedCache_attend_workspace bytes, 256-byte aligned. */
 typedef struct FaissAmdAttendParams {
@@ -575,8 +576,8 @@ int faiss_amd_PagedCache_attend_workspace(FaissAmdGpuResources* res, const Faiss
  * elements, the last dimension dense; finished (nullable, bytes [batch][beams]): such a beam's only candidate is (w, padToken)
  * with the value scores[b][w].  Candidates of probability zero or without a number (a row with NaN or +inf) are none; where
  * fewer than `keep` remain, score -inf, parent -1, token -1.  beams, keep <= 64.  Outputs [batch][keep].
- * Within a beam the order is that of the logits, exactly.  Between beams it is that of the values as computed: exponentials are
- * fp32, their sum fp64, which leaves a log-sum off by 1e-8 ... 1e-7 (2^-17 if all roundings went the same way). */
+ * Values are compared in fp64.  The log-sum that a beam's candidates share is of fp32 exponentials added in fp64: off by 1e-8 ... 1e-7
+ * (2^-17 if all roundings went the same way), and candidates of different beams that are closer may change places. */
 typedef struct FaissAmdBeamSelectParams {
     const void* logits;
     int64_t batchStride, beamStride;
