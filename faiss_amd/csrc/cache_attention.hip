@@ -326,9 +326,9 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
         }
     }
     const float vnew = fmaxf(w.vref, groups_max(lvs));
-    // the exponent of the lane's value scale: where there is none the probability is needed for the sum alone, and 2^-100 of the
-    // largest is as good as less
-    const float lv = lvs == kNoScale ? vnew : fmaxf(lvs, vnew - 100.f), iv = __builtin_amdgcn_exp2f(vnew - lv);
+    // the exponent of the lane's value scale: where there is none the probability is needed for the sum alone, and is not to raise
+    // the reference above the products that count
+    const float lv = fmaxf(lvs, vnew - 100.f), iv = __builtin_amdgcn_exp2f(vnew - lv);
     auto lane_max = [&](int t) {
         float mx = highest(sc[t][0][0], sc[t][0][1]);
 #pragma unroll

@@ -166,6 +166,31 @@ def test_attend_subnormal_scales(res, code):
                 check(got, lse, want, wl, tol, (code, nq, extra, tiles[0]))
 
 
+@pytest.mark.parametrize("code", ["e4m3", "int8"])
+@pytest.mark.parametrize("dim, bs", [(64, 16), (128, 32)])
+def test_attend_zero_values_with_most_of_the_probability(res, code, dim, bs):
+    """tokens whose values have the scale zero take up to all but 2^-40 of the probability; the others' products keep their digits"""
+    for nq in (1, 8, 60, 150):
+        for length, cols in ((131, 0), (700, 0), (5000, 400)):
+            c, table = paged(res, [length], bs, 1, dim, code, 3)
+            table = torch.cat([table, torch.full((1, cols), -1, dtype=I32, device="cuda")], 1)
+            some = table[0, 1:length // bs:3].long()
+            g = torch.Generator(device="cuda")
+            g.manual_seed(length + nq)
+            q = torch.randn((nq, 2, dim), generator=g, device="cuda").bfloat16()
+            for log2 in (4, 12, 20, 30, 40):
+                # an element of the queries that the zero-valued blocks' keys meet, and no others
+                c.k_codes.view(torch.uint8)[..., 0] = 0
+                c.k_codes[some, 0, :, 0] = torch.tensor(8.0, device="cuda").to(c.k_codes.dtype)
+                c.k_scales[some] = 2.0 ** -4
+                c.v_scales[some] = 0.0
+                q[:, :, 0] = log2 * math.log(2) / 0.5 * math.sqrt(dim)
+                for causal in (True, False):
+                    got, lse = c.attend(q, table, ints([length]), query_offsets=ints([0, nq]), causal=causal, return_lse=True)
+                    want, wl, tol = reference(c, q, table, [length], [0, nq], 1 / math.sqrt(dim), causal)
+                    check(got, lse, want, wl, tol, (nq, length, log2, causal))
+
+
 LARGE = {
     "ties": [(5, 0.01), (3, 0.01), (5, 0.01), (-7, 0.01)],
     "ties of other scales": [(5, 2.0 ** -9), (5, 2.0 ** 3), (-7, 2.0 ** 20), (5, 2.0 ** -12)] * 3,
