@@ -351,8 +351,8 @@ __device__ __forceinline__ void softmax_step(f32x4 (&sc)[NT][4], float ks, float
         change |= now[t] != w.top[t];
     }
     if (__ballot(change)) {
-        // A reference is off by 2^-23 of itself, which from 2^13 on is felt in the probabilities and from 2^30 on takes them out of
-        // fp32.  Such a row's scores are counted from their largest so far instead, as numbers of fp32
+        // A reference stands up to 2^-22 of itself above the largest score: the probabilities lose bits from 2^16 on and are zero from
+        // 2^27 on.  Such a row's scores are counted from their largest so far instead, as numbers of fp32
         bool far = false;
 #pragma unroll
         for (int t = 0; t < NT; ++t) far |= now[t] != w.top[t] && fabsf(now[t]) > kFar && fabsf(now[t]) < INFINITY;
@@ -695,7 +695,7 @@ __global__ __launch_bounds__(256) void cache_attend_direct_kernel(AttendArgs a, 
 // Many rows (prompts): bound by the arithmetic.  Each of the WAVES wavefronts has rows of its own; a tile's keys and values are loaded
 // and widened to fp16 once for all of them and laid into LDS fragment by fragment, in the order in which the matrix instructions'
 // lanes read them (no bank conflicts on either side).  Two such buffers: the next tile is loaded while one is worked on.
-// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 563 us, 856 TFLOP/s.  The matrix
+// Four requests of 2048 queries that end at token 8195, 16 heads over 4 of 128, e4m3: the call takes 563 - 569 us, 850 TFLOP/s.  The matrix
 // pipe is busy 35 % of the time: beside 64 matrix instructions a wavefront issues 265 other vector instructions per tile (34 of them
 // transcendental), and 250 registers leave two wavefronts per SIMD.  Half of the wavefronts half a tile behind the others (before the last
 // steps, which took 595 to 574) 620; the next tile's products between the softmax's instructions: it spills.  Ragged prompts: 356 us, of which
